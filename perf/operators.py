@@ -1,0 +1,424 @@
+"""The FP8 operators and the routing operator that are timed, each beside its plain form.
+
+A case names one call of one operator.  Its fields:
+
+    op      "quantise"  rows -> e4m3 codes and an f32 scale per row and 128 columns
+                        T, K, type; gather = copies of every row that are taken, in an expert-sorted order (0: the rows as they are)
+            "matmul"    codes [T,K] times a resident e4m3 weight [O,K] with an f32 scale per 128 x 128: T, K, O, type of the result
+            "route"     router logits [T,E] -> experts and weights of every token, and the rows they take in expert order
+                        k, score, type, groups, kept (groups a token may use), norm, scale, bias, padded (tokens that are none),
+                        closed (share of the experts that a token may not use)
+            "experts"   SwiGLU experts over expert-sorted rows of codes, both products in 8 bits: E, H, I, rows, zipf
+
+Weights, activations and logits are made on the GPU from the seed alone."""
+from __future__ import annotations
+
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+E4M3_MAX = 448.0
+MAX_FLOPS = 7.3e11         # the largest listed call
+MAX_WEIGHT_BYTES = 2.9e9
+MAX_ROW_VALUES = 32768 * 7168
+
+
+def listed() -> list[dict]:
+    return [
+        # activations of a decode step of eight conversations
+        dict(name="quantise_decode_8", op="quantise", T=8, K=2048, type="bf16", gather=0),
+        # the f32 residual rows of the ragged last chunk of a prompt
+        dict(name="quantise_chunk_709", op="quantise", T=709, K=7168, type="f32", gather=0),
+        # a prefill chunk whose rows are taken once for each of a token's eight experts
+        dict(name="quantise_gather_4096", op="quantise", T=4096, K=7168, type="bf16", gather=8),
+        # one token through a projection of a large layer: the weights are read once
+        dict(name="matmul_decode_1", op="matmul", T=1, K=7168, O=2048, type="bf16"),
+        # a prompt of odd length through a matrix whose sizes fill no tile
+        dict(name="matmul_odd_333", op="matmul", T=333, K=1000, O=1111, type="f32"),
+        # a prefill chunk through gate and up of a shared expert stored as one matrix
+        dict(name="matmul_prefill_4096", op="matmul", T=4096, K=7168, O=4096, type="bf16"),
+        # one token of a sigmoid router with a balance bias and group-limited choice
+        dict(name="route_decode_1", op="route", T=1, E=256, k=8, score="sigmoid", type="f32", groups=8, kept=4, norm=True,
+             scale=2.5, bias=0.01, padded=0, closed=0.0),
+        # a prompt on a softmax router that hands over bf16 logits
+        dict(name="route_prompt_512", op="route", T=512, E=128, k=8, score="softmax", type="bf16", groups=1, kept=1, norm=False,
+             scale=1.0, bias=0.0, padded=0, closed=0.0),
+        # many prompts at once, padded to a common length
+        dict(name="route_batch_16384", op="route", T=16384, E=384, k=8, score="softmax", type="f32", groups=1, kept=1, norm=True,
+             scale=1.0, bias=0.0, padded=300, closed=0.0),
+        # eight tokens decoded together: most experts that are touched have a row or two
+        dict(name="experts_decode_64", op="experts", E=128, H=2048, I=768, rows=64, zipf=0.0),
+        # a prompt of 512 tokens, eight experts each
+        dict(name="experts_prefill_4096", op="experts", E=128, H=2048, I=768, rows=4096, zipf=0.0),
+        # one of four ranks of a large layer: its share of the experts and of the rows, popularity skewed
+        dict(name="experts_large_8192", op="experts", E=64, H=7168, I=2048, rows=8192, zipf=0.6),
+    ]
+
+
+def _log_uniform(rng: random.Random, lo: int, hi: int) -> int:
+    return max(lo, min(hi, int(math.exp(rng.uniform(math.log(lo), math.log(hi + 1))))))
+
+
+def draw(rng: random.Random) -> dict:
+    """A call of the same ranges: one row to 16384 tokens, matrices up to the large layer's, odd sizes among them."""
+    while True:
+        op = rng.choice(["quantise", "matmul", "matmul", "route", "experts", "experts"])
+        if op == "quantise":
+            gather = rng.choice([0, 0, 4, 8])
+            case = dict(op=op, T=_log_uniform(rng, 1, 16384), K=_log_uniform(rng, 64, 7168), type=rng.choice(list(TYPES)), gather=gather)
+            if case["T"] * max(1, gather) * case["K"] > MAX_ROW_VALUES:
+                continue
+        elif op == "matmul":
+            K, O = _log_uniform(rng, 128, 7168), _log_uniform(rng, 128, 7168)
+            if rng.random() < 0.5:
+                K, O = K // 128 * 128, O // 128 * 128
+            case = dict(op=op, T=_log_uniform(rng, 1, 16384), K=K, O=O, type=rng.choice(list(TYPES)))
+        elif op == "route":
+            groups = rng.choice([1, 1, 4, 8])
+            E = max(groups, _log_uniform(rng, 8, 512) // groups * groups)
+            kept = max(1, groups // 2)
+            T = _log_uniform(rng, 1, 16384)
+            case = dict(op=op, T=T, E=E, k=rng.randint(1, min(8, E // groups * kept)), score=rng.choice(["softmax", "sigmoid"]),
+                        type=rng.choice(list(TYPES)), groups=groups, kept=kept, norm=rng.random() < 0.5, scale=rng.choice([1.0, 2.5]),
+                        bias=rng.choice([0.0, 0.01]), padded=rng.choice([0, T // 10]), closed=rng.choice([0.0, 0.0, 0.2]))
+        else:
+            H, I = _log_uniform(rng, 512, 7168) // 8 * 8, _log_uniform(rng, 256, 2048) // 8 * 8
+            if rng.random() < 0.5:
+                H, I = H // 128 * 128, I // 128 * 128
+            case = dict(op=op, E=_log_uniform(rng, 4, 128), H=H, I=I, rows=_log_uniform(rng, 1, 32768), zipf=rng.choice([0.0, 0.6, 1.2]))
+            if 3 * case["E"] * H * I > MAX_WEIGHT_BYTES or case["rows"] * H > MAX_ROW_VALUES:
+                continue
+        if work(case)["flops"] > MAX_FLOPS:
+            continue
+        return case
+
+
+# ---- what a user's program has in hand ---------------------------------------------------------------------
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+def _activations(T: int, K: int, gen: torch.Generator) -> torch.Tensor:
+    """Rows behind a norm: about N(0,1), a few channels ten times as large."""
+    channel = torch.where(torch.rand(K, device="cuda", generator=gen) < 0.01, 10.0, 1.0)
+    return torch.randn((T, K), device="cuda", generator=gen) * channel
+
+
+def _row_codes(x: torch.Tensor):
+    """f32 rows -> (codes as float8, scales f32 [T, blocks]): the definition of the row quantiser in f32."""
+    T, K = x.shape
+    B = _blocks(K)
+    if K % 128:
+        x = torch.nn.functional.pad(x, (0, B * 128 - K))
+    x = x.view(T, B, 128)
+    a = torch.nan_to_num(x, nan=0.0, posinf=math.inf, neginf=-math.inf).abs().amax(2)
+    s = torch.where(a > 0, (a / E4M3_MAX).clamp_min(2.0**-126), 1.0)
+    q = (x / s[:, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return q.view(torch.uint8).view(T, B * 128)[:, :K].view(torch.float8_e4m3fn), s
+
+
+def _weight(O: int, K: int, gen: torch.Generator):
+    """One matrix of a checkpoint: e4m3 codes [O,K] and an f32 scale per 128 x 128."""
+    Ob, Kb = _blocks(O), _blocks(K)
+    w = torch.zeros((Ob * 128, Kb * 128), device="cuda")
+    w[:O, :K].normal_(0.0, 0.02, generator=gen)
+    w = w.view(Ob, 128, Kb, 128)
+    s = w.abs().amax((1, 3)) / E4M3_MAX
+    q = (w / s[:, None, :, None]).clamp_(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn).view(torch.uint8)
+    return q.view(Ob * 128, Kb * 128)[:O, :K].contiguous().view(torch.float8_e4m3fn), s
+
+
+def _counts(rows: int, E: int, zipf: float, seed: int) -> list[int]:
+    """Rows per expert of `rows` pairs."""
+    r = np.random.RandomState(seed)
+    p = 1.0 / np.arange(1, E + 1) ** zipf
+    return r.multinomial(rows, r.permutation(p / p.sum())).tolist()
+
+
+def _padded_rows(codes: torch.Tensor) -> torch.Tensor:
+    """Codes in rows that start on 16 bytes, as the row quantiser leaves them."""
+    T, K = codes.shape
+    buf = torch.zeros((T, (K + 15) // 16 * 16), dtype=torch.uint8, device="cuda")
+    buf[:, :K] = codes.view(torch.uint8)
+    return buf[:, :K]
+
+
+def _by_block(s: torch.Tensor) -> torch.Tensor:
+    """Scales [T, blocks] with a block's scales next to each other, as the row quantiser leaves them."""
+    return s.t().contiguous().t()
+
+
+def prepare(case: dict, seed: int) -> dict:
+    gen = torch.Generator("cuda")
+    gen.manual_seed(seed)
+    st = dict(case)
+    op = case["op"]
+    if op == "quantise":
+        T, K = case["T"], case["K"]
+        st["x"] = _activations(T, K, gen).to(TYPES[case["type"]])
+        st["take"] = None
+        if case["gather"]:
+            st["take"] = torch.randperm(T * case["gather"], device="cuda", generator=gen).remainder(T).to(torch.int32)
+        if own:
+            R = T * max(1, case["gather"])
+            st["out"] = (torch.empty((R, (K + 15) // 16 * 16), dtype=torch.uint8, device="cuda")[:, :K],
+                         torch.empty((_blocks(K), R), device="cuda").t())
+    elif op == "matmul":
+        q, s = _row_codes(_activations(case["T"], case["K"], gen))
+        w, ws = _weight(case["O"], case["K"], gen)
+        st["q"], st["s"] = _padded_rows(q), _by_block(s)
+        if own:
+            st["w"] = _resident(w, ws)
+            st["y"] = torch.empty((case["T"], case["O"]), dtype=TYPES[case["type"]], device="cuda")
+        else:
+            st["w"], st["ws"] = w, ws
+    elif op == "route":
+        T, E = case["T"], case["E"]
+        logits = torch.randn((T, E), device="cuda", generator=gen)
+        if case["closed"]:
+            logits.masked_fill_(torch.rand((T, E), device="cuda", generator=gen) < case["closed"], -math.inf)
+        if case["padded"]:
+            logits[T - case["padded"]:] = -math.inf
+        st["logits"] = logits.to(TYPES[case["type"]])
+        st["bias"] = torch.randn(E, device="cuda", generator=gen) * case["bias"] if case["bias"] else None
+        if own:
+            new = lambda *n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+            st["out"] = (new(T, case["k"]), torch.empty((T, case["k"]), device="cuda"), new(E), new(T, case["k"]), new(T * case["k"]))
+    else:
+        E, H, I, rows = case["E"], case["H"], case["I"], case["rows"]
+        counts = _counts(rows, E, case["zipf"], seed)
+        st["counts"], st["seg"] = counts, torch.tensor(counts, dtype=torch.int32, device="cuda")
+        q, s = _row_codes(_activations(rows, H, gen))
+        st["q"], st["s"] = _padded_rows(q), _by_block(s)
+        weights = []
+        for _ in range(E):
+            one = [_weight(I, H, gen), _weight(I, H, gen), _weight(H, I, gen)]
+            weights.append([_resident(*m) for m in one] if own else one)
+        if own:
+            st["block"] = _expert_block(case, weights)
+            st["y"] = torch.empty((rows, H), dtype=torch.bfloat16, device="cuda")
+        else:
+            st["weights"] = weights
+    return st
+
+
+def _resident(codes: torch.Tensor, scales: torch.Tensor):
+    from speedycolibri_b200 import backend
+    from speedycolibri_b200.configs import FMT_FP8_B128
+
+    backend.init([0])
+    O, K = codes.shape
+    return backend.CudaTensor.from_device(FMT_FP8_B128, codes, scales, 1.0, K, O)
+
+
+def _expert_block(case: dict, weights):
+    from speedycolibri_b200.configs import FMT_FP8_B128
+    from speedycolibri_b200.moe import Config, Expert, Layer, MoeBlock
+
+    cfg = Config(case["H"], case["E"], 1, case["I"], fmt=FMT_FP8_B128)
+    layer = Layer(np.zeros((case["E"], case["H"]), np.uint16), [Expert(*w) for w in weights])
+    return MoeBlock(cfg, layer, case["rows"])
+
+
+# ---- one pass -------------------------------------------------------------------------------------------------
+def run(st: dict):
+    return (_run_own if own else _run_plain)(st)
+
+
+def _run_own(st: dict):
+    from speedycolibri_b200 import backend
+    from speedycolibri_b200.configs import SCORE_SIGMOID, SCORE_SOFTMAX
+
+    op = st["op"]
+    if op == "quantise":
+        codes, scales = backend.quantize_rows_fp8_dev(st["x"], st["take"], out=st["out"])
+        return codes.view(torch.float8_e4m3fn), scales
+    if op == "matmul":
+        return backend.matmul_fp8_dev(st["w"], st["q"], st["s"], out=st["y"])
+    if op == "route":
+        return tuple(backend.route_logits_dev(st["logits"], st["k"], SCORE_SOFTMAX if st["score"] == "softmax" else SCORE_SIGMOID,
+                                              select_bias=st["bias"], norm_topk=st["norm"], routed_scale=st["scale"],
+                                              n_group=st["groups"], topk_group=st["kept"], out=st["out"]))
+    st["block"].experts_fp8_dev(st["q"], st["s"], st["seg"], st["rows"], st["y"])
+    return st["y"]
+
+
+def _spread(s: torch.Tensor, K: int) -> torch.Tensor:
+    """Scales per block of the last axis -> per column."""
+    return s.repeat_interleave(128, 1)[:, :K]
+
+
+def _product(q: torch.Tensor, s: torch.Tensor, w: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
+    """Rows of codes times one weight, f32."""
+    K = w.shape[1]
+    a = q.float() * _spread(s, K)
+    b = w.float() * _spread(ws, K).repeat_interleave(128, 0)[: w.shape[0]]
+    return a @ b.t()
+
+
+def _run_plain(st: dict):
+    op = st["op"]
+    if op == "quantise":
+        x = st["x"] if st["take"] is None else st["x"][st["take"].long()]
+        return _row_codes(x.float())
+    if op == "matmul":
+        return _product(st["q"].view(torch.float8_e4m3fn), st["s"], st["w"], st["ws"]).to(TYPES[st["type"]])
+    if op == "route":
+        return _route_plain(st)
+    y = torch.empty((st["rows"], st["H"]), dtype=torch.bfloat16, device="cuda")
+    at = 0
+    for n, (gate, up, down) in zip(st["counts"], st["weights"]):
+        if n:
+            q, s = st["q"][at : at + n].view(torch.float8_e4m3fn), st["s"][at : at + n]
+            g, u = _product(q, s, *gate), _product(q, s, *up)
+            y[at : at + n] = _product(*_row_codes(g / (1.0 + torch.exp(-g)) * u), *down).to(torch.bfloat16)
+        at += n
+    return y
+
+
+def _route_plain(st: dict):
+    """Scores and keys in 64 bits: two experts may lie closer than 32 bits tell apart."""
+    z = st["logits"].double()
+    (T, E), k, G = z.shape, st["k"], st["groups"]
+    open_ = z > -math.inf
+    if st["score"] == "softmax":
+        top = z.amax(1, keepdim=True).nan_to_num(neginf=0.0)
+        e = torch.exp(z - top)
+        score = e / e.sum(1, keepdim=True).clamp_min(1e-300)
+    else:
+        score = 1.0 / (1.0 + torch.exp(-z))
+    key = score + st["bias"].double() if st["bias"] is not None else score
+    key = key.masked_fill(~open_, -math.inf)
+    if G > 1:
+        two = key.view(T, G, E // G).sort(dim=2, descending=True).values[:, :, :2]
+        best = two[:, :, 0] + two[:, :, 1:].clamp_min(-1e30).masked_fill(two[:, :, 1:] == -math.inf, 0.0).sum(2)
+        kept = best.sort(dim=1, descending=True, stable=True).indices[:, : st["kept"]]
+        use = torch.zeros((T, G), dtype=torch.bool, device=z.device).scatter_(1, kept, True)
+        key = key.masked_fill(~use.repeat_interleave(E // G, 1), -math.inf)
+    order = key.sort(dim=1, descending=True, stable=True)
+    idx, chosen = order.indices[:, :k], order.values[:, :k] > -math.inf
+    w = score.gather(1, idx).masked_fill(~chosen, 0.0)
+    if st["norm"]:
+        w = w / (w.sum(1, keepdim=True) + 1e-20)
+    idx = torch.where(chosen, idx, -1)
+    flat = torch.where(chosen, idx, E).reshape(-1)
+    rows = torch.bincount(flat, minlength=E + 1)[:E]
+    by_expert = flat.sort(stable=True).indices
+    slot = torch.empty_like(flat)
+    slot[by_expert] = torch.arange(T * k, device=z.device)
+    slot = torch.where(flat < E, slot, -1)
+    token = torch.where(torch.arange(T * k, device=z.device) < rows.sum(), by_expert // k, -1)
+    return (idx.int(), (w * st["scale"]).float(), rows.int(), slot.view(T, k).int(), token.int())
+
+
+# ---- work and the exact answers ---------------------------------------------------------------------------------
+def work(case: dict) -> dict:
+    size = {"bf16": 2, "f16": 2, "f32": 4}
+    op = case["op"]
+    if op == "quantise":
+        T, K = case["T"], case["K"]
+        R = T * max(1, case["gather"])
+        return {"bytes": T * K * size[case["type"]] + (4 * R if case["gather"] else 0) + R * (K + 4 * _blocks(K)), "flops": 2 * R * K}
+    if op == "matmul":
+        T, K, O = case["T"], case["K"], case["O"]
+        return {"bytes": T * (K + 4 * _blocks(K)) + O * K + 4 * _blocks(O) * _blocks(K) + T * O * size[case["type"]],
+                "flops": 2 * T * K * O}
+    if op == "route":
+        T, E, k = case["T"], case["E"], case["k"]
+        return {"bytes": T * E * size[case["type"]] + 16 * T * k + 4 * E, "flops": 4 * T * E}
+    E, H, I, rows = case["E"], case["H"], case["I"], case["rows"]
+    p = 1.0 / np.arange(1, E + 1) ** case["zipf"]
+    touched = float((1.0 - (1.0 - p / p.sum()) ** rows).sum())  # experts that have a row, on average
+    matrix = H * I + 4 * _blocks(H) * _blocks(I)
+    return {"bytes": touched * 3 * matrix + rows * (H + 4 * _blocks(H) + 2 * H), "flops": 6 * rows * H * I}
+
+
+def _to_e4m3(v: torch.Tensor) -> torch.Tensor:
+    """The nearest e4m3 value of each f64 value, ties to even, at most 448."""
+    a = v.abs().clamp_max(E4M3_MAX)
+    step = torch.exp2(torch.floor(torch.log2(a.clamp_min(2.0**-6))) - 3.0)
+    return torch.copysign((torch.round(a / step) * step).clamp_max(E4M3_MAX), v)
+
+
+def _exact_rows(x: torch.Tensor):
+    """f64 rows -> the values their codes stand for, and the scales, f64."""
+    parts, scales = [], []
+    for c in range(0, x.shape[1], 128):
+        b = x[:, c : c + 128]
+        s = b.abs().amax(1) / E4M3_MAX
+        s = torch.where(s > 0, s.clamp_min(2.0**-126), 1.0)
+        parts.append(_to_e4m3(b / s[:, None]))
+        scales.append(s)
+    return torch.cat(parts, 1), torch.stack(scales, 1)
+
+
+def _exact_product(rows: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
+    """sum over blocks of scale x scale x product of the codes, f64."""
+    y = torch.zeros((rows.shape[0], w.shape[0]), dtype=torch.float64, device=rows.device)
+    feature = torch.arange(w.shape[0], device=rows.device) // 128
+    for b in range(ws.shape[1]):
+        c = slice(128 * b, min(128 * (b + 1), w.shape[1]))
+        y += (rows[:, c] @ w[:, c].double().t()) * scales[:, b : b + 1].double() * ws[feature, b].double()
+    return y
+
+
+def exact(case: dict, seed: int):
+    global own
+    was, own = own, False
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    op = case["op"]
+    if op == "quantise":
+        x = st["x"].double()
+        return _exact_rows(x if st["take"] is None else x.index_select(0, st["take"].long()))
+    if op == "matmul":
+        return _exact_product(st["q"].view(torch.float8_e4m3fn).double(), st["s"], st["w"], st["ws"])
+    if op == "route":
+        return _exact_route(st)
+    out, at = [], 0
+    for n, (gate, up, down) in zip(st["counts"], st["weights"]):
+        q, s = st["q"][at : at + n].view(torch.float8_e4m3fn).double(), st["s"][at : at + n]
+        g = _exact_product(q, s, *gate)
+        out.append(_exact_product(*_exact_rows(g * torch.sigmoid(g) * _exact_product(q, s, *up)), *down))
+        at += n
+    return torch.cat(out)
+
+
+def _exact_route(st: dict):
+    """Token by token on the host; the whole numbers are compared with the plain form's and have no exact value here."""
+    z = st["logits"].double().cpu().numpy()
+    bias = st["bias"].double().cpu().numpy() if st["bias"] is not None else np.zeros(st["E"])
+    T, E, k, G = st["T"], st["E"], st["k"], st["groups"]
+    w = np.zeros((T, k))
+    for t in range(T):
+        free = [e for e in range(E) if z[t, e] > -math.inf]
+        if not free:
+            continue
+        if st["score"] == "softmax":
+            m = z[t, free].max()
+            p = np.exp(z[t] - m)
+            p = p / math.fsum(p)
+        else:
+            p = 1.0 / (1.0 + np.exp(-z[t]))
+        c = p + bias
+        if G > 1:
+            gs = E // G
+            marks = []
+            for g in range(G):
+                own_ = sorted((c[e] for e in free if e // gs == g), reverse=True)
+                if own_:
+                    marks.append((-sum(own_[:2]), g))
+            kept = {g for _, g in sorted(marks)[: st["kept"]]}
+            free = [e for e in free if e // gs in kept]
+        best = sorted(free, key=lambda e: (-c[e], e))[:k]
+        w[t, : len(best)] = p[best]
+    if st["norm"]:
+        w = w / (w.sum(1, keepdims=True) + 1e-20)
+    return (None, w * st["scale"], None, None, None)
