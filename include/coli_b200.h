@@ -35,6 +35,11 @@ extern "C" {
 #define COLI_FMT_MXFP4 6
 #define COLI_FMT_FP8_B128 8
 
+/* Element types of the device-pointer calls that take more than one. */
+#define COLI_TYPE_F32 0
+#define COLI_TYPE_F16 1
+#define COLI_TYPE_BF16 2
+
 /* Opaque, persistent HBM copy of one quantised matrix (backend_cuda.h:24). */
 typedef struct ColiCudaTensor ColiCudaTensor;
 
@@ -278,6 +283,16 @@ int coli_b200_moe_gather_local_dev(ColiMoe *moe, const void *x_dev, const int32_
  * 16-byte aligned (TMA reads the rows; the tcgen05 kernels write result rows 8 bytes at a time). */
 int coli_b200_moe_experts_dev(ColiMoe *moe, const void *rows_dev, const int32_t *seg_count_dev, int rows_cap,
                               int rows_expected, void *y_dev, void *stream);
+/* The same experts in 8-bit arithmetic (handles of format 8 only; the calls of "8-bit rows" below make
+ * the rows): codes_dev / scales_dev are expert-contiguous rows of H columns, seg_count_dev[n_local] the
+ * rows of each resident expert (counts that run past rows_cap are cut there).  h = act(gate x, up x) is
+ * quantised again, one scale per row and 128 features, by the rule of coli_b200_quantize_rows_fp8; both
+ * products are those of coli_b200_matmul_fp8_dev; y_dev is bf16 [rows, H] (16-byte aligned), written
+ * for the rows of the segments only: what lies behind the last one stays as it was.  rows_expected
+ * only selects how the work is cut, as above.  Uses the handle's workspace like the call above. */
+int coli_b200_moe_experts_fp8_dev(ColiMoe *moe, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row,
+                                  int64_t s_blk, const int32_t *seg_count_dev, int rows_cap, int rows_expected, void *y_dev,
+                                  void *stream);
 /* Shared expert over x_dev[T,H] -> y_dev[T,H] (bf16). */
 int coli_b200_moe_shared_dev(ColiMoe *moe, const void *x_dev, int T, void *y_dev, void *stream);
 /* partial[t] = sum over kk with slot >= 0 of w[t,kk] * y_rows[slot[t,kk]], kk ascending, f32 [T,H]
@@ -288,6 +303,34 @@ int coli_b200_moe_combine_partial_dev(ColiMoe *moe, const void *y_rows_dev, cons
 /* out[t] = bf16(partial[t] + shared_y[t]) (shared_y_dev may be NULL) — moe.rs:1875-1885. */
 int coli_b200_moe_finish_dev(ColiMoe *moe, const float *partial_dev, const void *shared_y_dev, void *out_dev, int T,
                              void *stream);
+
+/* ---- 8-bit rows: DEVICE pointers, asynchronous on `stream`, no handle, no workspace ----------------
+ * A matrix of rows in 8 bits is e4m3 codes [rows, K], `ld` bytes from row to row (a multiple of 16, at
+ * least K rounded up to 16; 16-byte aligned), and an f32 scale for each row and 128 columns, the scale
+ * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.
+ *
+ * Quantises rows x_dev of x_type (COLI_TYPE_*), x_stride elements apart: row r of the result is row r of
+ * x (rows <= T), or with row_token_dev [rows] row row_token_dev[r] of it; an entry outside [0,T) is no
+ * row, and its codes and scales are left as they were.  With a = the largest magnitude of the block's
+ * non-NaN values: scale = 1 if a == 0, else max(a / 448, 2^-126); code = e4m3(x / scale), to nearest
+ * even, saturating.  (The quotient is rounded once, where coli_b200_quantize_fp8_b128 multiplies by
+ * a rounded reciprocal.)  A NaN keeps a NaN code and an infinity makes its block's scale infinite, so that
+ * either shows in every product with the row.  Bytes K .. K rounded up to 16 of a row become zero. */
+int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_type, int64_t x_stride, const int32_t *row_token_dev,
+                                int T, int rows, int K, void *codes_dev, int64_t ld, float *scales_dev, int64_t s_row,
+                                int64_t s_blk, void *stream);
+/* y[r,o] = sum over blocks b of 128 columns of scale[r,b] * w_scale[o / 128, b] * (the product of the codes
+ * over the block): rows in 8 bits times a resident weight of format 8, y_dev [rows, O] of y_type, y_stride
+ * elements apart.  Products of codes are exact, sums are f32, each result is rounded once to y_type.  A
+ * weight code of 0x7F or 0xFF is a NaN here (the 16-bit expert calls read it as 480).  The same call gives
+ * the same bits; calls with another number of rows may share K among CTAs differently and differ in the
+ * last f32 bits. */
+int coli_b200_matmul_fp8_dev(const ColiCudaTensor *w, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row,
+                             int64_t s_blk, int rows, void *y_dev, int y_type, int64_t y_stride, void *stream);
+/* Synchronise the device and return 1 if every coli_b200_matmul_fp8_dev on it since the last check ran to
+ * completion, 0 (with an error text) if one abandoned a bounded device-side wait.  The expert calls report
+ * through coli_b200_moe_check. */
+int coli_b200_fp8_check(int device);
 
 /* ---- expert-parallel block: one call per rank (replaces crates/colibri-engine/src/moe.rs:1737-1794
  * `moe_sharded` and :1620-1734 `sharded_experts_partial`; the TCP request/response of

@@ -9,7 +9,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .configs import FMT_E4M3_ROW, FMT_FP8_B128, FMT_MXFP4, FMT_NVFP4
+from .configs import FMT_E4M3_ROW, FMT_FP8_B128, FMT_MXFP4, FMT_NVFP4, TYPE_BF16, TYPE_F16, TYPE_F32
 
 
 class CudaError(RuntimeError):
@@ -183,6 +183,105 @@ def quantize_fp8_b128_dev(w, device: int = 0):
     _check(_lib_().coli_b200_quantize_fp8_b128(device, w.data_ptr(), O, I, codes.data_ptr(), sc.data_ptr()),
            "coli_b200_quantize_fp8_b128")
     return codes, sc
+
+
+# ---- 8-bit rows: e4m3 codes and an f32 scale per row and 128 columns ---------------------------------------
+def _type_codes():
+    import torch
+
+    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def _stream_of(x, stream):
+    import torch
+
+    return torch.cuda.current_stream(x.device).cuda_stream if stream is None else stream
+
+
+def _on_cuda(what: str, ref, **tensors) -> None:
+    """Raises unless every given tensor is on the GPU of `ref`."""
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {ref.device}")
+    if not ref.is_cuda:
+        raise ValueError(f"{what}: needs CUDA tensors, not {ref.device}")
+
+
+def _check_rows_fp8(what: str, codes, scales, K: int) -> None:
+    R = codes.shape[0]
+    if codes.dim() != 2 or codes.element_size() != 1 or codes.shape[1] != K or (K > 1 and codes.stride(1) != 1):
+        raise ValueError(f"{what}: codes must be one byte each, [rows, {K}], columns next to each other")
+    if tuple(scales.shape) != (R, (K + 127) // 128) or scales.dtype != _f32():
+        raise ValueError(f"{what}: scales must be f32 [{R}, {(K + 127) // 128}], not {scales.dtype} {tuple(scales.shape)}")
+
+
+def _f32():
+    import torch
+
+    return torch.float32
+
+
+def _row_bytes(codes) -> int:
+    """Bytes from row to row; a single row may say anything."""
+    return codes.stride(0) if codes.shape[0] > 1 else max(codes.stride(0), (codes.shape[1] + 15) // 16 * 16)
+
+
+def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
+    """coli_b200_quantize_rows_fp8: rows of x (f32, f16 or bf16 [T,K] on the GPU, any row stride) -> (codes u8 [R,K],
+    scales f32 [R, ceil(K/128)]).  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry outside [0,T) leaves the
+    row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16 bytes and a block's
+    scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
+    import torch
+
+    ty = _type_codes().get(x.dtype)
+    if ty is None or x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("quantize_rows_fp8_dev: x must be f32, f16 or bf16 [T,K], columns next to each other")
+    T, K = x.shape
+    if row_token is not None and (row_token.dtype != torch.int32 or row_token.dim() != 1 or not row_token.is_contiguous()):
+        raise ValueError("quantize_rows_fp8_dev: row_token must be contiguous int32 [rows]")
+    R = T if row_token is None else row_token.shape[0]
+    if out is None:
+        codes = torch.empty((R, (K + 15) // 16 * 16), dtype=torch.uint8, device=x.device)[:, :K]
+        scales = torch.empty(((K + 127) // 128, R), dtype=torch.float32, device=x.device).t()
+    else:
+        codes, scales = out
+        _check_rows_fp8("quantize_rows_fp8_dev", codes, scales, K)
+        if codes.shape[0] != R:
+            raise ValueError(f"quantize_rows_fp8_dev: out has {codes.shape[0]} rows, not {R}")
+    _on_cuda("quantize_rows_fp8_dev", x, row_token=row_token, codes=codes, scales=scales)
+    _check(_lib_().coli_b200_quantize_rows_fp8(x.device.index, x.data_ptr(), ty, x.stride(0),
+                                               None if row_token is None else row_token.data_ptr(), T, R, K, codes.data_ptr(),
+                                               _row_bytes(codes), scales.data_ptr(), scales.stride(0), scales.stride(1),
+                                               _stream_of(x, stream)), "coli_b200_quantize_rows_fp8")
+    return codes, scales
+
+
+def matmul_fp8_dev(w: CudaTensor, codes, scales, out_dtype=None, out=None, stream=None):
+    """coli_b200_matmul_fp8_dev: 8-bit rows [R, w.I] times a resident weight of format 8 -> [R, w.O] as `out_dtype` (bf16
+    unless given) or into `out` (f32, f16 or bf16, any row stride)."""
+    import torch
+
+    _check_rows_fp8("matmul_fp8_dev", codes, scales, w.I)
+    R = codes.shape[0]
+    if out is None:
+        out = torch.empty((R, w.O), dtype=out_dtype or torch.bfloat16, device=codes.device)
+    elif tuple(out.shape) != (R, w.O) or (w.O > 1 and out.stride(1) != 1) or out_dtype not in (None, out.dtype):
+        raise ValueError(f"matmul_fp8_dev: out must be [{R}, {w.O}], columns next to each other, of the type asked for")
+    ty = _type_codes().get(out.dtype)
+    if ty is None:
+        raise ValueError(f"matmul_fp8_dev: results are f32, f16 or bf16, not {out.dtype}")
+    _on_cuda("matmul_fp8_dev", codes, scales=scales, out=out)
+    if codes.device.index != w.device:
+        raise ValueError(f"matmul_fp8_dev: the weight is on cuda:{w.device}, the rows on {codes.device}")
+    _check(_lib_().coli_b200_matmul_fp8_dev(w.handle, codes.data_ptr(), _row_bytes(codes), scales.data_ptr(), scales.stride(0),
+                                            scales.stride(1), R, out.data_ptr(), ty, max(out.stride(0), w.O) if R < 2 else out.stride(0),
+                                            _stream_of(codes, stream)), "coli_b200_matmul_fp8_dev")
+    return out
+
+
+def fp8_check(device: int = 0) -> None:
+    """Synchronise and raise if a matmul_fp8_dev on the device abandoned a bounded device-side wait."""
+    _check(_lib_().coli_b200_fp8_check(device), "coli_b200_fp8_check")
 
 
 # ---- the reference's host-pointer expert calls ---------------------------------------------------

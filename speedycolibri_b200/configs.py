@@ -9,6 +9,9 @@ FMT_MXFP4 = 6
 FMT_FP8_B128 = 8
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
 
 
 @dataclass(frozen=True)

@@ -9,6 +9,7 @@
 #include <mutex>
 #include <vector>
 
+#include "fp8.cuh"
 #include "host_state.cuh"
 
 // ---- errors ---------------------------------------------------------------------------------
@@ -1179,6 +1180,185 @@ extern "C" int coli_b200_moe_experts_dev(ColiMoe *m, const void *rows_dev, const
   }
   return run_segments(m, m->gate, m->up, m->down, m->seg_expert + m->first_local_seg, rows_dev, seg_count_dev, m->n_local_seg,
                       rows_cap, rows_expected < rows_cap ? rows_expected : rows_cap, y_dev, pick_stream(m, stream));
+}
+
+// ---- 8-bit rows ------------------------------------------------------------------------------------------
+namespace {
+// Makes `device` the current one for a call and puts the caller's back: these calls take the place of one line in a
+// program that drives several devices.
+struct OnDevice {
+  int before = -1;
+  bool ok = false;
+  explicit OnDevice(int device) {
+    DeviceContext *c = find_ctx(device);
+    if (!c) return;
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    ok = before == device || select_ctx(c);
+  }
+  ~OnDevice() {
+    if (ok && before >= 0) cudaSetDevice(before);
+  }
+};
+size_t type_size(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYPE_F16 || type == COLI_TYPE_BF16 ? 2 : 0; }
+bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// Codes are copied by TMA (16-byte rows), scales read one by one.
+bool check_fp8_rows(const char *who, const void *codes, int64_t ld, const float *scales, int64_t s_row, int64_t s_blk, int rows, int K) {
+  if (rows < 0 || (rows > 0 && (!codes || !scales))) {
+    coli_set_error("%s: bad row count %d or null pointer", who, rows);
+    return false;
+  }
+  if (ld < round_up(K, 16) || ld % 16 || !aligned_to(codes, 16) || !aligned_to(scales, 4)) {
+    coli_set_error("%s: rows of codes must start on 16 bytes, at least %d apart (ld=%lld)", who, round_up(K, 16), (long long)ld);
+    return false;
+  }
+  if (ld >= (int64_t)1 << 40 || s_row < 0 || s_blk < 0) {
+    coli_set_error("%s: bad stride (ld=%lld, scales %lld and %lld)", who, (long long)ld, (long long)s_row, (long long)s_blk);
+    return false;
+  }
+  return true;
+}
+}  // namespace
+
+extern "C" int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_type, int64_t x_stride, const int32_t *row_token_dev,
+                                           int T, int rows, int K, void *codes_dev, int64_t ld, float *scales_dev, int64_t s_row,
+                                           int64_t s_blk, void *stream) {
+  const size_t es = type_size(x_type);
+  if (T < 0 || K < 1 || K > INT32_MAX - 256 || es == 0 || (rows > 0 && T > 0 && !x_dev) || (!row_token_dev && rows > T)) {
+    coli_set_error("quantize_rows_fp8: bad shape or type (T=%d rows=%d K=%d type=%d) or null pointer", T, rows, K, x_type);
+    return 0;
+  }
+  if (x_stride < 0 || !aligned_to(x_dev, es) || !aligned_to(row_token_dev, 4)) {
+    coli_set_error("quantize_rows_fp8: misaligned pointer or negative stride");
+    return 0;
+  }
+  if (!check_fp8_rows("quantize_rows_fp8", codes_dev, ld, scales_dev, s_row, s_blk, rows, K)) return 0;
+  OnDevice on(device);
+  if (!on.ok) return 0;
+  colib::QuantRowsParams p;
+  p.x = x_dev;
+  p.type = x_type;
+  p.x_stride = (long)x_stride;
+  p.x_vec = aligned_to(x_dev, 16) && x_stride * es % 16 == 0;
+  p.row_token = row_token_dev;
+  p.T = T;
+  p.rows = rows;
+  p.K = K;
+  p.codes = (uint8_t *)codes_dev;
+  p.ld = (long)ld;
+  p.scales = scales_dev;
+  p.s_row = (long)s_row;
+  p.s_blk = (long)s_blk;
+  return colib::launch_quant_rows(p, (cudaStream_t)stream);
+}
+
+static colib::Fp8MmParams fp8_rows_params(const void *codes, int64_t ld, const float *scales, int64_t s_row, int64_t s_blk, int rows, int K, int O) {
+  colib::Fp8MmParams p = {};
+  p.codes = codes;
+  p.ld = (long)ld;
+  p.sx = scales;
+  p.s_row = (long)s_row;
+  p.s_blk = (long)s_blk;
+  p.rows = rows;
+  p.rows_expected = rows;
+  p.K = K;
+  p.O = O;
+  p.nseg = 1;
+  return p;
+}
+
+extern "C" int coli_b200_matmul_fp8_dev(const ColiCudaTensor *w, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row,
+                                        int64_t s_blk, int rows, void *y_dev, int y_type, int64_t y_stride, void *stream) {
+  if (!w || w->fmt != COLI_FMT_FP8_B128) {
+    coli_set_error("matmul_fp8_dev: the weight must be a resident handle of format %d (e4m3, f32 scale per 128 x 128)", COLI_FMT_FP8_B128);
+    return 0;
+  }
+  if (!check_fp8_rows("matmul_fp8_dev", codes_dev, ld, scales_dev, s_row, s_blk, rows, w->I)) return 0;
+  const size_t es = type_size(y_type);
+  if (es == 0 || (rows > 0 && !y_dev) || (rows > 1 && y_stride < w->O) || !aligned_to(y_dev, es ? es : 1)) {
+    coli_set_error("matmul_fp8_dev: bad result (type %d, stride %lld for %d features, null or misaligned pointer)", y_type, (long long)y_stride, w->O);
+    return 0;
+  }
+  OnDevice on(w->device);
+  if (!on.ok) return 0;
+  colib::Fp8MmParams p = fp8_rows_params(codes_dev, ld, scales_dev, s_row, s_blk, rows, w->I, w->O);
+  p.one.q = w->q;
+  p.one.s = w->s;
+  p.y = y_dev;
+  p.y_type = y_type;
+  p.y_stride = (long)y_stride;
+  p.y_vec = aligned_to(y_dev, 16) && y_stride * es % 16 == 0;
+  return colib::launch_fp8_mm(p, (cudaStream_t)stream);
+}
+
+extern "C" int coli_b200_fp8_check(int device) {
+  OnDevice on(device);
+  if (!on.ok) return 0;
+  CK(cudaDeviceSynchronize(), "fp8_check sync");
+  int code = 0;
+  if (!colib::fp8_take_status(&code)) return 0;
+  if (code == 0) return 1;
+  coli_set_error("an fp8 product abandoned a bounded wait (code %d: 1 copy, 2 MMA, 4 sums); results of that call are invalid", code);
+  return 0;
+}
+
+// gate/up with h quantised again, then down, over expert-contiguous 8-bit rows
+static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const void *codes, int64_t ld, const float *scales, int64_t s_row,
+                            int64_t s_blk, const int32_t *seg_count_dev, int n_seg, int rows_cap, int rows_expected, void *y_dev,
+                            cudaStream_t st) {
+  if (rows_cap == 0 || n_seg == 0) return 1;
+  const int H = m->L.H, I = m->L.I;
+  const long h_ld = round_up(I, 16);
+  // h's codes and, behind them, its scales take the place of the 16-bit h
+  const size_t need = (size_t)rows_cap * (h_ld + 4 * ((I + 127) / 128));
+  if (!ensure_h(m, m->seg_main, (need + 2 * (size_t)I - 1) / (2 * (size_t)I))) return 0;
+  uint8_t *h = (uint8_t *)m->seg_main.h;
+  float *hs = (float *)(h + (size_t)rows_cap * h_ld);
+  colib::Fp8MmParams p = fp8_rows_params(codes, ld, scales, s_row, s_blk, rows_cap, H, I);
+  p.nseg = n_seg;
+  p.rows_expected = rows_expected;
+  p.seg_count = seg_count_dev;
+  p.seg_expert = seg_expert_dev;
+  p.w0 = m->gate;
+  p.w1 = m->up;
+  p.h_codes = h;
+  p.h_scales = hs;
+  p.h_ld = h_ld;
+  p.act = m->act;
+  p.status = m->status;
+  if (!colib::launch_fp8_mm(p, st)) return 0;
+  colib::Fp8MmParams d = fp8_rows_params(h, h_ld, hs, 1, rows_cap, rows_cap, I, H);
+  d.nseg = n_seg;
+  d.rows_expected = rows_expected;
+  d.seg_count = seg_count_dev;
+  d.seg_expert = seg_expert_dev;
+  d.w0 = m->down;
+  d.y = y_dev;
+  d.y_type = COLI_TYPE_BF16;
+  d.y_stride = H;
+  d.y_vec = true;  // H is a multiple of 8
+  d.status = m->status;
+  return colib::launch_fp8_mm(d, st);
+}
+
+extern "C" int coli_b200_moe_experts_fp8_dev(ColiMoe *m, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row, int64_t s_blk,
+                                             const int32_t *seg_count_dev, int rows_cap, int rows_expected, void *y_dev, void *stream) {
+  if (!m) {
+    coli_set_error("moe_experts_fp8_dev: null handle");
+    return 0;
+  }
+  if (m->L.fmt != COLI_FMT_FP8_B128) {
+    coli_set_error("moe_experts_fp8_dev: the handle's experts have format %d, not %d (e4m3, f32 scale per 128 x 128)", m->L.fmt, COLI_FMT_FP8_B128);
+    return 0;
+  }
+  if (!check_fp8_rows("moe_experts_fp8_dev", codes_dev, ld, scales_dev, s_row, s_blk, rows_cap, m->L.H)) return 0;
+  if (rows_expected < 0 || (rows_cap > 0 && (!y_dev || !seg_count_dev)) || !aligned_to(y_dev, 16) || !aligned_to(seg_count_dev, 4)) {
+    coli_set_error("moe_experts_fp8_dev: bad row bounds, null pointer, or y_dev off the 16-byte grid");
+    return 0;
+  }
+  OnDevice on(m->ctx->device);
+  if (!on.ok) return 0;
+  return run_segments_fp8(m, m->seg_expert + m->first_local_seg, codes_dev, ld, scales_dev, s_row, s_blk, seg_count_dev, m->n_local_seg,
+                          rows_cap, rows_expected < rows_cap ? rows_expected : rows_cap, y_dev, pick_stream(m, stream));
 }
 
 extern "C" int coli_b200_moe_shared_dev(ColiMoe *m, const void *x_dev, int T, void *y_dev, void *stream) {

@@ -1,0 +1,562 @@
+// Products of 8-bit floating-point rows and weights with a scale for each block of 128, the quantiser that makes such
+// rows, and the expert FFN over them.
+//
+//   rows     q[r,k] e4m3, sx[r,b] f32: row r, columns 128b .. 128b+127 stand for sx[r,b] * q
+//   weights  FMT_FP8_B128 handles: codes qw[o,k], sw[o / 128, b] f32
+//   product  y[r,o] = sum_b sx[r,b] * sw[o/128,b] * ( sum_{k in b} q[r,k] * qw[o,k] )
+//
+// (crates/colibri-engine/src/convert.rs:731-741 has the weights' half of it; the reference multiplies f32 activations.)
+#include <cuda_fp8.h>
+
+#include "fp8.cuh"
+#include "tc_common.cuh"
+
+namespace colib {
+
+// ---- row quantiser ---------------------------------------------------------------------------------------------
+// 16 lanes share the 128 columns of a block, 8 each.
+//   a = largest |x| of the block's non-NaN values, s = 1 if a == 0 else max(a / 448, 2^-126), code = e4m3(x / s)
+// to nearest even, saturating; a NaN keeps a NaN code, and an infinity makes s infinite and its own code NaN, so
+// that either shows in every product with the row.
+__device__ __forceinline__ float row_scale(float a) { return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), 1.17549435e-38f) : 1.0f; }
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_quant_rows(QuantRowsParams p) {
+  coli_grid_dependency_sync();
+  const int KB = (p.K + 127) >> 7, kp = (p.K + 15) & ~15;
+  const int sub = threadIdx.x & 15;
+  const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  const long total = (long)p.rows * KB;
+  const bool wide = p.x_vec;
+  for (long g = (long)blockIdx.x * 16 + (threadIdx.x >> 4); g < total; g += (long)gridDim.x * 16) {
+    const int r = (int)(g / KB), b = (int)(g % KB);
+    int src = r;
+    if (p.row_token) {
+      src = p.row_token[r];
+      if ((unsigned)src >= (unsigned)p.T) continue;  // no token: the row is left as it was
+    }
+    const int c0 = b * 128 + sub * 8;
+    const T *x = (const T *)p.x + (long)src * p.x_stride + c0;
+    float v[8];
+    if (wide && c0 + 8 <= p.K) {
+      alignas(16) T raw[8];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(raw) / 16; ++i) reinterpret_cast<uint4 *>(raw)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i < p.K ? to_f32<T>(x[i]) : 0.0f;
+    }
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
+    const float s = row_scale(a);
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = e4m3x2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
+    if (c0 < kp) *reinterpret_cast<uint2 *>(p.codes + (size_t)r * p.ld + c0) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+    if (sub == 0) p.scales[(long)r * p.s_row + (long)b * p.s_blk] = s;
+  }
+}
+
+int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
+  const long groups = (long)p.rows * ((p.K + 127) / 128);
+  if (groups == 0) return 1;
+  const long ctas = (groups + 15) / 16;
+  const dim3 grid((unsigned)(ctas < 16L * COLI_SMS ? ctas : 16L * COLI_SMS));
+  coli_count_launch(1);
+  cudaError_t e;
+  if (p.type == COLI_TYPE_F32)
+    e = launch_dependent(k_quant_rows<float>, grid, dim3(256), 0, st, p);
+  else if (p.type == COLI_TYPE_F16)
+    e = launch_dependent(k_quant_rows<__half>, grid, dim3(256), 0, st, p);
+  else
+    e = launch_dependent(k_quant_rows<__nv_bfloat16>, grid, dim3(256), 0, st, p);
+  return coli_cuda_check(e, "row quantiser launch") ? 1 : 0;
+}
+
+// ---- product -----------------------------------------------------------------------------------------------------
+// One CTA makes tiles of 128 rows x BN features.  Per 128 columns (one k-tile, one scale block) a stage of the
+// shared-memory ring holds the rows' codes (one TMA box, 128-byte swizzle) and the weights' codes, which lie in HBM in
+// exactly that order (coli_fp8_chunk is the swizzle's permutation) and come as plain bulk copies; four tcgen05.mma
+// kind::f8f6f4 form the k-tile's product in one of two TMEM buffers, and eight warps add it to f32 registers, scaled:
+// a thread owns one row (its TMEM lane) and half of the features, so sx is one register and sw is uniform.
+// The scales are arbitrary f32, which the block-scaled MMA kinds do not take.
+constexpr int F8_BM = 128;
+constexpr int F8_EPI_WARPS = 8;
+constexpr int F8_THREADS = (F8_EPI_WARPS + 2) * 32;
+constexpr int F8_MAX_SEGS = 520;
+constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
+struct F8Maps {
+  CUtensorMap m[F8_MAPS];
+};
+static __device__ int g_fp8_status;  // of products without a handle of their own
+
+template <int BN>
+struct F8Smem {
+  static constexpr int A_BYTES = F8_BM * 128;
+  static constexpr int B_BYTES = BN * 128;
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int RED_LD = BN + 4;  // f32 a row of partial sums: rows start 4 banks apart
+  static constexpr int RING = STAGES * STAGE;
+  static_assert(F8_BM * RED_LD * 4 <= RING, "partial sums take the ring's place");
+  static constexpr int BARS = 2 * STAGES + 4;
+  static constexpr int TABLES = 2 * (F8_MAX_SEGS + 1) * 4;
+  static constexpr int BYTES = 1024 + RING + 8 * BARS + 16 + TABLES + 2 * 2 * F8_BM * 4;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
+      "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+struct F8Tile {
+  int seg, nt, row0, nrows;
+};
+// Tile t of the call: segments in order, a segment's feature tiles in order, its row tiles inside one (they share the
+// weights in L2).
+__device__ __forceinline__ F8Tile f8_tile(const int *tile_off, const int *row_off, int nseg, int t) {
+  int lo = 0, hi = nseg;  // tile_off[lo] <= t < tile_off[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile_off[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int n = row_off[lo + 1] - row_off[lo], mt = (n + F8_BM - 1) / F8_BM, l = t - tile_off[lo];
+  F8Tile r;
+  r.seg = lo;
+  r.nt = l / mt;
+  const int m = l - r.nt * mt;
+  r.row0 = row_off[lo] + m * F8_BM;
+  r.nrows = min(F8_BM, n - m * F8_BM);
+  return r;
+}
+
+template <typename OutT>
+__device__ __forceinline__ OutT f8_out(float v);
+template <>
+__device__ __forceinline__ float f8_out<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half f8_out<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 f8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Stores N consecutive values of one row; `valid` of them exist.
+template <typename OutT, int N>
+__device__ __forceinline__ void f8_store(OutT *dst, const float *v, int valid, bool vec) {
+  constexpr int PER = 16 / (int)sizeof(OutT) < N ? 16 / (int)sizeof(OutT) : N;
+  alignas(16) OutT o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = f8_out<OutT>(v[i]);
+#pragma unroll
+  for (int i = 0; i < N; i += PER) {
+    if (vec && i + PER <= valid) {
+      if constexpr (PER * sizeof(OutT) == 16)
+        *reinterpret_cast<uint4 *>(dst + i) = *reinterpret_cast<const uint4 *>(o + i);
+      else
+        *reinterpret_cast<uint2 *>(dst + i) = *reinterpret_cast<const uint2 *>(o + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (i + j < valid) dst[i + j] = o[i + j];
+    }
+  }
+}
+
+// GATED: features of two weights, h = act(gate, up), quantised again as rows (one scale per row and 128 features).
+// SPLIT: the CTAs of a cluster share the k-tiles of one tile and join their sums, in rank order, through distributed
+// shared memory: for calls with too few tiles for the SMs.
+template <bool GATED, int BN, bool SPLIT, typename OutT>
+__global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant__ F8Maps maps, const Fp8MmParams p) {
+  using S = F8Smem<BN>;
+  constexpr int NACC = BN / 2;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t ring = smem_u32(smem);
+  unsigned char *after = smem + S::RING;
+  const uint32_t full = smem_u32(after), empty = full + 8 * S::STAGES, dfull = empty + 8 * S::STAGES, dempty = dfull + 16;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(after + 8 * S::BARS);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *row_off = reinterpret_cast<int *>(after + 8 * S::BARS + 16);
+  int *tile_off = row_off + F8_MAX_SEGS + 1;
+  float *amax_s = reinterpret_cast<float *>(tile_off + F8_MAX_SEGS + 1);  // [tile parity][half][row]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int *status = p.status ? p.status : &g_fp8_status;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(dfull + 8 * b, 1);
+      mbar_init(dempty + 8 * b, F8_EPI_WARPS);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == F8_EPI_WARPS + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2u * BN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  coli_grid_dependency_sync();  // (the set-up above overlaps the predecessor's end)
+  // rows and tiles before every segment; counts that run past the buffer are cut
+  const int NT = p.n_tiles;
+  if (warp == 0) {
+    int rows = 0, tiles = 0;
+    for (int s0 = 0; s0 < p.nseg; s0 += 32) {
+      const int s = s0 + lane;
+      int n = s < p.nseg ? max(0, p.seg_count ? p.seg_count[s] : p.rows) : 0, incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl = (int)min((long)incl + u, (long)p.rows);
+      }
+      const int end = min(p.rows, (int)min((long)rows + incl, (long)p.rows));
+      int prev = __shfl_up_sync(0xffffffffu, end, 1);
+      if (lane == 0) prev = rows;
+      int t = (end - prev + F8_BM - 1) / F8_BM * NT;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += u;
+      }
+      if (s < p.nseg) {
+        row_off[s + 1] = end;
+        tile_off[s + 1] = tiles + t;
+      }
+      rows = __shfl_sync(0xffffffffu, end, 31);
+      tiles += __shfl_sync(0xffffffffu, t, 31);
+    }
+    if (lane == 0) row_off[0] = tile_off[0] = 0;
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int n_tiles = tile_off[p.nseg];
+  const uint32_t rank = SPLIT ? cluster_rank() : 0u;
+  const int world = SPLIT ? p.split : 1;
+  const int cluster0 = (int)blockIdx.x / world, clusters = (int)gridDim.x / world;
+  const int kb0 = SPLIT ? (int)((long)p.KT * rank / world) : 0, kb1 = SPLIT ? (int)((long)p.KT * (rank + 1) / world) : p.KT;
+
+  uint32_t it = 0;  // k-tiles so far: the ring's and the TMEM buffers' place and phase follow from it
+  bool alive = true;
+  for (int t = cluster0; t < n_tiles; t += clusters) {
+    const F8Tile tile = f8_tile(tile_off, row_off, p.nseg, t);
+    const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+    if (warp == F8_EPI_WARPS) {
+      // ---------------- copies ----------------
+      const uint8_t *q0 = p.w0 ? p.w0[ex].q : p.one.q, *q1 = GATED ? p.w1[ex].q : q0;
+      const int f0 = tile.nt * (GATED ? 128 : BN);
+      const uint32_t nb0 = (uint32_t)min(GATED ? 128 : BN, p.Op - f0) * 128u, nb1 = GATED ? nb0 : 0u;
+      int box = 0;
+      while ((8 << box) < tile.nrows) ++box;
+      const uint32_t bytes = (uint32_t)(8 << box) * 128u + nb0 + nb1;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u;
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
+        if (alive && elect_one()) {
+          const uint32_t a = ring + s * S::STAGE, b = a + S::A_BYTES, bar = full + 8 * s;
+          mbar_expect_tx(bar, bytes);
+          tma_load_2d(a, &maps.m[box], kb * 128, tile.row0, bar);
+          const size_t at = ((size_t)kb * p.Op + f0) * 128;
+          bulk_load(b, q0 + at, nb0, bar);
+          if (GATED) bulk_load(b + 128 * 128, q1 + at, nb1, bar);
+        }
+        __syncwarp();
+      }
+    } else if (warp == F8_EPI_WARPS + 1) {
+      // ---------------- products ----------------
+      // kind::f8f6f4: D = f32, A = B = e4m3 (format code 0), both K-major
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(F8_BM >> 4) << 24);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u, d = it & 1u, dph = (it >> 1) & 1u;
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(dempty + 8 * d, dph ^ 1u, abort_flag, status, TC_ERR_MMA_WAIT));
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, status, TC_ERR_MMA_WAIT));
+        tc_fence_after();
+        if (alive && elect_one()) {
+          const uint32_t a = ring + s * S::STAGE;
+          const uint64_t ad = umma_smem_desc(a), bd = umma_smem_desc(a + S::A_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f8(tmem + d * BN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
+          umma_commit(empty + 8 * s);
+          umma_commit(dfull + 8 * d);
+        }
+        __syncwarp();
+      }
+    } else {
+      // ---------------- scaled sums ----------------
+      const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+      const bool any = (warp & 3) * 32 < tile.nrows, mine = row < tile.nrows;
+      const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      const float *w0s = reinterpret_cast<const float *>(p.w0 ? p.w0[ex].s : p.one.s);
+      const float *w1s = GATED ? reinterpret_cast<const float *>(p.w1[ex].s) : nullptr;
+      const int fb = GATED ? tile.nt : min((tile.nt * BN + half * NACC) >> 7, (p.O - 1) >> 7);
+      w0s += (size_t)fb * p.KT;
+      if (GATED) w1s += (size_t)fb * p.KT;
+      const float *sx = p.sx + (long)(tile.row0 + (mine ? row : 0)) * p.s_row;
+      float acc[NACC];
+#pragma unroll
+      for (int i = 0; i < NACC; ++i) acc[i] = 0.0f;
+      float nx = 0.0f, nw0 = 0.0f, nw1 = 0.0f;
+      if (any && kb0 < kb1) {
+        nx = __ldg(sx + (long)kb0 * p.s_blk);
+        nw0 = __ldg(w0s + kb0);
+        if (GATED) nw1 = __ldg(w1s + kb0);
+      }
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t d = it & 1u, dph = (it >> 1) & 1u;
+        const float s0 = nx * nw0, s1 = GATED ? nx * nw1 : s0;
+        if (any && kb + 1 < kb1) {
+          nx = __ldg(sx + (long)(kb + 1) * p.s_blk);
+          nw0 = __ldg(w0s + kb + 1);
+          if (GATED) nw1 = __ldg(w1s + kb + 1);
+        }
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(dfull + 8 * d, dph, abort_flag, status, TC_ERR_EPI_WAIT));
+        tc_fence_after();
+        if (any && alive) {
+          uint32_t v[2][16];
+          auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < NACC / 32 ? 64 * half + 16 * c : 128 + 64 * half + 16 * (c - NACC / 32)) : half * NACC + 16 * c); };
+          tmem_ld16(column(0), v[0]);
+#pragma unroll
+          for (int c = 0; c < NACC / 16; ++c) {
+            tmem_ld_wait();
+            if (c + 1 < NACC / 16) tmem_ld16(column(c + 1), v[(c + 1) & 1]);
+            const float s = GATED && c >= NACC / 32 ? s1 : s0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[16 * c + i]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dempty + 8 * d);
+      }
+      if constexpr (SPLIT) {
+        // partial sums into the ring's place: its last copies have been multiplied
+        float *red = reinterpret_cast<float *>(smem);
+        if (mine && alive) {
+#pragma unroll
+          for (int c = 0; c < NACC / 4; ++c) {
+            const int col = GATED ? (4 * c < 64 ? 64 * half + 4 * c : 128 + 64 * half + 4 * c - 64) : half * NACC + 4 * c;
+            *reinterpret_cast<float4 *>(red + row * S::RED_LD + col) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+          }
+        }
+      } else if constexpr (GATED) {
+        // h of 64 features, the row's largest together with the other half's, codes
+        float a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          const float h = tile.nt * 128 + 64 * half + i < p.O ? coli_act_fast(acc[i], acc[64 + i], p.act) : 0.0f;
+          acc[i] = h;
+          a = fmaxf(a, fabsf(h));
+        }
+        float *am = amax_s + ((t / clusters) & 1) * 2 * F8_BM;
+        am[half * F8_BM + row] = a;
+        asm volatile("bar.sync 1, %0;" ::"n"(F8_EPI_WARPS * 32) : "memory");
+        a = fmaxf(a, am[(half ^ 1) * F8_BM + row]);
+        const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
+        if (mine && alive) {
+          uint8_t *dst = p.h_codes + (size_t)(tile.row0 + row) * p.h_ld + tile.nt * 128 + 64 * half;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = e4m3x2(acc[16 * c + 4 * i] * inv, acc[16 * c + 4 * i + 1] * inv) |
+                     (e4m3x2(acc[16 * c + 4 * i + 2] * inv, acc[16 * c + 4 * i + 3] * inv) << 16);
+            if (tile.nt * 128 + 64 * half + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (half == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
+        }
+      } else {
+        const int f = tile.nt * BN + half * NACC;
+        if (mine && alive && f < p.O) f8_store<OutT, NACC>((OutT *)p.y + (long)(tile.row0 + row) * p.y_stride + f, acc, p.O - f, p.y_vec);
+      }
+    }
+    if constexpr (SPLIT) {
+      cluster_sync();
+      alive = alive && !*abort_flag;
+      if (warp < F8_EPI_WARPS && alive) {
+        const uint32_t red = ring;
+        for (int i = (int)rank + world * warp; i < tile.nrows; i += world * F8_EPI_WARPS) {  // a warp per row
+          float4 v[BN / 128];
+#pragma unroll
+          for (int j = 0; j < BN / 128; ++j) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int r = 0; r < world; ++r) {
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j) {
+              const float4 u = ld_cluster4(red + (uint32_t)(i * S::RED_LD + 128 * j + 4 * lane) * 4u, (uint32_t)r);
+              v[j].x += u.x;
+              v[j].y += u.y;
+              v[j].z += u.z;
+              v[j].w += u.w;
+            }
+          }
+          if constexpr (GATED) {
+            const int f = tile.nt * 128 + 4 * lane;
+            const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+            float h[4], a = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              h[j] = f + j < p.O ? coli_act_fast(g[j], u[j], p.act) : 0.0f;
+              a = fmaxf(a, fabsf(h[j]));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
+            if (f < p.h_ld)
+              *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)(tile.row0 + i) * p.h_ld + f) =
+                  e4m3x2(h[0] * inv, h[1] * inv) | (e4m3x2(h[2] * inv, h[3] * inv) << 16);
+            if (lane == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + i] = s;
+          } else {
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j) {
+              const int f = tile.nt * BN + 128 * j + 4 * lane;
+              const float o[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+              if (f < p.O) f8_store<OutT, 4>((OutT *)p.y + (long)(tile.row0 + i) * p.y_stride + f, o, p.O - f, p.y_vec);
+            }
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is copied into again
+      cluster_sync();
+    }
+  }
+  if (warp == F8_EPI_WARPS && *abort_flag) {
+    // copies already issued still land in this CTA's shared memory: give them time before exit
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == F8_EPI_WARPS + 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN) : "memory");
+  }
+}
+
+// e4m3 rows [rows, K] that start `ld` bytes apart; box = 128 columns x box_rows rows; reads past either end give zeros
+static bool make_codes_map(CUtensorMap *map, const void *base, int rows, int K, long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    coli_set_error("cuTensorMapEncodeTiled failed with code %d (rows=%d K=%d ld=%ld)", (int)r, rows, K, ld);
+    return false;
+  }
+  return true;
+}
+
+template <bool GATED, int BN, bool SPLIT, typename OutT>
+static int launch_f8(const F8Maps &maps, const Fp8MmParams &p, int grid, cudaStream_t st) {
+  static ColiPerDeviceOnce attr_once;
+  auto *kernel = k_fp8_mm<GATED, BN, SPLIT, OutT>;
+  if (!coli_set_smem_limit(attr_once, kernel, F8Smem<BN>::BYTES, "fp8 product shared-memory attribute")) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(F8_THREADS);
+  cfg.dynamicSmemBytes = F8Smem<BN>::BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 2 : 1;
+  coli_count_launch(1);
+  return coli_cuda_check(cudaLaunchKernelEx(&cfg, kernel, maps, p), "fp8 product launch") ? 1 : 0;
+}
+template <bool GATED, typename OutT>
+static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int grid, cudaStream_t st) {
+  if constexpr (!GATED)
+    if (bn == 128) return p.split > 1 ? launch_f8<false, 128, true, OutT>(maps, p, grid, st) : launch_f8<false, 128, false, OutT>(maps, p, grid, st);
+  return p.split > 1 ? launch_f8<GATED, 256, true, OutT>(maps, p, grid, st) : launch_f8<GATED, 256, false, OutT>(maps, p, grid, st);
+}
+
+int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
+  if (p.rows == 0 || p.nseg == 0) return 1;
+  if (p.nseg > F8_MAX_SEGS) {
+    coli_set_error("fp8 product: %d segments (at most %d)", p.nseg, F8_MAX_SEGS);
+    return 0;
+  }
+  p.KT = (p.K + 127) / 128;
+  p.Op = round_up(p.O, 16);
+  const bool gated = p.h_codes != nullptr;
+  // Row tiles the call is likely to have, and the most it can have.  Both are functions of the call's shapes alone.
+  const int most = p.seg_count ? p.rows / F8_BM + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + F8_BM - 1) / F8_BM;
+  const int likely = p.seg_count ? p.rows_expected / F8_BM + (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : most;
+  int bn = 256;
+  if (!gated && (long)likely * ((p.O + 255) / 256) < COLI_SMS) bn = 128;
+  const int fw = gated ? 128 : bn;
+  p.n_tiles = (p.O + fw - 1) / fw;
+  const long tiles = (long)(likely > 0 ? likely : 1) * p.n_tiles;
+  p.split = 1;
+  while (p.split < 8 && tiles * p.split * 2 <= COLI_SMS && p.split * 2 <= p.KT) p.split *= 2;
+  F8Maps maps;
+  for (int b = 0; b < F8_MAPS; ++b)
+    if (!make_codes_map(&maps.m[b], p.codes, p.rows, p.K, p.ld, 8 << b)) return 0;
+  const long bound = (long)most * p.n_tiles;
+  const int clusters = (int)(bound < COLI_SMS / p.split ? bound : COLI_SMS / p.split);
+  if (gated) return launch_f8_shape<true, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);
+  if (p.y_type == COLI_TYPE_F32) return launch_f8_shape<false, float>(maps, p, bn, clusters * p.split, st);
+  if (p.y_type == COLI_TYPE_F16) return launch_f8_shape<false, __half>(maps, p, bn, clusters * p.split, st);
+  return launch_f8_shape<false, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);
+}
+
+int fp8_take_status(int *code) {
+  CK(cudaMemcpyFromSymbol(code, g_fp8_status, sizeof(int)), "fp8 status read");
+  const int zero = 0;
+  if (*code) CK(cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int)), "fp8 status clear");
+  return 1;
+}
+
+}  // namespace colib

@@ -10,7 +10,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from .backend import CudaTensor, _check, _lib_, _np_ptr
+from .backend import CudaTensor, _check, _check_rows_fp8, _lib_, _np_ptr, _on_cuda, _row_bytes, _stream_of
 from .configs import FMT_NVFP4, SCORE_SIGMOID, SCORE_SOFTMAX, MoeShape
 
 
@@ -219,6 +219,24 @@ class MoeBlock:
     def experts_dev(self, rows, seg_count, rows_expected, y, stream):
         _check(_lib_().coli_b200_moe_experts_dev(self.handle, rows.data_ptr(), seg_count.data_ptr(), rows.shape[0], rows_expected,
                                                  y.data_ptr(), stream), "coli_b200_moe_experts_dev")
+
+    def experts_fp8_dev(self, codes, scales, seg_count, rows_expected, y, stream=None):
+        """The resident experts over expert-contiguous 8-bit rows (backend.quantize_rows_fp8_dev makes them), asynchronous on
+        the current torch stream: codes [R,H], scales [R, ceil(H/128)], seg_count int32 [local experts], y bf16 [R,H]."""
+        import torch
+
+        R, H = codes.shape[0], self.cfg.hidden
+        _check_rows_fp8("experts_fp8_dev", codes, scales, H)
+        if y.dtype != torch.bfloat16 or tuple(y.shape) != (R, H) or not y.is_contiguous():
+            raise ValueError(f"experts_fp8_dev: y must be contiguous bf16 [{R}, {H}]")
+        if seg_count.dtype != torch.int32 or seg_count.numel() != self.local_experts() or not seg_count.is_contiguous():
+            raise ValueError(f"experts_fp8_dev: seg_count must be contiguous int32 [{self.local_experts()}]")
+        _on_cuda("experts_fp8_dev", codes, scales=scales, seg_count=seg_count, y=y)
+        if codes.device.index != self.device:
+            raise ValueError(f"experts_fp8_dev: the handle is on cuda:{self.device}, the rows on {codes.device}")
+        _check(_lib_().coli_b200_moe_experts_fp8_dev(self.handle, codes.data_ptr(), _row_bytes(codes), scales.data_ptr(), scales.stride(0),
+                                                     scales.stride(1), seg_count.data_ptr(), R, rows_expected, y.data_ptr(),
+                                                     _stream_of(codes, stream)), "coli_b200_moe_experts_fp8_dev")
 
     def shared_dev(self, x, y, stream):
         _check(_lib_().coli_b200_moe_shared_dev(self.handle, x.data_ptr(), x.shape[0], y.data_ptr(), stream),
