@@ -332,6 +332,28 @@ int coli_b200_matmul_fp8_dev(const ColiCudaTensor *w, const void *codes_dev, int
  * through coli_b200_moe_check. */
 int coli_b200_fp8_check(int device);
 
+/* ---- routing from the caller's own logits: DEVICE pointers, asynchronous on `stream` ------------------
+ * logits_dev [T,E] of `type` (COLI_TYPE_*), `stride` elements from row to row.  With z = logit + logit_bias (may be
+ * NULL) an expert takes part where z > -inf: -inf and NaN close it to that token, a row of them is no token.
+ *   score  softmax over the open experts, or sigmoid
+ *   choice score + select_bias (may be NULL), compared in 64 bits; ties go to the lowest expert.  With n_group > 1 only
+ *          experts of the topk_group best groups (contiguous; a group's mark is the sum of its two best choices, or
+ *          its only one; ties to the lowest)
+ *   weight score of the chosen, divided by their sum + 1e-20 if norm_topk, times routed_scale
+ * topk_idx_dev / topk_w_dev [T,k] in descending order of choice; where fewer than k can be chosen the rest is -1 and 0.
+ * For the chosen pairs in expert order (ascending expert, then token): expert_rows_dev [E] pairs of each expert, slot_dev
+ * [T,k] the row of each pair or -1, row_token_dev [T*k] the token of each row, -1 behind the last: what
+ * coli_b200_quantize_rows_fp8, the expert calls and coli_b200_moe_combine_partial_dev take (with every
+ * expert resident).  E <= 512, k <= 32, at most 32 groups.
+ * workspace_dev: coli_b200_route_logits_workspace(T, E) bytes that no other call in flight uses (NULL where that is 0).
+ * The same call gives the same bits.  (The block's own router compares f32 scores, as the reference does,
+ * and takes expert 0 where nothing can be chosen.) */
+size_t coli_b200_route_logits_workspace(int T, int E);
+int coli_b200_route_logits(int device, const void *logits_dev, int type, int64_t stride, const float *select_bias_dev,
+                           const float *logit_bias_dev, int T, int E, int k, int score, int norm_topk, float routed_scale,
+                           int n_group, int topk_group, int32_t *topk_idx_dev, float *topk_w_dev, int32_t *expert_rows_dev,
+                           int32_t *slot_dev, int32_t *row_token_dev, void *workspace_dev, void *stream);
+
 /* ---- expert-parallel block: one call per rank (replaces crates/colibri-engine/src/moe.rs:1737-1794
  * `moe_sharded` and :1620-1734 `sharded_experts_partial`; the TCP request/response of
  * crates/colibri-cluster/src/transport.rs:33-58 becomes an all-to-all over NCCL send/recv) -----------

@@ -9,8 +9,8 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libcoli_b200.so")
-SOURCES = ["abi.cu", "ep.cu", "routing.cu", "layout.cu", "expert_small.cu", "expert_tc_tmem.cu", "combine.cu", "fp8.cu"]
-HEADERS = ["internal.cuh", "host_state.cuh", "host_copy.cuh", "tc_common.cuh", "fp8.cuh", "coli_math.h", os.path.join("..", "..", "include", "coli_b200.h")]
+SOURCES = ["abi.cu", "ep.cu", "routing.cu", "layout.cu", "expert_small.cu", "expert_tc_tmem.cu", "combine.cu", "fp8.cu", "route_logits.cu"]
+HEADERS = ["internal.cuh", "host_state.cuh", "host_copy.cuh", "tc_common.cuh", "fp8.cuh", "route_logits.cuh", "coli_math.h", os.path.join("..", "..", "include", "coli_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-ffp-contract=off", "-shared",
@@ -133,6 +133,8 @@ SIGNATURES = {
     "coli_b200_moe_experts_fp8_dev": (_i, [_P, _P, _l, _P, _l, _l, _P, _i, _i, _P, _P]),
     "coli_b200_quantize_rows_fp8": (_i, [_i, _P, _i, _l, _P, _i, _i, _i, _P, _l, _P, _l, _l, _P]),
     "coli_b200_matmul_fp8_dev": (_i, [_P, _P, _l, _P, _l, _l, _i, _P, _i, _l, _P]),
+    "coli_b200_route_logits_workspace": (_sz, [_i, _i]),
+    "coli_b200_route_logits": (_i, [_i, _P, _i, _l, _P, _P, _i, _i, _i, _i, _i, _f, _i, _i, _P, _P, _P, _P, _P, _P, _P]),
     "coli_b200_fp8_check": (_i, [_i]),
     "coli_b200_moe_shared_dev": (_i, [_P, _P, _i, _P, _P]),
     "coli_b200_moe_combine_partial_dev": (_i, [_P, _P, _P, _P, _P, _i, _P]),

@@ -5,11 +5,12 @@ memory (their ``data_ptr()`` is what crosses the ABI)."""
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 
 from . import _lib
-from .configs import FMT_E4M3_ROW, FMT_FP8_B128, FMT_MXFP4, FMT_NVFP4, TYPE_BF16, TYPE_F16, TYPE_F32
+from .configs import FMT_E4M3_ROW, FMT_FP8_B128, FMT_MXFP4, FMT_NVFP4, SCORE_SOFTMAX, TYPE_BF16, TYPE_F16, TYPE_F32
 
 
 class CudaError(RuntimeError):
@@ -282,6 +283,53 @@ def matmul_fp8_dev(w: CudaTensor, codes, scales, out_dtype=None, out=None, strea
 def fp8_check(device: int = 0) -> None:
     """Synchronise and raise if a matmul_fp8_dev on the device abandoned a bounded device-side wait."""
     _check(_lib_().coli_b200_fp8_check(device), "coli_b200_fp8_check")
+
+
+# ---- routing from given logits -------------------------------------------------------------------------------
+class Routing(NamedTuple):
+    """What route_logits_dev answers: experts and weights of every token, and the rows its pairs take in expert order."""
+
+    idx: object          # int32 [T,k], -1: none
+    w: object            # f32 [T,k]
+    expert_rows: object  # int32 [E]
+    slot: object         # int32 [T,k], -1: none
+    row_token: object    # int32 [T*k], -1 behind the last row
+
+
+def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=None, logit_bias=None, norm_topk: bool = False,
+                     routed_scale: float = 1.0, n_group: int = 1, topk_group: int = 1, out=None, stream=None) -> Routing:
+    """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing.  Biases are f32 [E];
+    -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are written in place."""
+    import torch
+
+    ty = _type_codes().get(logits.dtype)
+    if ty is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("route_logits_dev: logits must be f32, f16 or bf16 [T,E], experts next to each other")
+    T, E = logits.shape
+    for name, b in (("select_bias", select_bias), ("logit_bias", logit_bias)):
+        if b is not None and (b.dtype != torch.float32 or b.numel() != E or not b.is_contiguous() or b.device != logits.device):
+            raise ValueError(f"route_logits_dev: {name} must be contiguous f32 [{E}] on {logits.device}")
+    if out is None:
+        new = lambda dtype, *n: torch.empty(n, dtype=dtype, device=logits.device)  # noqa: E731
+        out = Routing(new(torch.int32, T, k), new(torch.float32, T, k), new(torch.int32, E), new(torch.int32, T, k), new(torch.int32, T * k))
+    else:
+        out = Routing(*out)
+        for name, t, shape in zip(Routing._fields, out, ((T, k), (T, k), (E,), (T, k), (T * k,))):
+            if tuple(t.shape) != shape or t.dtype != (torch.float32 if name == "w" else torch.int32) or not t.is_contiguous():
+                raise ValueError(f"route_logits_dev: out.{name} must be contiguous {'f32' if name == 'w' else 'int32'} {list(shape)}")
+    _on_cuda("route_logits_dev", logits, **out._asdict())
+    lib = _lib_()
+    n = lib.coli_b200_route_logits_workspace(T, E)
+    work = torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+    if work is not None and stream is not None:
+        work.record_stream(torch.cuda.ExternalStream(stream, device=logits.device))
+    _check(lib.coli_b200_route_logits(logits.device.index, logits.data_ptr(), ty, logits.stride(0) if T > 1 else E,
+                                      None if select_bias is None else select_bias.data_ptr(),
+                                      None if logit_bias is None else logit_bias.data_ptr(), T, E, k, score, int(norm_topk), float(routed_scale),
+                                      n_group, topk_group, out.idx.data_ptr(), out.w.data_ptr(), out.expert_rows.data_ptr(),
+                                      out.slot.data_ptr(), out.row_token.data_ptr(), None if work is None else work.data_ptr(),
+                                      _stream_of(logits, stream)), "coli_b200_route_logits")
+    return out
 
 
 # ---- the reference's host-pointer expert calls ---------------------------------------------------

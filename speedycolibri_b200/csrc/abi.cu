@@ -11,6 +11,7 @@
 
 #include "fp8.cuh"
 #include "host_state.cuh"
+#include "route_logits.cuh"
 
 // ---- errors ---------------------------------------------------------------------------------
 static thread_local char g_err[512] = "";
@@ -1299,6 +1300,66 @@ extern "C" int coli_b200_fp8_check(int device) {
   if (code == 0) return 1;
   coli_set_error("an fp8 product abandoned a bounded wait (code %d: 1 copy, 2 MMA, 4 sums); results of that call are invalid", code);
   return 0;
+}
+
+extern "C" size_t coli_b200_route_logits_workspace(int T, int E) {
+  if (T < 1 || E < 1) return 0;
+  const int c = colib::route_logits_chunk(T), chunks = (T + c - 1) / c;
+  return chunks == 1 ? 0 : (size_t)chunks * E;
+}
+
+extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int type, int64_t stride, const float *select_bias_dev,
+                                      const float *logit_bias_dev, int T, int E, int k, int score, int norm_topk, float routed_scale,
+                                      int n_group, int topk_group, int32_t *topk_idx_dev, float *topk_w_dev, int32_t *expert_rows_dev,
+                                      int32_t *slot_dev, int32_t *row_token_dev, void *workspace_dev, void *stream) {
+  const size_t es = type_size(type);
+  if (T < 0 || E < 1 || E > 512 || k < 1 || k > 32 || k > E || es == 0 || (int64_t)T * k > INT32_MAX) {
+    coli_set_error("route_logits: unsupported shape T=%d E=%d k=%d type=%d (E <= 512, k <= min(32, E), T * k below 2^31)", T, E, k, type);
+    return 0;
+  }
+  if (score != COLI_SCORE_SOFTMAX && score != COLI_SCORE_SIGMOID) {
+    coli_set_error("route_logits: unknown score function %d", score);
+    return 0;
+  }
+  if (n_group < 1 || topk_group < 1 || topk_group > n_group || n_group > 32 || E % n_group || k > topk_group * (E / n_group)) {
+    coli_set_error("route_logits: %d of %d groups of %d experts do not hold k=%d (at most 32 groups, which divide E)", topk_group, n_group, E, k);
+    return 0;
+  }
+  if (!expert_rows_dev || (T > 0 && (!logits_dev || !topk_idx_dev || !topk_w_dev || !slot_dev || !row_token_dev)) ||
+      (coli_b200_route_logits_workspace(T, E) && !workspace_dev)) {
+    coli_set_error("route_logits: null pointer");
+    return 0;
+  }
+  if (stride < 0 || (T > 1 && stride < E) || !aligned_to(logits_dev, es) || !aligned_to(select_bias_dev, 4) || !aligned_to(logit_bias_dev, 4) ||
+      !aligned_to(topk_idx_dev, 4) || !aligned_to(topk_w_dev, 4) || !aligned_to(expert_rows_dev, 4) || !aligned_to(slot_dev, 4) ||
+      !aligned_to(row_token_dev, 4)) {
+    coli_set_error("route_logits: row stride %lld for %d experts, or a misaligned pointer", (long long)stride, E);
+    return 0;
+  }
+  OnDevice on(device);
+  if (!on.ok) return 0;
+  if (T == 0) return coli_cuda_check(cudaMemsetAsync(expert_rows_dev, 0, sizeof(int32_t) * E, (cudaStream_t)stream), "count clear") ? 1 : 0;
+  colib::RouteLogitsParams p = {};
+  p.logits = logits_dev;
+  p.type = type;
+  p.stride = (long)stride;
+  p.T = T;
+  p.E = E;
+  p.k = k;
+  p.score = score;
+  p.norm_topk = norm_topk;
+  p.routed_scale = routed_scale;
+  p.n_group = n_group;
+  p.topk_group = topk_group;
+  p.select_bias = select_bias_dev;
+  p.logit_bias = logit_bias_dev;
+  p.idx = topk_idx_dev;
+  p.w = topk_w_dev;
+  p.expert_rows = expert_rows_dev;
+  p.slot = slot_dev;
+  p.row_token = row_token_dev;
+  p.chunk_rows = (uint8_t *)workspace_dev;
+  return colib::launch_route_logits(p, (cudaStream_t)stream);
 }
 
 // gate/up with h quantised again, then down, over expert-contiguous 8-bit rows
