@@ -18,7 +18,7 @@ class CudaError(RuntimeError):
 
 
 def _lib_():
-    return _lib.load()
+    return _lib._lib or _lib.load()
 
 
 def _check(ok: int, what: str) -> None:
@@ -187,96 +187,104 @@ def quantize_fp8_b128_dev(w, device: int = 0):
 
 
 # ---- 8-bit rows: e4m3 codes and an f32 scale per row and 128 columns ---------------------------------------
-def _type_codes():
-    import torch
+# A decode step makes these calls by the dozen and its kernels take a few microseconds each, so what stands around the C call
+# reads every property of a tensor once (each costs 0.1 to 0.2 us).
+class _Torch:
+    """torch, looked up by the first device call: the host-array calls do without it."""
 
-    return {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    def __init__(self):
+        import torch
 
-
-def _stream_of(x, stream):
-    import torch
-
-    return torch.cuda.current_stream(x.device).cuda_stream if stream is None else stream
-
-
-def _on_cuda(what: str, ref, **tensors) -> None:
-    """Raises unless every given tensor is on the GPU of `ref`."""
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {ref.device}")
-    if not ref.is_cuda:
-        raise ValueError(f"{what}: needs CUDA tensors, not {ref.device}")
+        self.types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        self.f32, self.i32, self.bf16, self.u8, self.empty = torch.float32, torch.int32, torch.bfloat16, torch.uint8, torch.empty
+        # the handle of a device's current stream; the public way builds a Stream object for it (2.3 us against 0.1)
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _check_rows_fp8(what: str, codes, scales, K: int) -> None:
-    R = codes.shape[0]
-    if codes.dim() != 2 or codes.element_size() != 1 or codes.shape[1] != K or (K > 1 and codes.stride(1) != 1):
+_torch = None
+
+
+def _torch_() -> _Torch:
+    global _torch
+    if _torch is None:
+        _torch = _Torch()
+    return _torch
+
+
+def _same_gpu(what: str, device: int, *tensors) -> None:
+    """Raises unless every given tensor is on GPU `device` (-1: the host)."""
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{what}: tensors on {t.device} and on {'cuda:%d' % device if device >= 0 else 'the host'}")
+    if device < 0:
+        raise ValueError(f"{what}: needs CUDA tensors")
+
+
+def _rows_fp8(what: str, codes, scales, K: int):
+    """(rows, bytes from row to row, strides of the scales) of a matrix in 8 bits, checked."""
+    shape, stride = codes.shape, codes.stride()
+    if len(shape) != 2 or shape[1] != K or codes.element_size() != 1 or (K > 1 and stride[1] != 1):
         raise ValueError(f"{what}: codes must be one byte each, [rows, {K}], columns next to each other")
-    if tuple(scales.shape) != (R, (K + 127) // 128) or scales.dtype != _f32():
+    R = shape[0]
+    if scales.shape != (R, (K + 127) // 128) or scales.dtype != _torch_().f32:
         raise ValueError(f"{what}: scales must be f32 [{R}, {(K + 127) // 128}], not {scales.dtype} {tuple(scales.shape)}")
-
-
-def _f32():
-    import torch
-
-    return torch.float32
-
-
-def _row_bytes(codes) -> int:
-    """Bytes from row to row; a single row may say anything."""
-    return codes.stride(0) if codes.shape[0] > 1 else max(codes.stride(0), (codes.shape[1] + 15) // 16 * 16)
+    s_row, s_blk = scales.stride()
+    ld = stride[0]
+    if R < 2:  # (a single row may say anything)
+        ld = max(ld, (K + 15) // 16 * 16)
+    return R, ld, s_row, s_blk
 
 
 def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     """coli_b200_quantize_rows_fp8: rows of x (f32, f16 or bf16 [T,K] on the GPU, any row stride) -> (codes u8 [R,K],
-    scales f32 [R, ceil(K/128)]).  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry outside [0,T) leaves the
-    row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16 bytes and a block's
-    scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
-    import torch
-
-    ty = _type_codes().get(x.dtype)
-    if ty is None or x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+    scales f32 [R, ceil(K/128)]), on the current torch stream.  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
+    outside [0,T) leaves the row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16
+    bytes and a block's scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
+    th = _torch or _torch_()
+    ty, shape, xs = th.types.get(x.dtype), x.shape, x.stride()
+    if ty is None or len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and xs[1] != 1):
         raise ValueError("quantize_rows_fp8_dev: x must be f32, f16 or bf16 [T,K], columns next to each other")
-    T, K = x.shape
-    if row_token is not None and (row_token.dtype != torch.int32 or row_token.dim() != 1 or not row_token.is_contiguous()):
+    T, K = shape
+    if row_token is None:
+        R, take = T, None
+    elif row_token.dtype != th.i32 or row_token.dim() != 1 or not row_token.is_contiguous():
         raise ValueError("quantize_rows_fp8_dev: row_token must be contiguous int32 [rows]")
-    R = T if row_token is None else row_token.shape[0]
+    else:
+        R, take = row_token.shape[0], row_token.data_ptr()
     if out is None:
-        codes = torch.empty((R, (K + 15) // 16 * 16), dtype=torch.uint8, device=x.device)[:, :K]
-        scales = torch.empty(((K + 127) // 128, R), dtype=torch.float32, device=x.device).t()
+        codes = th.empty((R, (K + 15) // 16 * 16), dtype=th.u8, device=x.device)[:, :K]
+        scales = th.empty(((K + 127) // 128, R), dtype=th.f32, device=x.device).t()
     else:
         codes, scales = out
-        _check_rows_fp8("quantize_rows_fp8_dev", codes, scales, K)
-        if codes.shape[0] != R:
-            raise ValueError(f"quantize_rows_fp8_dev: out has {codes.shape[0]} rows, not {R}")
-    _on_cuda("quantize_rows_fp8_dev", x, row_token=row_token, codes=codes, scales=scales)
-    _check(_lib_().coli_b200_quantize_rows_fp8(x.device.index, x.data_ptr(), ty, x.stride(0),
-                                               None if row_token is None else row_token.data_ptr(), T, R, K, codes.data_ptr(),
-                                               _row_bytes(codes), scales.data_ptr(), scales.stride(0), scales.stride(1),
-                                               _stream_of(x, stream)), "coli_b200_quantize_rows_fp8")
+    rows, ld, s_row, s_blk = _rows_fp8("quantize_rows_fp8_dev", codes, scales, K)
+    if rows != R:
+        raise ValueError(f"quantize_rows_fp8_dev: out has {rows} rows, not {R}")
+    device = x.get_device()
+    _same_gpu("quantize_rows_fp8_dev", device, codes, scales, row_token)
+    if not _lib_().coli_b200_quantize_rows_fp8(device, x.data_ptr(), ty, xs[0], take, T, R, K, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk,
+                                               th.stream(device) if stream is None else stream):
+        _check(0, "coli_b200_quantize_rows_fp8")
     return codes, scales
 
 
 def matmul_fp8_dev(w: CudaTensor, codes, scales, out_dtype=None, out=None, stream=None):
     """coli_b200_matmul_fp8_dev: 8-bit rows [R, w.I] times a resident weight of format 8 -> [R, w.O] as `out_dtype` (bf16
-    unless given) or into `out` (f32, f16 or bf16, any row stride)."""
-    import torch
-
-    _check_rows_fp8("matmul_fp8_dev", codes, scales, w.I)
-    R = codes.shape[0]
+    unless given) or into `out` (f32, f16 or bf16, any row stride), on the current torch stream."""
+    th = _torch or _torch_()
+    R, ld, s_row, s_blk = _rows_fp8("matmul_fp8_dev", codes, scales, w.I)
+    O = w.O
     if out is None:
-        out = torch.empty((R, w.O), dtype=out_dtype or torch.bfloat16, device=codes.device)
-    elif tuple(out.shape) != (R, w.O) or (w.O > 1 and out.stride(1) != 1) or out_dtype not in (None, out.dtype):
-        raise ValueError(f"matmul_fp8_dev: out must be [{R}, {w.O}], columns next to each other, of the type asked for")
-    ty = _type_codes().get(out.dtype)
-    if ty is None:
-        raise ValueError(f"matmul_fp8_dev: results are f32, f16 or bf16, not {out.dtype}")
-    _on_cuda("matmul_fp8_dev", codes, scales=scales, out=out)
-    if codes.device.index != w.device:
-        raise ValueError(f"matmul_fp8_dev: the weight is on cuda:{w.device}, the rows on {codes.device}")
-    _check(_lib_().coli_b200_matmul_fp8_dev(w.handle, codes.data_ptr(), _row_bytes(codes), scales.data_ptr(), scales.stride(0),
-                                            scales.stride(1), R, out.data_ptr(), ty, max(out.stride(0), w.O) if R < 2 else out.stride(0),
-                                            _stream_of(codes, stream)), "coli_b200_matmul_fp8_dev")
+        out = th.empty((R, O), dtype=out_dtype or th.bf16, device=codes.device)
+    ty, stride = th.types.get(out.dtype), out.stride()
+    if out.shape != (R, O) or (O > 1 and stride[1] != 1) or ty is None or (out_dtype is not None and out_dtype != out.dtype):
+        raise ValueError(f"matmul_fp8_dev: the result must be f32, f16 or bf16 [{R}, {O}], columns next to each other, of the type asked for")
+    device = codes.get_device()
+    _same_gpu("matmul_fp8_dev", device, scales, out)
+    if device != w.device:
+        raise ValueError(f"matmul_fp8_dev: the weight is on cuda:{w.device}, the rows on cuda:{device}")
+    if not _lib_().coli_b200_matmul_fp8_dev(w.handle, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk, R, out.data_ptr(), ty, stride[0],
+                                            th.stream(device) if stream is None else stream):
+        _check(0, "coli_b200_matmul_fp8_dev")
     return out
 
 
@@ -298,37 +306,40 @@ class Routing(NamedTuple):
 
 def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=None, logit_bias=None, norm_topk: bool = False,
                      routed_scale: float = 1.0, n_group: int = 1, topk_group: int = 1, out=None, stream=None) -> Routing:
-    """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing.  Biases are f32 [E];
-    -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are written in place."""
-    import torch
-
-    ty = _type_codes().get(logits.dtype)
-    if ty is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing, on the current torch
+    stream.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are written in place."""
+    th = _torch or _torch_()
+    ty, shape, zs = th.types.get(logits.dtype), logits.shape, logits.stride()
+    if ty is None or len(shape) != 2 or (shape[1] > 1 and zs[1] != 1):
         raise ValueError("route_logits_dev: logits must be f32, f16 or bf16 [T,E], experts next to each other")
-    T, E = logits.shape
+    T, E = shape
     for name, b in (("select_bias", select_bias), ("logit_bias", logit_bias)):
-        if b is not None and (b.dtype != torch.float32 or b.numel() != E or not b.is_contiguous() or b.device != logits.device):
-            raise ValueError(f"route_logits_dev: {name} must be contiguous f32 [{E}] on {logits.device}")
+        if b is not None and (b.dtype != th.f32 or b.numel() != E or not b.is_contiguous()):
+            raise ValueError(f"route_logits_dev: {name} must be contiguous f32 [{E}]")
     if out is None:
-        new = lambda dtype, *n: torch.empty(n, dtype=dtype, device=logits.device)  # noqa: E731
-        out = Routing(new(torch.int32, T, k), new(torch.float32, T, k), new(torch.int32, E), new(torch.int32, T, k), new(torch.int32, T * k))
+        new = lambda dtype, *n: th.empty(n, dtype=dtype, device=logits.device)  # noqa: E731
+        out = Routing(new(th.i32, T, k), new(th.f32, T, k), new(th.i32, E), new(th.i32, T, k), new(th.i32, T * k))
     else:
-        out = Routing(*out)
-        for name, t, shape in zip(Routing._fields, out, ((T, k), (T, k), (E,), (T, k), (T * k,))):
-            if tuple(t.shape) != shape or t.dtype != (torch.float32 if name == "w" else torch.int32) or not t.is_contiguous():
-                raise ValueError(f"route_logits_dev: out.{name} must be contiguous {'f32' if name == 'w' else 'int32'} {list(shape)}")
-    _on_cuda("route_logits_dev", logits, **out._asdict())
+        if type(out) is not Routing:
+            out = Routing(*out)
+        pairs = (T, k)
+        for name, t, want in zip(Routing._fields, out, (pairs, pairs, (E,), pairs, (T * k,))):
+            if t.shape != want or t.dtype != (th.f32 if name == "w" else th.i32) or not t.is_contiguous():
+                raise ValueError(f"route_logits_dev: out.{name} must be contiguous {'f32' if name == 'w' else 'int32'} {list(want)}")
+    device = logits.get_device()
+    _same_gpu("route_logits_dev", device, select_bias, logit_bias, *out)
     lib = _lib_()
     n = lib.coli_b200_route_logits_workspace(T, E)
-    work = torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+    work = th.empty(n, dtype=th.u8, device=logits.device) if n else None
     if work is not None and stream is not None:
+        import torch
+
         work.record_stream(torch.cuda.ExternalStream(stream, device=logits.device))
-    _check(lib.coli_b200_route_logits(logits.device.index, logits.data_ptr(), ty, logits.stride(0) if T > 1 else E,
-                                      None if select_bias is None else select_bias.data_ptr(),
-                                      None if logit_bias is None else logit_bias.data_ptr(), T, E, k, score, int(norm_topk), float(routed_scale),
-                                      n_group, topk_group, out.idx.data_ptr(), out.w.data_ptr(), out.expert_rows.data_ptr(),
-                                      out.slot.data_ptr(), out.row_token.data_ptr(), None if work is None else work.data_ptr(),
-                                      _stream_of(logits, stream)), "coli_b200_route_logits")
+    if not lib.coli_b200_route_logits(device, logits.data_ptr(), ty, zs[0] if T > 1 else E, None if select_bias is None else select_bias.data_ptr(),
+                                      None if logit_bias is None else logit_bias.data_ptr(), T, E, k, score, norm_topk, routed_scale, n_group,
+                                      topk_group, out.idx.data_ptr(), out.w.data_ptr(), out.expert_rows.data_ptr(), out.slot.data_ptr(),
+                                      out.row_token.data_ptr(), None if work is None else work.data_ptr(), th.stream(device) if stream is None else stream):
+        _check(0, "coli_b200_route_logits")
     return out
 
 

@@ -1189,15 +1189,16 @@ namespace {
 // program that drives several devices.
 struct OnDevice {
   int before = -1;
-  bool ok = false;
+  bool ok = false, back = false;
   explicit OnDevice(int device) {
     DeviceContext *c = find_ctx(device);
     if (!c) return;
     if (cudaGetDevice(&before) != cudaSuccess) before = -1;
     ok = before == device || select_ctx(c);
+    back = ok && before >= 0 && before != device;
   }
   ~OnDevice() {
-    if (ok && before >= 0) cudaSetDevice(before);
+    if (back) cudaSetDevice(before);
   }
 };
 size_t type_size(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYPE_F16 || type == COLI_TYPE_BF16 ? 2 : 0; }

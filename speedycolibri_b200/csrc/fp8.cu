@@ -14,73 +14,168 @@
 namespace colib {
 
 // ---- row quantiser ---------------------------------------------------------------------------------------------
-// 16 lanes share the 128 columns of a block, 8 each.
-//   a = largest |x| of the block's non-NaN values, s = 1 if a == 0 else max(a / 448, 2^-126), code = e4m3(x / s)
+//   a = largest |x| of a block's non-NaN values, s = 1 if a == 0 else max(a / 448, 2^-126), code = e4m3(x / s)
 // to nearest even, saturating; a NaN keeps a NaN code, and an infinity makes s infinite and its own code NaN, so
 // that either shows in every product with the row.
-__device__ __forceinline__ float row_scale(float a) { return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), 1.17549435e-38f) : 1.0f; }
+//
+// Both quotients are the correctly rounded ones: bf16 rows have many values exactly half-way between two codes, where
+// a product with a rounded reciprocal falls to either side.  With y = 1 / b rounded to nearest and q within a unit of a / b,
+// q + (a - q b) y rounds to the quotient (Markstein, IBM J. Res. Dev. 34, 1990): two FMAs, where a division
+// is ten instructions and a branch (32768 rows of 7168 bf16: 287 us with divisions next to a border only).
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+  const float q = a * y;
+  return fmaf(fmaf(-q, b, a), y, q);
+}
+// two quotients by the same b at once
+__device__ __forceinline__ float2 quotients(float2 a, float b, float y) {
+  uint64_t q, r, a2, nb, y2;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a2) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(nb) : "f"(-b));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y2) : "f"(y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a2), "l"(y2));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a2));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(r), "l"(y2));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(q));
+  return d;
+}
+__device__ __forceinline__ float row_scale(float a) {
+  constexpr float TINY = 1.17549435e-38f;              // 2^-126
+  const float s = fmaxf(quotient(a, 448.0f, 1.0f / 448.0f), TINY);
+  if (!(a >= 7.8886090522e-31f && a <= 3.4028235e38f))  // (the remainder is exact from 2^-100 up; none of an infinity)
+    return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), TINY) : 1.0f;
+  return s;
+}
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t d;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) { return e4m3x4(a.x, a.y, b.x, b.y); }
+
+// Eight lanes share a block, 16 columns each in pieces of 16 bytes; a warp takes QR_STEPS times four blocks of a row and
+// goes through the rows with the next one's pieces already requested; the warps of a CTA take neighbouring rows, whose
+// scales of a block lie side by side.
+constexpr int QR_STEPS = 2, QR_COLS = QR_STEPS * 512;
+template <typename T>
+struct QrPieces {
+  static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 16 / VEC;
+  uint4 q[QR_STEPS][LOADS];
+};
+template <typename T>
+__device__ __forceinline__ void qr_request(QrPieces<T> &d, const QuantRowsParams &p, int src, int c0) {
+  constexpr int VEC = QrPieces<T>::VEC;
+  const T *x = (const T *)p.x + (long)src * p.x_stride;
+#pragma unroll
+  for (int j = 0; j < QR_STEPS; ++j)
+#pragma unroll
+    for (int l = 0; l < QrPieces<T>::LOADS; ++l) {
+      const int c = c0 + 512 * j + 8 * VEC * l;
+      if (p.x_vec && c + VEC <= p.K) {
+        d.q[j][l] = __ldg(reinterpret_cast<const uint4 *>(x + c));
+      } else {
+        alignas(16) T raw[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) raw[i] = c + i < p.K ? x[c + i] : T(0.0f);
+        d.q[j][l] = *reinterpret_cast<const uint4 *>(raw);
+      }
+    }
+}
+// largest magnitude of a word's one or two values (maxima drop NaN)
+__device__ __forceinline__ float qr_amax(float a, uint32_t w, float) { return fmaxf(a, fabsf(__uint_as_float(w))); }
+__device__ __forceinline__ __half2 qr_amax(__half2 a, uint32_t w, __half) { return __hmax2(a, __habs2(*reinterpret_cast<const __half2 *>(&w))); }
+__device__ __forceinline__ __nv_bfloat162 qr_amax(__nv_bfloat162 a, uint32_t w, __nv_bfloat16) {
+  return __hmax2(a, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&w)));
+}
+__device__ __forceinline__ float qr_amax_out(float a) { return a; }
+__device__ __forceinline__ float qr_amax_out(__half2 a) { return fmaxf(__low2float(a), __high2float(a)); }
+__device__ __forceinline__ float qr_amax_out(__nv_bfloat162 a) { return fmaxf(__low2float(a), __high2float(a)); }
+__device__ __forceinline__ void qr_zero(float &a) { a = 0.0f; }
+__device__ __forceinline__ void qr_zero(__half2 &a) { a = __half2(__half(0.0f), __half(0.0f)); }
+__device__ __forceinline__ void qr_zero(__nv_bfloat162 &a) { a = __nv_bfloat162(__nv_bfloat16(0.0f), __nv_bfloat16(0.0f)); }
+__device__ __forceinline__ float2 qr_pair(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float2 qr_pair(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
+struct QrMax {
+  using type = float;
+};
 template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+struct QrMax<__half> {
+  using type = __half2;
+};
 template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+struct QrMax<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_quant_rows(QuantRowsParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(QuantRowsParams p) {
+  using P = QrPieces<T>;
   coli_grid_dependency_sync();
-  const int KB = (p.K + 127) >> 7, kp = (p.K + 15) & ~15;
-  const int sub = threadIdx.x & 15;
-  const unsigned mask = 0xffffu << (threadIdx.x & 16);
-  const long total = (long)p.rows * KB;
-  const bool wide = p.x_vec;
-  for (long g = (long)blockIdx.x * 16 + (threadIdx.x >> 4); g < total; g += (long)gridDim.x * 16) {
-    const int r = (int)(g / KB), b = (int)(g % KB);
-    int src = r;
-    if (p.row_token) {
-      src = p.row_token[r];
-      if ((unsigned)src >= (unsigned)p.T) continue;  // no token: the row is left as it was
+  const int kp = (p.K + 15) & ~15;
+  const int lane = threadIdx.x & 31, sub = lane & 7;
+  const int c0 = blockIdx.y * QR_COLS + (lane >> 3) * 128 + sub * P::VEC;
+  const int step = gridDim.x * 8;
+  // source of a row; outside [0, T): none
+  auto source = [&](long r) { return r < p.rows ? (p.row_token ? __ldg(p.row_token + r) : (int)r) : -1; };
+  auto valid = [&](int src) { return (unsigned)src < (unsigned)p.T; };
+  long r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  P now, next;
+  int src = source(r), src_next = source(r + step);
+  if (valid(src)) qr_request<T>(now, p, src, c0);
+  for (; r < p.rows; r += step) {
+    const int src_after = source(r + 2 * (long)step);
+    if (valid(src_next)) qr_request<T>(next, p, src_next, c0);
+    if (valid(src)) {  // (no token: the row is left as it was)
+#pragma unroll
+      for (int j = 0; j < QR_STEPS; ++j) {
+        typename QrMax<T>::type m;
+        qr_zero(m);
+#pragma unroll
+        for (int l = 0; l < P::LOADS; ++l) m = qr_amax(qr_amax(qr_amax(qr_amax(m, now.q[j][l].x, T()), now.q[j][l].y, T()), now.q[j][l].z, T()), now.q[j][l].w, T());
+        float a = qr_amax_out(m);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const float s = row_scale(a), y = __frcp_rn(s);
+        const float b = s <= 3.4028235e38f ? s : 0.0f;  // (x times the reciprocal of an infinite s as it is)
+#pragma unroll
+        for (int l = 0; l < P::LOADS; ++l) {
+          const int c = c0 + 512 * j + 8 * P::VEC * l;
+          const uint4 q = now.q[j][l];
+          uint8_t *dst = p.codes + (size_t)r * p.ld + c;
+          if constexpr (sizeof(T) == 4) {
+            const uint32_t w = e4m3x4(quotients(make_float2(__uint_as_float(q.x), __uint_as_float(q.y)), b, y),
+                                      quotients(make_float2(__uint_as_float(q.z), __uint_as_float(q.w)), b, y));
+            if (c < kp) *reinterpret_cast<uint32_t *>(dst) = w;
+          } else {
+            const uint2 w = make_uint2(e4m3x4(quotients(qr_pair(q.x, T()), b, y), quotients(qr_pair(q.y, T()), b, y)),
+                                       e4m3x4(quotients(qr_pair(q.z, T()), b, y), quotients(qr_pair(q.w, T()), b, y)));
+            if (c < kp) *reinterpret_cast<uint2 *>(dst) = w;
+          }
+        }
+        const int block = (c0 + 512 * j) >> 7;
+        if (sub == 0 && block * 128 < p.K) p.scales[r * p.s_row + (long)block * p.s_blk] = s;
+      }
     }
-    const int c0 = b * 128 + sub * 8;
-    const T *x = (const T *)p.x + (long)src * p.x_stride + c0;
-    float v[8];
-    if (wide && c0 + 8 <= p.K) {
-      alignas(16) T raw[8];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(raw) / 16; ++i) reinterpret_cast<uint4 *>(raw)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(raw[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c0 + i < p.K ? to_f32<T>(x[i]) : 0.0f;
-    }
-    float a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
-    const float s = row_scale(a);
-    uint32_t q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = e4m3x2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
-    if (c0 < kp) *reinterpret_cast<uint2 *>(p.codes + (size_t)r * p.ld + c0) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-    if (sub == 0) p.scales[(long)r * p.s_row + (long)b * p.s_blk] = s;
+    now = next;
+    src = src_next;
+    src_next = src_after;
   }
 }
 
 int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
-  const long groups = (long)p.rows * ((p.K + 127) / 128);
-  if (groups == 0) return 1;
-  const long ctas = (groups + 15) / 16;
-  const dim3 grid((unsigned)(ctas < 16L * COLI_SMS ? ctas : 16L * COLI_SMS));
+  if (p.rows == 0) return 1;
+  const int chunks = (p.K + QR_COLS - 1) / QR_COLS;
+  if (chunks > 65535) {
+    coli_set_error("row quantiser: %d columns (at most %d)", p.K, 65535 * QR_COLS);
+    return 0;
+  }
+  // CTAs that fit the SMs at once go through the rows
+  const int fit = COLI_SMS * (p.type == COLI_TYPE_F32 ? 2 : 4), groups = (p.rows + 7) / 8;
+  const int each = fit / chunks > 0 ? fit / chunks : 1;
+  const dim3 grid((unsigned)(groups < each ? groups : each), (unsigned)chunks);
   coli_count_launch(1);
   cudaError_t e;
   if (p.type == COLI_TYPE_F32)
@@ -404,8 +499,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = e4m3x2(acc[16 * c + 4 * i] * inv, acc[16 * c + 4 * i + 1] * inv) |
-                     (e4m3x2(acc[16 * c + 4 * i + 2] * inv, acc[16 * c + 4 * i + 3] * inv) << 16);
+              w[i] = e4m3x4(acc[16 * c + 4 * i] * inv, acc[16 * c + 4 * i + 1] * inv, acc[16 * c + 4 * i + 2] * inv, acc[16 * c + 4 * i + 3] * inv);
             if (tile.nt * 128 + 64 * half + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
           }
           if (half == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
@@ -448,7 +542,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
             const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
             if (f < p.h_ld)
               *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)(tile.row0 + i) * p.h_ld + f) =
-                  e4m3x2(h[0] * inv, h[1] * inv) | (e4m3x2(h[2] * inv, h[3] * inv) << 16);
+                  e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
             if (lane == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + i] = s;
           } else {
 #pragma unroll
@@ -542,8 +636,16 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   p.split = 1;
   while (p.split < 8 && tiles * p.split * 2 <= COLI_SMS && p.split * 2 <= p.KT) p.split *= 2;
   F8Maps maps;
+  // One segment has full boxes and a last one; behind counts on the device any may come (an encoding takes 0.3 us).
+  auto box_of = [](int n) {
+    int b = 0;
+    while ((8 << b) < n) ++b;
+    return b;
+  };
+  const int last = p.rows % F8_BM ? p.rows % F8_BM : F8_BM;
   for (int b = 0; b < F8_MAPS; ++b)
-    if (!make_codes_map(&maps.m[b], p.codes, p.rows, p.K, p.ld, 8 << b)) return 0;
+    if (p.seg_count || b == box_of(last) || (b == F8_MAPS - 1 && p.rows >= F8_BM))
+      if (!make_codes_map(&maps.m[b], p.codes, p.rows, p.K, p.ld, 8 << b)) return 0;
   const long bound = (long)most * p.n_tiles;
   const int clusters = (int)(bound < COLI_SMS / p.split ? bound : COLI_SMS / p.split);
   if (gated) return launch_f8_shape<true, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);

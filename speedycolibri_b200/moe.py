@@ -10,7 +10,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib
-from .backend import CudaTensor, _check, _check_rows_fp8, _lib_, _np_ptr, _on_cuda, _row_bytes, _stream_of
+from .backend import CudaTensor, _check, _lib_, _np_ptr, _rows_fp8, _same_gpu, _torch_
 from .configs import FMT_NVFP4, SCORE_SIGMOID, SCORE_SOFTMAX, MoeShape
 
 
@@ -223,20 +223,19 @@ class MoeBlock:
     def experts_fp8_dev(self, codes, scales, seg_count, rows_expected, y, stream=None):
         """The resident experts over expert-contiguous 8-bit rows (backend.quantize_rows_fp8_dev makes them), asynchronous on
         the current torch stream: codes [R,H], scales [R, ceil(H/128)], seg_count int32 [local experts], y bf16 [R,H]."""
-        import torch
-
-        R, H = codes.shape[0], self.cfg.hidden
-        _check_rows_fp8("experts_fp8_dev", codes, scales, H)
-        if y.dtype != torch.bfloat16 or tuple(y.shape) != (R, H) or not y.is_contiguous():
+        th, H = _torch_(), self.cfg.hidden
+        R, ld, s_row, s_blk = _rows_fp8("experts_fp8_dev", codes, scales, H)
+        if y.dtype != th.bf16 or y.shape != (R, H) or not y.is_contiguous():
             raise ValueError(f"experts_fp8_dev: y must be contiguous bf16 [{R}, {H}]")
-        if seg_count.dtype != torch.int32 or seg_count.numel() != self.local_experts() or not seg_count.is_contiguous():
+        if seg_count.dtype != th.i32 or seg_count.numel() != self.local_experts() or not seg_count.is_contiguous():
             raise ValueError(f"experts_fp8_dev: seg_count must be contiguous int32 [{self.local_experts()}]")
-        _on_cuda("experts_fp8_dev", codes, scales=scales, seg_count=seg_count, y=y)
-        if codes.device.index != self.device:
-            raise ValueError(f"experts_fp8_dev: the handle is on cuda:{self.device}, the rows on {codes.device}")
-        _check(_lib_().coli_b200_moe_experts_fp8_dev(self.handle, codes.data_ptr(), _row_bytes(codes), scales.data_ptr(), scales.stride(0),
-                                                     scales.stride(1), seg_count.data_ptr(), R, rows_expected, y.data_ptr(),
-                                                     _stream_of(codes, stream)), "coli_b200_moe_experts_fp8_dev")
+        device = codes.get_device()
+        _same_gpu("experts_fp8_dev", device, scales, seg_count, y)
+        if device != self.device:
+            raise ValueError(f"experts_fp8_dev: the handle is on cuda:{self.device}, the rows on cuda:{device}")
+        if not _lib_().coli_b200_moe_experts_fp8_dev(self.handle, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk, seg_count.data_ptr(), R,
+                                                     rows_expected, y.data_ptr(), th.stream(device) if stream is None else stream):
+            _check(0, "coli_b200_moe_experts_fp8_dev")
 
     def shared_dev(self, x, y, stream):
         _check(_lib_().coli_b200_moe_shared_dev(self.handle, x.data_ptr(), x.shape[0], y.data_ptr(), stream),
