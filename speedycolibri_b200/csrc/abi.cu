@@ -111,6 +111,7 @@ extern "C" int coli_cuda_init(const int *devices, int count) {
       delete c;
       return 0;
     }
+    colib::fp8_status_word();  // (here, so that no later call looks it up inside a stream capture)
     g_ctx[g_ndev++] = c;
   }
   return 1;
@@ -1370,36 +1371,36 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
   if (rows_cap == 0 || n_seg == 0) return 1;
   const int H = m->L.H, I = m->L.I;
   const long h_ld = round_up(I, 16);
-  // h's codes and, behind them, its scales take the place of the 16-bit h
-  const size_t need = (size_t)rows_cap * (h_ld + 4 * ((I + 127) / 128));
-  if (!ensure_h(m, m->seg_main, (need + 2 * (size_t)I - 1) / (2 * (size_t)I))) return 0;
-  uint8_t *h = (uint8_t *)m->seg_main.h;
-  float *hs = (float *)(h + (size_t)rows_cap * h_ld);
-  colib::Fp8MmParams p = fp8_rows_params(codes, ld, scales, s_row, s_blk, rows_cap, H, I);
-  p.nseg = n_seg;
-  p.rows_expected = rows_expected;
-  p.seg_count = seg_count_dev;
-  p.seg_expert = seg_expert_dev;
+  colib::Fp8MmParams p = fp8_rows_params(codes, ld, scales, s_row, s_blk, rows_cap, H, I), d = fp8_rows_params(nullptr, h_ld, nullptr, 1, rows_cap, rows_cap, I, H);
+  p.nseg = d.nseg = n_seg;
+  p.rows_expected = d.rows_expected = rows_expected;
+  p.seg_count = d.seg_count = seg_count_dev;
+  p.seg_expert = d.seg_expert = seg_expert_dev;
+  p.act = m->act;
+  p.status = d.status = m->status;
   p.w0 = m->gate;
   p.w1 = m->up;
-  p.h_codes = h;
-  p.h_scales = hs;
-  p.h_ld = h_ld;
-  p.act = m->act;
-  p.status = m->status;
-  if (!colib::launch_fp8_mm(p, st)) return 0;
-  colib::Fp8MmParams d = fp8_rows_params(h, h_ld, hs, 1, rows_cap, rows_cap, I, H);
-  d.nseg = n_seg;
-  d.rows_expected = rows_expected;
-  d.seg_count = seg_count_dev;
-  d.seg_expert = seg_expert_dev;
   d.w0 = m->down;
   d.y = y_dev;
   d.y_type = COLI_TYPE_BF16;
   d.y_stride = H;
   d.y_vec = true;  // H is a multiple of 8
-  d.status = m->status;
-  return colib::launch_fp8_mm(d, st);
+  // what stands between the two products takes the place of the 16-bit h: segments of a few rows leave h in f32, longer ones
+  // its codes and behind them its scales
+  const bool few = colib::fp8_stream_ok(p);
+  const size_t need = few ? (size_t)rows_cap * I * 4 : (size_t)rows_cap * (h_ld + 4 * ((I + 127) / 128));
+  if (!ensure_h(m, m->seg_main, (need + 2 * (size_t)I - 1) / (2 * (size_t)I))) return 0;
+  uint8_t *h = (uint8_t *)m->seg_main.h;
+  if (few) {
+    p.h32 = d.h32 = (float *)h;
+  } else {
+    p.h_codes = h;
+    p.h_scales = (float *)(h + (size_t)rows_cap * h_ld);
+    p.h_ld = h_ld;
+    d.codes = h;
+    d.sx = p.h_scales;
+  }
+  return colib::launch_fp8_mm(p, st) && colib::launch_fp8_mm(d, st);
 }
 
 extern "C" int coli_b200_moe_experts_fp8_dev(ColiMoe *m, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row, int64_t s_blk,

@@ -6,9 +6,8 @@
 //   product  y[r,o] = sum_b sx[r,b] * sw[o/128,b] * ( sum_{k in b} q[r,k] * qw[o,k] )
 //
 // (crates/colibri-engine/src/convert.rs:731-741 has the weights' half of it; the reference multiplies f32 activations.)
-#include <cuda_fp8.h>
-
 #include "fp8.cuh"
+#include "fp8_common.cuh"
 #include "tc_common.cuh"
 
 namespace colib {
@@ -17,43 +16,6 @@ namespace colib {
 //   a = largest |x| of a block's non-NaN values, s = 1 if a == 0 else max(a / 448, 2^-126), code = e4m3(x / s)
 // to nearest even, saturating; a NaN keeps a NaN code, and an infinity makes s infinite and its own code NaN, so
 // that either shows in every product with the row.
-//
-// Both quotients are the correctly rounded ones: bf16 rows have many values exactly half-way between two codes, where
-// a product with a rounded reciprocal falls to either side.  With y = 1 / b rounded to nearest and q within a unit of a / b,
-// q + (a - q b) y rounds to the quotient (Markstein, IBM J. Res. Dev. 34, 1990): two FMAs, where a division
-// is ten instructions and a branch (32768 rows of 7168 bf16: 287 us with divisions next to a border only).
-__device__ __forceinline__ float quotient(float a, float b, float y) {
-  const float q = a * y;
-  return fmaf(fmaf(-q, b, a), y, q);
-}
-// two quotients by the same b at once
-__device__ __forceinline__ float2 quotients(float2 a, float b, float y) {
-  uint64_t q, r, a2, nb, y2;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(a2) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(nb) : "f"(-b));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(y2) : "f"(y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a2), "l"(y2));
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a2));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(r), "l"(y2));
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(q));
-  return d;
-}
-__device__ __forceinline__ float row_scale(float a) {
-  constexpr float TINY = 1.17549435e-38f;              // 2^-126
-  const float s = fmaxf(quotient(a, 448.0f, 1.0f / 448.0f), TINY);
-  if (!(a >= 7.8886090522e-31f && a <= 3.4028235e38f))  // (the remainder is exact from 2^-100 up; none of an infinity)
-    return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), TINY) : 1.0f;
-  return s;
-}
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  uint16_t d;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
-__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) { return e4m3x4(a.x, a.y, b.x, b.y); }
-
 // Eight lanes share a block, 16 columns each in pieces of 16 bytes; a warp takes QR_STEPS times four blocks of a row and
 // goes through the rows with the next one's pieces already requested; the warps of a CTA take neighbouring rows, whose
 // scales of a block lie side by side.
@@ -197,7 +159,6 @@ int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
 constexpr int F8_BM = 128;
 constexpr int F8_EPI_WARPS = 8;
 constexpr int F8_THREADS = (F8_EPI_WARPS + 2) * 32;
-constexpr int F8_MAX_SEGS = 520;
 constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
 struct F8Maps {
   CUtensorMap m[F8_MAPS];
@@ -218,10 +179,6 @@ struct F8Smem {
   static constexpr int BYTES = 1024 + RING + 8 * BARS + 16 + TABLES + 2 * 2 * F8_BM * 4;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc),
@@ -243,39 +200,6 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
-
-struct F8Tile {
-  int seg, nt, row0, nrows;
-};
-// Tile t of the call: segments in order, a segment's feature tiles in order, its row tiles inside one (they share the
-// weights in L2).
-__device__ __forceinline__ F8Tile f8_tile(const int *tile_off, const int *row_off, int nseg, int t) {
-  int lo = 0, hi = nseg;  // tile_off[lo] <= t < tile_off[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (tile_off[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const int n = row_off[lo + 1] - row_off[lo], mt = (n + F8_BM - 1) / F8_BM, l = t - tile_off[lo];
-  F8Tile r;
-  r.seg = lo;
-  r.nt = l / mt;
-  const int m = l - r.nt * mt;
-  r.row0 = row_off[lo] + m * F8_BM;
-  r.nrows = min(F8_BM, n - m * F8_BM);
-  return r;
-}
-
-template <typename OutT>
-__device__ __forceinline__ OutT f8_out(float v);
-template <>
-__device__ __forceinline__ float f8_out<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half f8_out<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 f8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // Stores N consecutive values of one row; `valid` of them exist.
 template <typename OutT, int N>
@@ -317,7 +241,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   int *tile_off = row_off + F8_MAX_SEGS + 1;
   float *amax_s = reinterpret_cast<float *>(tile_off + F8_MAX_SEGS + 1);  // [tile parity][half][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int *status = p.status ? p.status : &g_fp8_status;
+  int *status = p.status;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -337,36 +261,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     tc_fence_before();
   }
   coli_grid_dependency_sync();  // (the set-up above overlaps the predecessor's end)
-  // rows and tiles before every segment; counts that run past the buffer are cut
-  const int NT = p.n_tiles;
-  if (warp == 0) {
-    int rows = 0, tiles = 0;
-    for (int s0 = 0; s0 < p.nseg; s0 += 32) {
-      const int s = s0 + lane;
-      int n = s < p.nseg ? max(0, p.seg_count ? p.seg_count[s] : p.rows) : 0, incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl = (int)min((long)incl + u, (long)p.rows);
-      }
-      const int end = min(p.rows, (int)min((long)rows + incl, (long)p.rows));
-      int prev = __shfl_up_sync(0xffffffffu, end, 1);
-      if (lane == 0) prev = rows;
-      int t = (end - prev + F8_BM - 1) / F8_BM * NT;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += u;
-      }
-      if (s < p.nseg) {
-        row_off[s + 1] = end;
-        tile_off[s + 1] = tiles + t;
-      }
-      rows = __shfl_sync(0xffffffffu, end, 31);
-      tiles += __shfl_sync(0xffffffffu, t, 31);
-    }
-    if (lane == 0) row_off[0] = tile_off[0] = 0;
-  }
+  if (warp == 0) f8_tables<F8_BM>(p, row_off, tile_off, lane);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -379,7 +274,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   uint32_t it = 0;  // k-tiles so far: the ring's and the TMEM buffers' place and phase follow from it
   bool alive = true;
   for (int t = cluster0; t < n_tiles; t += clusters) {
-    const F8Tile tile = f8_tile(tile_off, row_off, p.nseg, t);
+    const F8Tile tile = f8_tile<F8_BM>(tile_off, row_off, p.nseg, t);
     const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
     if (warp == F8_EPI_WARPS) {
       // ---------------- copies ----------------
@@ -618,12 +513,14 @@ static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int
 
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   if (p.rows == 0 || p.nseg == 0) return 1;
+  if (!p.status && !(p.status = fp8_status_word())) return 0;
   if (p.nseg > F8_MAX_SEGS) {
     coli_set_error("fp8 product: %d segments (at most %d)", p.nseg, F8_MAX_SEGS);
     return 0;
   }
   p.KT = (p.K + 127) / 128;
   p.Op = round_up(p.O, 16);
+  if (p.h32 || fp8_stream_ok(p)) return launch_fp8_stream(p, st);
   const bool gated = p.h_codes != nullptr;
   // Row tiles the call is likely to have, and the most it can have.  Both are functions of the call's shapes alone.
   const int most = p.seg_count ? p.rows / F8_BM + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + F8_BM - 1) / F8_BM;
@@ -654,10 +551,23 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   return launch_f8_shape<false, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);
 }
 
+// Device address of the current device's status word, looked up once per device (as the routing scratch is).
+static int *g_fp8_status_addr[COLI_CUDA_MAX_DEVICES];
+int *fp8_status_word() {
+  int dev = -1;
+  if (!coli_cuda_check(cudaGetDevice(&dev), "fp8 status: cudaGetDevice") || dev < 0 || dev >= COLI_CUDA_MAX_DEVICES) return nullptr;
+  int *at = __atomic_load_n(&g_fp8_status_addr[dev], __ATOMIC_ACQUIRE);
+  if (!at) {
+    if (!coli_cuda_check(cudaGetSymbolAddress((void **)&at, g_fp8_status), "fp8 status: cudaGetSymbolAddress")) return nullptr;
+    __atomic_store_n(&g_fp8_status_addr[dev], at, __ATOMIC_RELEASE);
+  }
+  return at;
+}
 int fp8_take_status(int *code) {
-  CK(cudaMemcpyFromSymbol(code, g_fp8_status, sizeof(int)), "fp8 status read");
-  const int zero = 0;
-  if (*code) CK(cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int)), "fp8 status clear");
+  int *at = fp8_status_word();
+  if (!at) return 0;
+  CK(cudaMemcpy(code, at, sizeof(int), cudaMemcpyDeviceToHost), "fp8 status read");
+  if (*code) CK(cudaMemset(at, 0, sizeof(int)), "fp8 status clear");
   return 1;
 }
 

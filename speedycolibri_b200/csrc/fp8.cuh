@@ -36,12 +36,22 @@ struct Fp8MmParams {
   uint8_t *h_codes;          // when not null: h = act(w0 x, w1 x) quantised again: codes [rows, O], h_ld bytes apart,
   float *h_scales;           // and scales [ceil(O / 128)][rows]
   long h_ld;
+  float *h32;                // segments of a few rows: h as it is, f32 [rows, O or K]: written instead of h_codes when w1 is
+                             // given, and otherwise read in place of codes and quantised on the way, behind the call that wrote it
   ActParams act;
   int *status;               // device word for a bounded wait that gave up, or null: the library's own
   // filled in by the launcher
   int KT, Op, n_tiles, split;
 };
+// Whether segments are short enough for the streaming kernel (fp8_stream.cu).  A function of shapes alone.
+static inline bool fp8_stream_ok(const Fp8MmParams &p) {
+  if (!p.seg_count) return p.rows <= 16;
+  const int segs = p.rows_expected < p.nseg ? p.rows_expected : p.nseg;
+  return p.rows_expected <= 6L * segs;
+}
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st);
-int fp8_take_status(int *code);  // the library's own status word of the current device, cleared when set
+int launch_fp8_stream(Fp8MmParams p, cudaStream_t st);  // called by launch_fp8_mm
+int *fp8_status_word();          // the library's own status word on the current device
+int fp8_take_status(int *code);  // its value, and cleared when set
 
 }  // namespace colib

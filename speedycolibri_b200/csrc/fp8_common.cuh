@@ -1,0 +1,115 @@
+// Device pieces that the FP8 row kernels share: the quantiser's arithmetic, the tables of segments and tiles, bulk copies.
+#pragma once
+#include "fp8.cuh"
+
+namespace colib {
+
+constexpr int F8_MAX_SEGS = 520;
+
+// Both quotients are the correctly rounded ones: bf16 rows have many values exactly half-way between two codes, where
+// a product with a rounded reciprocal falls to either side.  With y = 1 / b rounded to nearest and q within a unit of a / b,
+// q + (a - q b) y rounds to the quotient (Markstein, IBM J. Res. Dev. 34, 1990): two FMAs, where a division
+// is ten instructions and a branch (32768 rows of 7168 bf16: 287 us with divisions next to a border only).
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+  const float q = a * y;
+  return fmaf(fmaf(-q, b, a), y, q);
+}
+// two quotients by the same b at once
+__device__ __forceinline__ float2 quotients(float2 a, float b, float y) {
+  uint64_t q, r, a2, nb, y2;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a2) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(nb) : "f"(-b));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y2) : "f"(y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a2), "l"(y2));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a2));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(r), "l"(y2));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(q));
+  return d;
+}
+__device__ __forceinline__ float row_scale(float a) {
+  constexpr float TINY = 1.17549435e-38f;              // 2^-126
+  const float s = fmaxf(quotient(a, 448.0f, 1.0f / 448.0f), TINY);
+  if (!(a >= 7.8886090522e-31f && a <= 3.4028235e38f))  // (the remainder is exact from 2^-100 up; none of an infinity)
+    return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), TINY) : 1.0f;
+  return s;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) { return e4m3x4(a.x, a.y, b.x, b.y); }
+
+// `bytes` (a multiple of 16) in a row, global -> shared memory, counted by the barrier
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+template <typename OutT>
+__device__ __forceinline__ OutT f8_out(float v);
+template <>
+__device__ __forceinline__ float f8_out<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half f8_out<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 f8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+struct F8Tile {
+  int seg, nt, row0, nrows;
+};
+// Rows and tiles before every segment, by one warp; counts that run past the buffer are cut.
+template <int BM>
+__device__ __forceinline__ void f8_tables(const Fp8MmParams &p, int *row_off, int *tile_off, int lane) {
+  int rows = 0, tiles = 0;
+  for (int s0 = 0; s0 < p.nseg; s0 += 32) {
+    const int s = s0 + lane;
+    int incl = s < p.nseg ? max(0, p.seg_count ? p.seg_count[s] : p.rows) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl = (int)min((long)incl + u, (long)p.rows);
+    }
+    const int end = (int)min((long)rows + incl, (long)p.rows);
+    int prev = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) prev = rows;
+    int t = (end - prev + BM - 1) / BM * p.n_tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += u;
+    }
+    if (s < p.nseg) {
+      row_off[s + 1] = end;
+      tile_off[s + 1] = tiles + t;
+    }
+    rows = __shfl_sync(0xffffffffu, end, 31);
+    tiles += __shfl_sync(0xffffffffu, t, 31);
+  }
+  if (lane == 0) row_off[0] = tile_off[0] = 0;
+}
+// Tile t of the call, BM rows by one feature tile: segments in order, a segment's feature tiles in order, its row tiles
+// inside one (they share the weights in L2).
+template <int BM>
+__device__ __forceinline__ F8Tile f8_tile(const int *tile_off, const int *row_off, int nseg, int t) {
+  int lo = 0, hi = nseg;  // tile_off[lo] <= t < tile_off[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tile_off[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int n = row_off[lo + 1] - row_off[lo], mt = (n + BM - 1) / BM, l = t - tile_off[lo];
+  F8Tile r;
+  r.seg = lo;
+  r.nt = l / mt;
+  const int m = l - r.nt * mt;
+  r.row0 = row_off[lo] + m * BM;
+  r.nrows = min(BM, n - m * BM);
+  return r;
+}
+
+}  // namespace colib

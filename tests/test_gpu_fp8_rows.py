@@ -112,7 +112,8 @@ def product_bound(q, s, w, want, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("T,K,O", [(1, 1, 1), (1, 128, 128), (1, 1024, 2048), (2, 300, 257), (8, 4096, 130), (31, 1000, 1111), (128, 256, 256),
+@pytest.mark.parametrize("T,K,O", [(1, 1, 1), (1, 128, 128), (1, 1024, 2048), (2, 300, 257), (8, 4096, 130), (9, 300, 4500), (16, 2048, 5000),
+                                   (7, 200, 80000), (31, 1000, 1111), (128, 256, 256),
                                    (129, 384, 512), (333, 1000, 1111), (700, 640, 1000), (3000, 256, 2048)])
 def test_product(gpu_backend, dtype, T, K, O):
     w, wv = weight(gpu_backend, O, K, 5)
@@ -192,7 +193,8 @@ def expert_rows(q, s, counts, values):
 
 @pytest.mark.parametrize("E,H,I,counts", [
     (1, 8, 8, [1]), (4, 64, 32, [0, 3, 0, 2]), (3, 256, 136, [1, 1, 1]), (8, 1024, 256, [1] * 8), (5, 320, 192, [130, 0, 7, 257, 1]),
-    (6, 520, 264, [128, 129, 127, 0, 1, 300]), (16, 512, 512, [40] * 16), (40, 128, 128, [3, 0] * 20)])
+    (6, 520, 264, [128, 129, 127, 0, 1, 300]), (16, 512, 512, [40] * 16), (40, 128, 128, [3, 0] * 20),
+    (64, 1024, 136, [1] * 60 + [17, 0, 9, 2]), (12, 264, 520, [6] * 12), (300, 136, 264, [0, 1, 5] * 100)])
 def test_experts(gpu_backend, E, H, I, counts):
     R = sum(counts)
     block, values = expert_layer(gpu_backend, E, H, I, R)
@@ -222,8 +224,9 @@ def test_rows_behind_the_last_segment_stay(gpu_backend, expected):
     block.close()
 
 
+@pytest.mark.parametrize("expected", [1, 20])
 @pytest.mark.parametrize("counts", [[5, 100, 5], [-3, 8, 2**31 - 1], [2**31 - 1, 2**31 - 1, 1], [0, 0, 0]])
-def test_counts_past_the_buffer_are_cut(gpu_backend, counts):
+def test_counts_past_the_buffer_are_cut(gpu_backend, counts, expected):
     H, R = 128, 20
     block, _ = expert_layer(gpu_backend, 3, H, 64, R)
     q, s = gpu_backend.quantize_rows_fp8_dev(rows(R, H, 32))
@@ -232,8 +235,8 @@ def test_counts_past_the_buffer_are_cut(gpu_backend, counts):
         cut.append(min(max(n, 0), left))
         left -= cut[-1]
     y, want = (torch.full((R, H), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
-    block.experts_fp8_dev(q, s, torch.tensor(counts, dtype=torch.int32, device="cuda"), R, y)
-    block.experts_fp8_dev(q, s, torch.tensor(cut, dtype=torch.int32, device="cuda"), R, want)
+    block.experts_fp8_dev(q, s, torch.tensor(counts, dtype=torch.int32, device="cuda"), expected, y)
+    block.experts_fp8_dev(q, s, torch.tensor(cut, dtype=torch.int32, device="cuda"), expected, want)
     block.check()
     assert torch.equal(y, want) and (y[R - left :] == 3.0).all()
     block.close()
