@@ -158,25 +158,40 @@ int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
 // The scales are arbitrary f32, which the block-scaled MMA kinds do not take.
 constexpr int F8_BM = 128;
 constexpr int F8_EPI_WARPS = 8;
-constexpr int F8_THREADS = (F8_EPI_WARPS + 2) * 32;
+constexpr int F8_THREADS = (F8_EPI_WARPS + 4) * 32;  // (two warps stand by: registers are moved between whole warpgroups)
+// 168 registers a thread at launch are 64512; the summing warps take 208 of them each, the others keep 88: all of them.
+constexpr int F8_REGS_SUM = 208, F8_REGS_OTHER = 88;
 constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
 struct F8Maps {
   CUtensorMap m[F8_MAPS];
 };
 static __device__ int g_fp8_status;  // of products without a handle of their own
 
+// What the roles need to know of a tile, looked up ahead of them by a warp of its own.
+struct F8Info {
+  const uint8_t *q0, *q1;  // codes of the tile's first feature, k-tile 0
+  const float *s0, *s1;    // scales of its first block of features
+  int nt, row0, nrows, pad;
+};
+constexpr int F8_INFOS = 4;
+constexpr int F8_CHUNK = 8;   // k-tiles whose scales are handed over at once
 template <int BN>
 struct F8Smem {
   static constexpr int A_BYTES = F8_BM * 128;
   static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int STAGES = BN == 256 ? 3 : 5;
   static constexpr int RED_LD = BN + 4;  // f32 a row of partial sums: rows start 4 banks apart
   static constexpr int RING = STAGES * STAGE;
   static_assert(F8_BM * RED_LD * 4 <= RING, "partial sums take the ring's place");
-  static constexpr int BARS = 2 * STAGES + 4;
+  static constexpr int OUT_LD = 128 + 16;  // bytes a row of a warp's staged results: rows start 4 banks apart
+  static constexpr int OUT = F8_EPI_WARPS * 32 * OUT_LD;
+  static constexpr int INFOS = F8_INFOS * (int)sizeof(F8Info);
+  static constexpr int SCALES = 2 * F8_CHUNK * (F8_BM + 2) * 4;  // two chunks: [k-tile][row] of sx, then [k-tile][block of features] of sw
+  static constexpr int BARS = 2 * STAGES + 4 + 2 * F8_INFOS + 4;
   static constexpr int TABLES = 2 * (F8_MAX_SEGS + 1) * 4;
-  static constexpr int BYTES = 1024 + RING + 8 * BARS + 16 + TABLES + 2 * 2 * F8_BM * 4;
+  static constexpr int BYTES = 1024 + RING + OUT + INFOS + SCALES + 8 * BARS + 16 + TABLES + 2 * 2 * F8_BM * 4;
+  static_assert(BYTES <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -201,24 +216,119 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-// Stores N consecutive values of one row; `valid` of them exist.
+// Four consecutive values of one row; `valid` of them exist.
+template <typename OutT>
+__device__ __forceinline__ void f8_store4(OutT *dst, const float (&v)[4], int valid, bool vec) {
+  alignas(16) OutT o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = f8_out<OutT>(v[i]);
+  if (vec && valid >= 4) {
+    if constexpr (sizeof(OutT) == 4)
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(o);
+    else
+      *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) dst[j] = o[j];
+  }
+}
+// A warp's 32 rows x N columns, a row in each lane, to y: 128 bytes of every row at a time through shared memory, so that a
+// store instruction writes whole lines of four rows (lane by lane it is 32 lines of 16 bytes: 5600 cycles a tile of 128 x 256,
+// of 16 k-tiles at 1180).
 template <typename OutT, int N>
-__device__ __forceinline__ void f8_store(OutT *dst, const float *v, int valid, bool vec) {
-  constexpr int PER = 16 / (int)sizeof(OutT) < N ? 16 / (int)sizeof(OutT) : N;
-  alignas(16) OutT o[N];
+__device__ __forceinline__ void f8_store_rows(unsigned char *stage, OutT *y, long stride, const float *acc, int rows, int cols, bool vec, int lane) {
+  constexpr int LD = F8Smem<256>::OUT_LD, PER = 16 / (int)sizeof(OutT), CH = 128 / (int)sizeof(OutT);
+  const uint32_t at = smem_u32(stage);
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = f8_out<OutT>(v[i]);
+  for (int c = 0; c < N / CH; ++c) {
+    if (c * CH >= cols) break;
 #pragma unroll
-  for (int i = 0; i < N; i += PER) {
-    if (vec && i + PER <= valid) {
-      if constexpr (PER * sizeof(OutT) == 16)
-        *reinterpret_cast<uint4 *>(dst + i) = *reinterpret_cast<const uint4 *>(o + i);
-      else
-        *reinterpret_cast<uint2 *>(dst + i) = *reinterpret_cast<const uint2 *>(o + i);
-    } else {
+    for (int i = 0; i < 8; ++i) {
+      alignas(16) OutT o[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (i + j < valid) dst[i + j] = o[i + j];
+      for (int j = 0; j < PER; ++j) o[j] = f8_out<OutT>(acc[c * CH + i * PER + j]);
+      *reinterpret_cast<uint4 *>(stage + lane * LD + 16 * i) = *reinterpret_cast<const uint4 *>(o);
+    }
+    __syncwarp();
+    const int col = c * CH + (lane & 7) * PER;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      const uint4 v = lds128(at + (uint32_t)(r * LD + 16 * (lane & 7)));
+      if (r < rows) {
+        OutT *dst = y + (long)r * stride + col;
+        if (vec && col + PER <= cols) {
+          *reinterpret_cast<uint4 *>(dst) = v;
+        } else {
+          const OutT *o = reinterpret_cast<const OutT *>(&v);
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (col + j < cols) dst[j] = o[j];
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// c += (x, y) * s
+__device__ __forceinline__ void f8_add_scaled(float2 &c, float x, float y, float s) {
+  uint64_t cc, v, ss;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(cc) : "f"(c.x), "f"(c.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(cc) : "l"(v), "l"(ss));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(c.x), "=f"(c.y) : "l"(cc));
+}
+
+// One warp sums row i of the tile over the CTAs of the cluster and writes what becomes of it.
+template <bool GATED, int BN, typename OutT>
+__device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &tile, uint32_t red, int world, int i, int lane) {
+  float4 v[BN / 128];
+#pragma unroll
+  for (int j = 0; j < BN / 128; ++j) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int r = 0; r < world; ++r) {
+#pragma unroll
+    for (int j = 0; j < BN / 128; ++j) {
+      const float4 u = ld_cluster4(red + (uint32_t)(i * F8Smem<BN>::RED_LD + 128 * j + 4 * lane) * 4u, (uint32_t)r);
+      v[j].x += u.x;
+      v[j].y += u.y;
+      v[j].z += u.z;
+      v[j].w += u.w;
+    }
+  }
+  if constexpr (GATED) {
+    const int f = tile.nt * 128 + 4 * lane;
+    const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+    float h[4], a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = f + j < p.O ? coli_act_fast(g[j], u[j], p.act) : 0.0f;
+      a = fmaxf(a, fabsf(h[j]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
+    if (f < p.h_ld) *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)(tile.row0 + i) * p.h_ld + f) = e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+    if (lane == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + i] = s;
+  } else {
+#pragma unroll
+    for (int j = 0; j < BN / 128; ++j) {
+      const int f = tile.nt * BN + 128 * j + 4 * lane;
+      const float o[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      if (f < p.O) f8_store4<OutT>((OutT *)p.y + (long)(tile.row0 + i) * p.y_stride + f, o, p.O - f, p.y_vec);
     }
   }
 }
@@ -233,8 +343,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = smem_u32(smem);
-  unsigned char *after = smem + S::RING;
+  F8Info *infos = reinterpret_cast<F8Info *>(smem + S::RING + S::OUT);
+  float *scales = reinterpret_cast<float *>(infos + F8_INFOS);
+  unsigned char *after = smem + S::RING + S::OUT + S::INFOS + S::SCALES;
   const uint32_t full = smem_u32(after), empty = full + 8 * S::STAGES, dfull = empty + 8 * S::STAGES, dempty = dfull + 16;
+  const uint32_t known = dempty + 16, forgotten = known + 8 * F8_INFOS;
+  const uint32_t scaled = forgotten + 8 * F8_INFOS, unscaled = scaled + 16;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(after + 8 * S::BARS);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *row_off = reinterpret_cast<int *>(after + 8 * S::BARS + 16);
@@ -251,6 +365,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     for (int b = 0; b < 2; ++b) {
       mbar_init(dfull + 8 * b, 1);
       mbar_init(dempty + 8 * b, F8_EPI_WARPS);
+    }
+    for (int i = 0; i < F8_INFOS; ++i) {
+      mbar_init(known + 8 * i, 1);
+      mbar_init(forgotten + 8 * i, F8_EPI_WARPS + 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(scaled + 8 * i, 1);
+      mbar_init(unscaled + 8 * i, F8_EPI_WARPS);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -270,99 +392,210 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   const int world = SPLIT ? p.split : 1;
   const int cluster0 = (int)blockIdx.x / world, clusters = (int)gridDim.x / world;
   const int kb0 = SPLIT ? (int)((long)p.KT * rank / world) : 0, kb1 = SPLIT ? (int)((long)p.KT * (rank + 1) / world) : p.KT;
-
-  uint32_t it = 0;  // k-tiles so far: the ring's and the TMEM buffers' place and phase follow from it
+  // the CTAs of a cluster meet twice a tile: sums written, sums read
+  auto meet = [&] {
+    if constexpr (SPLIT) cluster_sync();
+  };
+  uint32_t it = 0;   // k-tiles so far: the ring's and the TMEM buffers' place and phase follow from it
+  uint32_t nth = 0;  // tiles so far
   bool alive = true;
-  for (int t = cluster0; t < n_tiles; t += clusters) {
-    const F8Tile tile = f8_tile<F8_BM>(tile_off, row_off, p.nseg, t);
-    const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+  // the nth tile of this CTA, as a reader; every lane must have it before the warp forgets it
+  auto recall = [&](F8Info &i) {
+    const uint32_t s = nth % F8_INFOS, ph = (nth / F8_INFOS) & 1u;
+    alive = alive && __all_sync(0xffffffffu, mbar_wait(known + 8 * s, ph, abort_flag, status, TC_ERR_TMA_WAIT));
+    i = infos[s];
+    if (!alive) i.nrows = 0;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(forgotten + 8 * s);
+    ++nth;
+  };
+
+  if (warp >= F8_EPI_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_REGS_OTHER));
     if (warp == F8_EPI_WARPS) {
       // ---------------- copies ----------------
-      const uint8_t *q0 = p.w0 ? p.w0[ex].q : p.one.q, *q1 = GATED ? p.w1[ex].q : q0;
-      const int f0 = tile.nt * (GATED ? 128 : BN);
-      const uint32_t nb0 = (uint32_t)min(GATED ? 128 : BN, p.Op - f0) * 128u, nb1 = GATED ? nb0 : 0u;
-      int box = 0;
-      while ((8 << box) < tile.nrows) ++box;
-      const uint32_t bytes = (uint32_t)(8 << box) * 128u + nb0 + nb1;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u;
-        alive = alive && __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
-        if (alive && elect_one()) {
-          const uint32_t a = ring + s * S::STAGE, b = a + S::A_BYTES, bar = full + 8 * s;
-          mbar_expect_tx(bar, bytes);
-          tma_load_2d(a, &maps.m[box], kb * 128, tile.row0, bar);
-          const size_t at = ((size_t)kb * p.Op + f0) * 128;
-          bulk_load(b, q0 + at, nb0, bar);
-          if (GATED) bulk_load(b + 128 * 128, q1 + at, nb1, bar);
+      for (int t = cluster0; t < n_tiles; t += clusters) {
+        F8Info tile;
+        recall(tile);
+        const int f0 = tile.nt * (GATED ? 128 : BN);
+        const uint32_t nb = (uint32_t)min(GATED ? 128 : BN, p.Op - f0) * 128u;
+        int box = 0;
+        while ((8 << box) < tile.nrows) ++box;
+        const uint32_t bytes = (uint32_t)(8 << box) * 128u + (GATED ? 2 * nb : nb);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u;
+          alive = alive && __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
+          if (alive && elect_one()) {
+            const uint32_t a = ring + s * S::STAGE, b = a + S::A_BYTES, bar = full + 8 * s;
+            mbar_expect_tx(bar, bytes);
+            tma_load_2d(a, &maps.m[box], kb * 128, tile.row0, bar);
+            const size_t at = (size_t)kb * p.Op * 128;
+            bulk_load(b, tile.q0 + at, nb, bar);
+            if (GATED) bulk_load(b + 128 * 128, tile.q1 + at, nb, bar);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        meet();
+        meet();
+      }
+      if (*abort_flag) {
+        // copies already issued still land in this CTA's shared memory: give them time before exit
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
       }
     } else if (warp == F8_EPI_WARPS + 1) {
       // ---------------- products ----------------
       // kind::f8f6f4: D = f32, A = B = e4m3 (format code 0), both K-major
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(F8_BM >> 4) << 24);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u, d = it & 1u, dph = (it >> 1) & 1u;
-        alive = alive && __all_sync(0xffffffffu, mbar_wait(dempty + 8 * d, dph ^ 1u, abort_flag, status, TC_ERR_MMA_WAIT));
-        alive = alive && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, status, TC_ERR_MMA_WAIT));
-        tc_fence_after();
-        if (alive && elect_one()) {
-          const uint32_t a = ring + s * S::STAGE;
-          const uint64_t ad = umma_smem_desc(a), bd = umma_smem_desc(a + S::A_BYTES);
+      for (int t = cluster0; t < n_tiles; t += clusters) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u, d = it & 1u, dph = (it >> 1) & 1u;
+          alive = alive && __all_sync(0xffffffffu, mbar_wait(dempty + 8 * d, dph ^ 1u, abort_flag, status, TC_ERR_MMA_WAIT));
+          alive = alive && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, status, TC_ERR_MMA_WAIT));
+          tc_fence_after();
+          if (alive && elect_one()) {
+            const uint32_t a = ring + s * S::STAGE;
+            const uint64_t ad = umma_smem_desc(a), bd = umma_smem_desc(a + S::A_BYTES);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f8(tmem + d * BN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
-          umma_commit(empty + 8 * s);
-          umma_commit(dfull + 8 * d);
+            for (int k = 0; k < 4; ++k) umma_f8(tmem + d * BN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
+            umma_commit(empty + 8 * s);
+            umma_commit(dfull + 8 * d);
+          }
+          __syncwarp();
+        }
+        meet();
+        meet();
+      }
+    } else if (warp == F8_EPI_WARPS + 2) {
+      // ---------------- tiles ahead ----------------
+      for (int t = cluster0; t < n_tiles; t += clusters, ++nth) {
+        const uint32_t s = nth % F8_INFOS, ph = (nth / F8_INFOS) & 1u;
+        const F8Tile tile = f8_tile<F8_BM>(tile_off, row_off, p.nseg, t);
+        const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+        const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
+        const int f0 = tile.nt * (GATED ? 128 : BN);
+        F8Info i;
+        i.q0 = w0.q + (size_t)f0 * 128;
+        i.q1 = w1.q + (size_t)f0 * 128;
+        i.s0 = reinterpret_cast<const float *>(w0.s) + (size_t)(f0 >> 7) * p.KT;
+        i.s1 = reinterpret_cast<const float *>(w1.s) + (size_t)(f0 >> 7) * p.KT;
+        i.nt = tile.nt;
+        i.row0 = tile.row0;
+        i.nrows = tile.nrows;
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(forgotten + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
+        if (alive && lane == 0) {
+          infos[s] = i;
+          mbar_arrive(known + 8 * s);
         }
         __syncwarp();
+        meet();
+        meet();
       }
     } else {
-      // ---------------- scaled sums ----------------
-      const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-      const bool any = (warp & 3) * 32 < tile.nrows, mine = row < tile.nrows;
-      const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const float *w0s = reinterpret_cast<const float *>(p.w0 ? p.w0[ex].s : p.one.s);
-      const float *w1s = GATED ? reinterpret_cast<const float *>(p.w1[ex].s) : nullptr;
-      const int fb = GATED ? tile.nt : min((tile.nt * BN + half * NACC) >> 7, (p.O - 1) >> 7);
-      w0s += (size_t)fb * p.KT;
-      if (GATED) w1s += (size_t)fb * p.KT;
-      const float *sx = p.sx + (long)(tile.row0 + (mine ? row : 0)) * p.s_row;
-      float acc[NACC];
+      // ---------------- scales: sx of the tile's rows, sw of its one or two blocks of features ----------------
+      for (int t = cluster0; t < n_tiles; t += clusters) {
+        F8Info tile;
+        recall(tile);
+        // (a second block past the end has no scales, and is not stored)
+        const float *sw = (lane & 1) == 0 ? tile.s0 : GATED ? tile.s1 : BN == 256 && tile.nt * BN + 128 < p.O ? tile.s0 + p.KT : tile.s0;
+        const float *sx[4];
 #pragma unroll
-      for (int i = 0; i < NACC; ++i) acc[i] = 0.0f;
-      float nx = 0.0f, nw0 = 0.0f, nw1 = 0.0f;
-      if (any && kb0 < kb1) {
-        nx = __ldg(sx + (long)kb0 * p.s_blk);
-        nw0 = __ldg(w0s + kb0);
-        if (GATED) nw1 = __ldg(w1s + kb0);
+        for (int j = 0; j < 4; ++j) sx[j] = p.sx + (long)(tile.row0 + min(lane + 32 * j, max(tile.nrows, 1) - 1)) * p.s_row;
+        for (int kb = kb0; kb < kb1; kb += F8_CHUNK, ++it) {
+          float x[F8_CHUNK][4];
+          const float w = lane < 2 * F8_CHUNK ? __ldg(sw + min(kb + (lane >> 1), kb1 - 1)) : 0.0f;
+#pragma unroll
+          for (int u = 0; u < F8_CHUNK; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][j] = kb + u < kb1 ? __ldg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
+          const uint32_t s = it & 1u, ph = (it >> 1) & 1u;
+          alive = alive && __all_sync(0xffffffffu, mbar_wait(unscaled + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
+          if (alive) {
+            float *at = scales + s * F8_CHUNK * (F8_BM + 2);
+#pragma unroll
+            for (int u = 0; u < F8_CHUNK; ++u)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) at[u * F8_BM + lane + 32 * j] = x[u][j];
+            if (lane < 2 * F8_CHUNK) at[F8_CHUNK * F8_BM + lane] = w;
+          }
+          __syncwarp();
+          if (alive && lane == 0) mbar_arrive(scaled + 8 * s);
+        }
+        meet();
+        meet();
       }
+    }
+  } else {
+    // ---------------- scaled sums ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    F8Info tile;
+    tile.nrows = 0;
+    uint32_t chunk = 0;  // of scales, so far
+    float nx = 0.0f, nw0 = 0.0f, nw1 = 0.0f;
+    // This thread's scales of k-tile kb, requested a k-tile ahead: beside the products' operands a read of shared memory takes
+    // two to three hundred cycles.
+    auto scales_of = [&](int kb) {
+      const uint32_t u = (uint32_t)(kb - kb0) % F8_CHUNK;
+      if (u == 0) alive = alive && __all_sync(0xffffffffu, mbar_wait(scaled + 8 * (chunk & 1u), (chunk >> 1) & 1u, abort_flag, status, TC_ERR_EPI_WAIT));
+      const float *at = scales + (chunk & 1u) * (F8_CHUNK * (F8_BM + 2));
+      nx = at[u * F8_BM + row];
+      nw0 = at[F8_CHUNK * F8_BM + 2 * u + (GATED || BN == 128 ? 0 : half)];
+      if (GATED) nw1 = at[F8_CHUNK * F8_BM + 2 * u + 1];
+      if (u == F8_CHUNK - 1 || kb + 1 == kb1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(unscaled + 8 * (chunk & 1u));
+        ++chunk;
+      }
+    };
+    if (cluster0 < n_tiles) {
+      recall(tile);
+      scales_of(kb0);
+    }
+    for (int t = cluster0; t < n_tiles; t += clusters) {
+      const bool any = (warp & 3) * 32 < tile.nrows;
+      float2 acc[NACC / 2];
+#pragma unroll
+      for (int i = 0; i < NACC / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t d = it & 1u, dph = (it >> 1) & 1u;
         const float s0 = nx * nw0, s1 = GATED ? nx * nw1 : s0;
-        if (any && kb + 1 < kb1) {
-          nx = __ldg(sx + (long)(kb + 1) * p.s_blk);
-          nw0 = __ldg(w0s + kb + 1);
-          if (GATED) nw1 = __ldg(w1s + kb + 1);
-        }
+        if (kb + 1 < kb1) scales_of(kb + 1);
         alive = alive && __all_sync(0xffffffffu, mbar_wait(dfull + 8 * d, dph, abort_flag, status, TC_ERR_EPI_WAIT));
         tc_fence_after();
         if (any && alive) {
-          uint32_t v[2][16];
-          auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < NACC / 32 ? 64 * half + 16 * c : 128 + 64 * half + 16 * (c - NACC / 32)) : half * NACC + 16 * c); };
-          tmem_ld16(column(0), v[0]);
+          // FLY loads of 16 columns at a time, the next ones requested as each is added, so that the buffer goes back to the
+          // products after few round trips (with 64 columns on their way the sums no longer fit the registers); two sums an
+          // instruction.
+          constexpr int CH = NACC / 16, FLY = CH == 8 ? 3 : 4;
+          uint32_t v[FLY][16];
+          auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < CH / 2 ? 64 * half + 16 * c : 128 + 64 * half + 16 * (c - CH / 2)) : half * NACC + 16 * c); };
 #pragma unroll
-          for (int c = 0; c < NACC / 16; ++c) {
+          for (int c = 0; c < FLY; ++c) tmem_ld16(column(c), v[c]);
+#pragma unroll
+          for (int c0 = 0; c0 < CH; c0 += FLY) {
             tmem_ld_wait();
-            if (c + 1 < NACC / 16) tmem_ld16(column(c + 1), v[(c + 1) & 1]);
-            const float s = GATED && c >= NACC / 32 ? s1 : s0;
+            if (c0 + FLY >= CH) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(dempty + 8 * d);
+            }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[16 * c + i]);
+            for (int c = c0; c < c0 + FLY && c < CH; ++c) {
+              const float s = GATED && c >= CH / 2 ? s1 : s0;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f8_add_scaled(acc[8 * c + i], __uint_as_float(v[c - c0][2 * i]), __uint_as_float(v[c - c0][2 * i + 1]), s);
+              if (c + FLY < CH) tmem_ld16(column(c + FLY), v[c - c0]);
+            }
           }
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(dempty + 8 * d);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dempty + 8 * d);
       }
+      float *flat = reinterpret_cast<float *>(acc);
+      const bool mine = row < tile.nrows;
       if constexpr (SPLIT) {
         // partial sums into the ring's place: its last copies have been multiplied
         float *red = reinterpret_cast<float *>(smem);
@@ -370,17 +603,25 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
 #pragma unroll
           for (int c = 0; c < NACC / 4; ++c) {
             const int col = GATED ? (4 * c < 64 ? 64 * half + 4 * c : 128 + 64 * half + 4 * c - 64) : half * NACC + 4 * c;
-            *reinterpret_cast<float4 *>(red + row * S::RED_LD + col) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+            *reinterpret_cast<float4 *>(red + row * S::RED_LD + col) = make_float4(flat[4 * c], flat[4 * c + 1], flat[4 * c + 2], flat[4 * c + 3]);
           }
         }
+        meet();
+        alive = alive && !*abort_flag;
+        for (int i = (int)rank + world * warp; alive && i < tile.nrows; i += world * F8_EPI_WARPS) f8_join_row<GATED, BN, OutT>(p, tile, ring, world, i, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is copied into again
+        meet();
       } else if constexpr (GATED) {
         // h of 64 features, the row's largest together with the other half's, codes
         float a = 0.0f;
+        const int left = p.O - tile.nt * 128 - 64 * half;  // features that exist
+        if (any) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const float h = tile.nt * 128 + 64 * half + i < p.O ? coli_act_fast(acc[i], acc[64 + i], p.act) : 0.0f;
-          acc[i] = h;
-          a = fmaxf(a, fabsf(h));
+          for (int i = 0; i < 64; ++i) {
+            const float h = coli_act_fast(flat[i], flat[64 + i], p.act);  // (selected, not branched around: the 64 chains overlap)
+            flat[i] = i < left ? h : 0.0f;
+            a = fmaxf(a, fabsf(flat[i]));
+          }
         }
         float *am = amax_s + ((t / clusters) & 1) * 2 * F8_BM;
         am[half * F8_BM + row] = a;
@@ -394,68 +635,22 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = e4m3x4(acc[16 * c + 4 * i] * inv, acc[16 * c + 4 * i + 1] * inv, acc[16 * c + 4 * i + 2] * inv, acc[16 * c + 4 * i + 3] * inv);
+              w[i] = e4m3x4(flat[16 * c + 4 * i] * inv, flat[16 * c + 4 * i + 1] * inv, flat[16 * c + 4 * i + 2] * inv, flat[16 * c + 4 * i + 3] * inv);
             if (tile.nt * 128 + 64 * half + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
           }
           if (half == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
         }
       } else {
-        const int f = tile.nt * BN + half * NACC;
-        if (mine && alive && f < p.O) f8_store<OutT, NACC>((OutT *)p.y + (long)(tile.row0 + row) * p.y_stride + f, acc, p.O - f, p.y_vec);
+        const int f = tile.nt * BN + half * NACC, r0 = (warp & 3) * 32;
+        if (any && alive && f < p.O)
+          f8_store_rows<OutT, NACC>(smem + S::RING + warp * 32 * S::OUT_LD, (OutT *)p.y + (long)(tile.row0 + r0) * p.y_stride + f, p.y_stride, flat,
+                                    tile.nrows - r0, p.O - f, p.y_vec, lane);
+      }
+      if (t + clusters < n_tiles) {
+        recall(tile);
+        scales_of(kb0);
       }
     }
-    if constexpr (SPLIT) {
-      cluster_sync();
-      alive = alive && !*abort_flag;
-      if (warp < F8_EPI_WARPS && alive) {
-        const uint32_t red = ring;
-        for (int i = (int)rank + world * warp; i < tile.nrows; i += world * F8_EPI_WARPS) {  // a warp per row
-          float4 v[BN / 128];
-#pragma unroll
-          for (int j = 0; j < BN / 128; ++j) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int r = 0; r < world; ++r) {
-#pragma unroll
-            for (int j = 0; j < BN / 128; ++j) {
-              const float4 u = ld_cluster4(red + (uint32_t)(i * S::RED_LD + 128 * j + 4 * lane) * 4u, (uint32_t)r);
-              v[j].x += u.x;
-              v[j].y += u.y;
-              v[j].z += u.z;
-              v[j].w += u.w;
-            }
-          }
-          if constexpr (GATED) {
-            const int f = tile.nt * 128 + 4 * lane;
-            const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-            float h[4], a = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              h[j] = f + j < p.O ? coli_act_fast(g[j], u[j], p.act) : 0.0f;
-              a = fmaxf(a, fabsf(h[j]));
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
-            if (f < p.h_ld)
-              *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)(tile.row0 + i) * p.h_ld + f) =
-                  e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-            if (lane == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + i] = s;
-          } else {
-#pragma unroll
-            for (int j = 0; j < BN / 128; ++j) {
-              const int f = tile.nt * BN + 128 * j + 4 * lane;
-              const float o[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-              if (f < p.O) f8_store<OutT, 4>((OutT *)p.y + (long)(tile.row0 + i) * p.y_stride + f, o, p.O - f, p.y_vec);
-            }
-          }
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is copied into again
-      cluster_sync();
-    }
-  }
-  if (warp == F8_EPI_WARPS && *abort_flag) {
-    // copies already issued still land in this CTA's shared memory: give them time before exit
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   }
   tc_fence_before();
   __syncthreads();

@@ -3,8 +3,9 @@
 // kernel is to keep enough of them in flight on every SM.
 //
 // A warp owns slabs of 16 output features over all k-tiles (or `ksplit` warps share a task's k-tiles and join their sums in
-// a fixed order).  A slab's k-tile lies in HBM as 2 KB in a row and comes by one bulk copy into a ring of the warp's own, across
-// the ends of tasks; four mma.sync of 16 features x 8 rows x 32 columns per 8 rows form the k-tile's product, which is added,
+// a fixed order).  A slab's k-tile lies in HBM as 2 KB in a row and is copied into a ring of the warp's own, across
+// the ends of tasks (16 bytes a lane: a bulk copy costs the SM's copy engine 93 cycles however short it is, and 2 KB
+// at a time reach 22 bytes a clock, less than HBM gives an SM); four mma.sync of 16 features x 8 rows x 32 columns per 8 rows form the k-tile's product, which is added,
 // scaled, to f32 registers.  The order of columns inside a k-tile is the same for both operands and otherwise free: a lane
 // takes 16-byte chunks t and t + 4 of its feature and of its row.  Rows come straight from global memory (every warp of
 // the SM reads the same few kilobytes, out of L1).
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   int *status = p.status;
 
-  for (int i = threadIdx.x; i < S::SLOTS; i += FS_THREADS) mbar_init(bars + 8 * i, 1);
+  for (int i = threadIdx.x; i < S::SLOTS; i += FS_THREADS) mbar_init(bars + 8 * i, 32);
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
   // the copies: unit u is k-tile kt0 + u % per_task of the warp's task u / per_task
   int issued = 0, i_task = first, i_kt = kt0;
   const uint8_t *q0 = nullptr, *q1 = nullptr;
-  uint32_t unit_bytes = 0;
+  bool both = true;
+  int i_slot = 0;
   bool alive = true;
   auto issue = [&]() {  // the next unit into its slot (whole warp)
     if (i_kt == kt0) {
@@ -124,17 +126,20 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
       const size_t at = (size_t)tile.nt * (GATED ? 16 : 16 * M) * 128;
       q0 = (p.w0 ? p.w0[ex].q : p.one.q) + at;
       q1 = GATED ? p.w1[ex].q + at : nullptr;
-      unit_bytes = GATED ? 2048u : (uint32_t)min(16 * M, p.Op - tile.nt * 16 * M) * 128u;
+      both = (tile.nt + 1) * 16 * M <= p.Op;
     }
-    const int slot = issued % depth;
-    if (elect_one()) {
-      const uint32_t dst = ring + (uint32_t)slot * S::UNIT, b = bar + 8u * (uint32_t)slot;
-      const size_t off = (size_t)i_kt * p.Op * 128;
-      mbar_expect_tx(b, GATED ? 4096u : unit_bytes);
-      bulk_load(dst, q0 + off, unit_bytes, b);
-      if (GATED) bulk_load(dst + 2048, q1 + off, 2048u, b);
+    const uint32_t dst = ring + (uint32_t)i_slot * S::UNIT + (uint32_t)lane * 16;
+    const size_t off = (size_t)i_kt * p.Op * 128 + lane * 16;
+#pragma unroll
+    for (int c = 0; c < M * 4; ++c) {
+      if (GATED && c >= 4)
+        cp_async16(dst + c * 512, q1 + off + (c - 4) * 512);
+      else if (GATED || M == 1 || c < 4 || both)  // (the last unit of an odd number of slabs is half a one)
+        cp_async16(dst + c * 512, q0 + off + c * 512);
     }
-    __syncwarp();
+    // the lane's copies count once they have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar + 8u * (uint32_t)i_slot) : "memory");
+    if (++i_slot == depth) i_slot = 0;
     ++issued;
     if (++i_kt == kt1) {
       i_kt = kt0;
@@ -145,7 +150,8 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
   if (early) coli_grid_wait();
   coli_grid_trigger();  // (behind the wait: what a successor reads early is complete then)
 
-  int used = 0;
+  int used = 0, slot = 0;
+  uint32_t phase = 0;
   for (int task = first; works && task < tasks; task += stride) {
     const F8Tile tile = f8_tile<ROWS>(tile_off, row_off, p.nseg, task);
     const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
@@ -185,8 +191,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
         sw0 = __ldg(w0s + kt + 1);
         if (GATED) sw1 = __ldg(w1s + kt + 1);
       }
-      const int slot = used % depth;
-      alive = alive && __all_sync(0xffffffffu, mbar_wait(bar + 8u * (uint32_t)slot, (uint32_t)(used / depth) & 1u, abort_flag, status, TC_ERR_TMA_WAIT));
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(bar + 8u * (uint32_t)slot, phase, abort_flag, status, TC_ERR_TMA_WAIT));
       const uint32_t src = ring + (uint32_t)slot * S::UNIT + (uint32_t)g * 128;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
@@ -203,6 +208,10 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(d[i], rows.sx[n][i & 1] * sw, acc[m][n][i]);
         }
+      }
+      if (++slot == depth) {
+        slot = 0;
+        phase ^= 1u;
       }
       __syncwarp();  // the slot has been read
       if (alive && issued < n_units) issue();
@@ -244,10 +253,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const Fp8MmParams 
         }
     }
   }
-  if (*abort_flag && issued > used) {
-    // copies already issued still land in this CTA's shared memory: give them time before exit
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // (none are left unless a wait gave up)
 }
 
 template <bool GATED, bool HIN, int M, int NT, typename OutT>
