@@ -7,9 +7,9 @@
 
 namespace colib {
 
-constexpr int RL_WARPS = 8;
-// per warp: candidate keys and scores, their ids
-constexpr int RL_CAND_BYTES = 32 * (8 + 8 + 4);
+constexpr int RL_MAX_WARPS = 32;
+// per warp: keys of the candidates, their ids
+constexpr int RL_CAND_BYTES = 32 * (8 + 4);
 
 template <typename T>
 __device__ __forceinline__ double rl_load(const T *p);
@@ -36,23 +36,58 @@ __device__ __forceinline__ double rl_warp_sum(double v) {
   return v;
 }
 
+// exp of a non-positive (softmax) or any (sigmoid) argument, relative error below 1e-15: n = rint(x log2 e), Taylor's polynomial
+// of degree 13 in r = x - n ln 2 (two steps), |r| <= 0.347: remainder 4e-18 / (1 - r) relative; times 2^n.  As coli_expf
+// (coli_math.h), whose result is rounded to f32.  Arguments are cut to +-708: beyond, a weight is below f32's least either way.
+__device__ __forceinline__ double rl_exp(double x) {
+  x = fmin(fmax(x, -708.0), 708.0);
+  const double n = rint(x * 1.4426950408889634074);
+  double r = fma(n, -6.93147180369123816490e-01, x);
+  r = fma(n, -1.90821492927058770002e-10, r);
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return p * __hiloint2double((1023 + (int)n) << 20, 0);
+}
+
+// the same of an f32 value
+__device__ __forceinline__ uint32_t rl_key32(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float rl_value32(uint32_t key) { return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key); }
+
+template <typename Key>
 struct RlCand {
-  uint64_t *key;
-  double *score;
+  Key *key;
   int *id;
 };
+__device__ __forceinline__ uint32_t rl_upper(uint32_t k) { return k; }
+__device__ __forceinline__ uint32_t rl_upper(uint64_t k) { return (uint32_t)(k >> 32); }
 
-// The k best keys of a warp (lane + 32 s holds expert lane + 32 s; largest key, then lowest expert; 0 is none) into places
+// The k best keys of a warp (slot s of a lane holds expert lane + 32 s; largest key, then lowest expert; 0 is none) into places
 // 0 .. of `c`, in order.  Returns how many there are, at most k.  The k-th largest of the lanes' best keys bounds the k-th largest of
 // all from below (taken by its upper word alone): a little over k candidates as a rule, and each finds its place by
 // counting.  More than 32 of them (many equal logits) take k rounds.
-template <int SLOTS>
-__device__ __forceinline__ int rl_select(const uint64_t (&key)[SLOTS], const double (&score)[SLOTS], int k, const RlCand &c, int lane) {
-  uint64_t best = 0;
+template <int SLOTS, typename Key>
+__device__ __forceinline__ int rl_select(Key (&key)[SLOTS], int k, const RlCand<Key> &c, int lane) {
+  Key best = 0;
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) best = key[s] > best ? key[s] : best;
-  const uint32_t bhi = (uint32_t)(best >> 32);
+  const uint32_t bhi = rl_upper(best);
   uint32_t *hi = reinterpret_cast<uint32_t *>(c.key);
+  __syncwarp();
   hi[lane] = bhi;
   __syncwarp();
   int above = 0;
@@ -62,89 +97,149 @@ __device__ __forceinline__ int rl_select(const uint64_t (&key)[SLOTS], const dou
     above += (q.x > bhi) + (q.y > bhi) + (q.z > bhi) + (q.w > bhi);
   }
   const uint32_t bound = max(1u, __reduce_min_sync(0xffffffffu, above < k ? bhi : 0xffffffffu));
-  uint32_t holders[SLOTS];
-  int n = 0;
+  uint32_t mine = 0u;  // this lane's slots at or above the bound
 #pragma unroll
-  for (int s = 0; s < SLOTS; ++s) {
-    holders[s] = __ballot_sync(0xffffffffu, (uint32_t)(key[s] >> 32) >= bound);
-    n += __popc(holders[s]);
-  }
+  for (int s = 0; s < SLOTS; ++s) mine |= (uint32_t)(rl_upper(key[s]) >= bound) << s;
+  const int n = (int)__reduce_add_sync(0xffffffffu, (unsigned)__popc(mine));
   if (n <= 32) {
-    int at = 0;
+    // places in any order, then everyone counts who comes before it
+    int at = __popc(mine);
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      if ((uint32_t)(key[s] >> 32) >= bound) {
-        const int i = at + __popc(holders[s] & ((1u << lane) - 1u));
-        c.key[i] = key[s];
-        c.score[i] = score[s];
-        c.id[i] = s * 32 + lane;
-      }
-      at += __popc(holders[s]);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += u;
     }
+    at -= __popc(mine);
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+      if ((mine >> s) & 1u) {
+        c.key[at] = key[s];
+        c.id[at] = s * 32 + lane;
+        ++at;
+      }
     __syncwarp();
-    const uint64_t mk = lane < n ? c.key[lane] : 0;
-    const double ms = lane < n ? c.score[lane] : 0.0;
+    const Key mk = lane < n ? c.key[lane] : 0;
     const int mi = lane < n ? c.id[lane] : 0;
     int rank = 0;
-    for (int j = 0; j < n; ++j) {  // a slot's candidates precede the next slot's and lanes ascend: j < lane is the lower id
-      const uint64_t other = c.key[j];
-      rank += other > mk || (other == mk && j < lane);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const Key other = c.key[j];
+      rank += other > mk || (other == mk && c.id[j] < mi);
     }
     __syncwarp();
     if (lane < n && rank < k) {
-      c.score[rank] = ms;
+      c.key[rank] = mk;
       c.id[rank] = mi;
     }
     __syncwarp();
     return min(n, k);
   }
-  uint64_t left[SLOTS];
-#pragma unroll
-  for (int s = 0; s < SLOTS; ++s) left[s] = key[s];
   int found = 0;
   for (; found < k; ++found) {
-    uint64_t bk = 0;
-    double bs = 0.0;
+    Key bk = 0;
     int bid = 0x7fffffff;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s)
-      if (left[s] > bk) {
-        bk = left[s];
-        bs = score[s];
+      if (key[s] > bk) {
+        bk = key[s];
         bid = s * 32 + lane;
       }
-    const uint32_t top_hi = __reduce_max_sync(0xffffffffu, (uint32_t)(bk >> 32));
-    if (top_hi == 0u) break;
-    const uint32_t top_lo = __reduce_max_sync(0xffffffffu, (uint32_t)(bk >> 32) == top_hi ? (uint32_t)bk : 0u);
-    const bool holds = (uint32_t)(bk >> 32) == top_hi && (uint32_t)bk == top_lo;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, rl_upper(bk));
+    if (top == 0u) break;
+    const uint32_t low = __reduce_max_sync(0xffffffffu, rl_upper(bk) == top ? (uint32_t)bk : 0u);
+    const bool holds = rl_upper(bk) == top && (uint32_t)bk == low;
     const int win = (int)__reduce_min_sync(0xffffffffu, holds ? (uint32_t)bid : 0x7fffffffu);
     if (holds && bid == win) {
-      c.score[found] = bs;
+      c.key[found] = bk;
       c.id[found] = win;
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s)
-        if (s * 32 + lane == win) left[s] = 0;
+        if (s * 32 + lane == win) key[s] = 0;
     }
   }
   __syncwarp();
   return found;
 }
 
-// One warp routes one token; `row` is E doubles of shared memory of its own (groups only).
-template <typename T, int SLOTS>
-__device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, const RlCand &c, double *row, int lane) {
-  const T *z0 = (const T *)p.logits + (long)t * p.stride;
-  const double NEG_INF = __longlong_as_double(0xfff0000000000000ll);
-  double score[SLOTS];
-  bool open[SLOTS];
+// Experts outside the topk_group best groups lose their keys.  A group's mark is the sum of its two best choices (the one, where only
+// one is open); `per` lanes share a group.  Returns how far the last mark kept lies above the first one left out.
+template <int SLOTS, typename Key, typename Real>
+__device__ __forceinline__ Real rl_groups(const RouteLogitsParams &p, Key (&key)[SLOTS], const Real (&choice)[SLOTS], Real none, Real *row, Real *marks,
+                                          int lane) {
+  const int G = p.n_group, gs = p.E / G;
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s)
+    if (lane + 32 * s < p.E) row[lane + 32 * s] = key[s] ? choice[s] : none;
+  __syncwarp();
+  int per = 1;
+  while (2 * per * G <= 32) per *= 2;
+  const int g = lane / per;
+  Real m1 = none, m2 = none;
+  if (g < G)
+#pragma unroll 4
+    for (int i = lane % per; i < gs; i += per) {
+      const Real v = row[g * gs + i];
+      m2 = v > m1 ? m1 : (v > m2 ? v : m2);
+      m1 = v > m1 ? v : m1;
+    }
+  for (int o = 1; o < per; o <<= 1) {
+    const Real o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
+    const Real lo = m1 < o1 ? m1 : o1, hi = m2 > o2 ? m2 : o2;
+    m2 = lo > hi ? lo : hi;
+    m1 = m1 > o1 ? m1 : o1;
+  }
+  const bool some = g < G && m1 > none;
+  const Real mark = some ? (m2 > none ? m1 + m2 : m1) : none;
+  if (lane % per == 0 && g < G) marks[g] = mark;
+  __syncwarp();
+  int above = 0;
+  for (int j = 0; j < G; ++j) above += marks[j] > mark || (marks[j] == mark && j < g);
+  const bool keep = some && above < p.topk_group;
+  const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+  Real last = keep ? mark : -none, first = some && !keep ? mark : none;
+  for (int o = 1; o < 32; o <<= 1) {
+    const Real a = __shfl_xor_sync(0xffffffffu, last, o), b = __shfl_xor_sync(0xffffffffu, first, o);
+    last = a < last ? a : last;
+    first = b > first ? b : first;
+  }
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int e = lane + 32 * s;
-    double z = e < p.E ? rl_load<T>(z0 + e) : NEG_INF;
-    if (p.logit_bias && e < p.E) z += (double)__ldg(p.logit_bias + e);
-    open[s] = z > NEG_INF;
-    score[s] = open[s] ? z : NEG_INF;
+    if (e < p.E && !((kept >> ((e / gs) * per)) & 1u)) key[s] = 0;
   }
+  __syncwarp();
+  return last - first;
+}
+
+// What the weights need besides a chosen expert's own logit.
+struct RlNorm {
+  double top, sum;  // softmax: the largest z, and the sum of exp(z - top); 0: not needed
+  int n;            // experts chosen, -1: undecided
+};
+template <typename T>
+__device__ __forceinline__ double rl_z(const RouteLogitsParams &p, const T *z0, int e) {
+  const double z = rl_load<T>(z0 + e);
+  return p.logit_bias ? z + (double)__ldg(p.logit_bias + e) : z;
+}
+// (a largest logit of infinity shares the mass with its equals)
+__device__ __forceinline__ double rl_over(double z, double top) { return z == top ? 1.0 : rl_exp(z - top); }
+
+// The choice in 64 bits throughout: where 32 do not decide it.
+template <typename T, int SLOTS>
+__device__ __noinline__ RlNorm rl_choose64(const RouteLogitsParams &p, const T *z0, unsigned char *cand, double *row, int lane) {
+  RlNorm norm;
+  const double NEG_INF = __longlong_as_double(0xfff0000000000000ll);
+  const RlCand<uint64_t> c = {reinterpret_cast<uint64_t *>(cand), reinterpret_cast<int *>(cand + 256)};
+  double score[SLOTS];
+  uint64_t key[SLOTS];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    const int e = lane + 32 * s;
+    const double z = e < p.E ? rl_z<T>(p, z0, e) : NEG_INF;
+    key[s] = z > NEG_INF;
+    score[s] = key[s] ? z : NEG_INF;
+  }
+  norm.top = norm.sum = 0.0;
   if (p.score == COLI_SCORE_SOFTMAX) {
     double m = NEG_INF;
 #pragma unroll
@@ -153,79 +248,135 @@ __device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, cons
     double sum = 0.0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      // (an infinite largest logit shares the mass with its equals)
-      score[s] = score[s] == m ? (open[s] ? 1.0 : 0.0) : exp(score[s] - m);
+      score[s] = key[s] ? rl_over(score[s], m) : 0.0;
       sum += score[s];
     }
-    sum = rl_warp_sum(sum);
+    norm.top = m;
+    norm.sum = sum = rl_warp_sum(sum);
     const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) score[s] *= inv;
   } else {
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) score[s] = 1.0 / (1.0 + exp(-score[s]));
+    for (int s = 0; s < SLOTS; ++s) score[s] = 1.0 / (1.0 + rl_exp(-score[s]));
   }
-  uint64_t key[SLOTS];
-  double choice[SLOTS];
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int e = lane + 32 * s;
-    choice[s] = p.select_bias && e < p.E ? score[s] + (double)__ldg(p.select_bias + e) : score[s];
-    key[s] = open[s] ? rl_key(choice[s]) : 0;
+    if (p.select_bias && e < p.E) score[s] += (double)__ldg(p.select_bias + e);
+    key[s] = key[s] && score[s] > NEG_INF ? rl_key(score[s]) : 0;
   }
-  if (p.n_group > 1) {
-    // a group's mark is the sum of its two best (of one, where only one is open); `per` lanes share a group
-    const int G = p.n_group, gs = p.E / G;
+  if (p.n_group > 1) rl_groups<SLOTS, uint64_t, double>(p, key, score, NEG_INF, row, reinterpret_cast<double *>(cand), lane);
+  norm.n = rl_select<SLOTS, uint64_t>(key, p.k, c, lane);
+  return norm;
+}
+
+// The choice in 32 bits: by the logits themselves where neither a bias nor groups ask for scores, and else by f32 scores, as long as no
+// two that it hangs on lie within their errors (-1: they do).  An f32 score is off by at most 2^-19 of itself (__expf: 2^-21 and
+// 2^-23 of its argument, whose share of the score is below 2^-20) and by what the rounding of z takes from it, 2^-23 |z|
+// with a logit bias; a choice by another 2^-23 of itself.
+template <typename T, int SLOTS>
+__device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *z0, unsigned char *cand, float *row, int lane, RlNorm &norm) {
+  const float NEG_INF = __uint_as_float(0xff800000u);
+  const RlCand<uint32_t> c = {reinterpret_cast<uint32_t *>(cand), reinterpret_cast<int *>(cand + 256)};
+  const bool softmax = p.score == COLI_SCORE_SOFTMAX;
+  const bool scored = p.select_bias || p.logit_bias || p.n_group > 1;
+  float z[SLOTS];
+  uint32_t key[SLOTS];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) z[s] = lane + 32 * s < p.E ? (float)rl_load<T>(z0 + lane + 32 * s) : NEG_INF;
+  if (p.logit_bias) {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s)
-      if (lane + 32 * s < p.E) row[lane + 32 * s] = key[s] ? choice[s] : NEG_INF;
-    __syncwarp();
-    int per = 1;
-    while (2 * per * G <= 32) per *= 2;
-    const int g = lane / per;
-    double m1 = NEG_INF, m2 = NEG_INF;
-    if (g < G)
-      for (int i = lane % per; i < gs; i += per) {
-        const double v = row[g * gs + i];
-        m2 = v > m1 ? m1 : fmax(m2, v);
-        m1 = fmax(m1, v);
-      }
-    for (int o = 1; o < per; o <<= 1) {
-      const double o1 = __shfl_xor_sync(0xffffffffu, m1, o), o2 = __shfl_xor_sync(0xffffffffu, m2, o);
-      m2 = fmax(fmin(m1, o1), fmax(m2, o2));
-      m1 = fmax(m1, o1);
+      if (lane + 32 * s < p.E) z[s] += __ldg(p.logit_bias + lane + 32 * s);
+  }
+  uint32_t top = 0u;
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    key[s] = z[s] > NEG_INF ? rl_key32(z[s]) : 0u;
+    top = max(top, key[s]);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  norm.top = norm.sum = 0.0;
+  if (top == 0u) return 0;  // every expert is closed
+  const float m = rl_value32(top);
+  if (softmax) {
+    // an infinite sum of z and its bias may be a rounded one
+    if (p.logit_bias && !(fabsf(m) <= 3.0e38f)) return -1;
+    norm.top = (double)m;
+    // (where the weights are divided by their own sum, and that holds the largest, the sum over all experts drops out)
+    if (!p.norm_topk || scored) {
+      double sum = 0.0;
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) sum += key[s] ? rl_over((double)z[s], norm.top) : 0.0;
+      norm.sum = rl_warp_sum(sum);
     }
-    uint64_t *gk = c.key;
-    const uint64_t mark = g < G && m1 > NEG_INF ? rl_key(m2 > NEG_INF ? m1 + m2 : m1) : 0;
-    if (lane % per == 0 && g < G) gk[g] = mark;
-    __syncwarp();
-    int above = 0;
-    for (int j = 0; j < G; ++j) above += gk[j] > mark || (gk[j] == mark && j < g);
-    const uint32_t kept = __ballot_sync(0xffffffffu, g < G && mark != 0 && above < p.topk_group);
+  }
+  float apart = 0.0f;  // how far two choices must lie apart
+  if (scored) {
+    if (p.logit_bias && softmax) return -1;  // (top and sum are wanted to 64 bits)
+    const float inv = softmax ? (float)(1.0 / norm.sum) : 0.0f;
+    float choice[SLOTS], size = 0.0f, arg = 0.0f;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int e = lane + 32 * s;
-      if (e < p.E && !((kept >> ((e / gs) * per)) & 1u)) key[s] = 0;
+      choice[s] = softmax ? (z[s] == m ? 1.0f : __expf(z[s] - m)) * inv : __fdividef(1.0f, 1.0f + __expf(fminf(-z[s], 80.0f)));
+      if (p.select_bias && e < p.E) choice[s] += __ldg(p.select_bias + e);
+      if (key[s]) {
+        key[s] = choice[s] > NEG_INF ? rl_key32(choice[s]) : 0u;
+        size = fmaxf(size, fabsf(choice[s]));
+        arg = fmaxf(arg, fminf(fabsf(z[s]), 128.0f));
+      }
     }
-    __syncwarp();
+    size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
+    arg = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(arg)));
+    apart = 2.0f * (1.9e-6f + 2.4e-7f * size + (p.logit_bias ? 1.2e-7f * arg : 0.0f));
+    if (p.n_group > 1) {
+      const float gap = rl_groups<SLOTS, uint32_t, float>(p, key, choice, NEG_INF, row, reinterpret_cast<float *>(cand), lane);
+      if (!(gap > 2.0f * apart)) return -1;
+    }
   }
-  const int n = rl_select<SLOTS>(key, score, p.k, c, lane);
-  double w = lane < n ? c.score[lane] : 0.0;
+  const int n = rl_select<SLOTS, uint32_t>(key, min(scored ? p.k + 1 : p.k, 32), c, lane);
+  if (scored) {
+    if (n == 32 && p.k == 32) return -1;  // (the 33rd is not known)
+    const bool near = lane + 1 < n && !(rl_value32(c.key[lane]) - rl_value32(c.key[lane + 1]) > apart);
+    if (__any_sync(0xffffffffu, near)) return -1;
+  }
+  return min(n, p.k);
+}
+
+// One warp routes one token; `row` is E doubles of shared memory of its own (groups only).
+template <typename T, int SLOTS>
+__device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane) {
+  const T *z0 = (const T *)p.logits + (long)t * p.stride;
+  RlNorm norm;
+  norm.n = rl_choose32<T, SLOTS>(p, z0, cand, reinterpret_cast<float *>(row), lane, norm);
+  if (norm.n < 0) norm = rl_choose64<T, SLOTS>(p, z0, cand, row, lane);
+  const int n = norm.n;
+  const int *ids = reinterpret_cast<const int *>(cand + 256);
+  double w = 0.0;
+  if (lane < n) {
+    const double z = rl_z<T>(p, z0, ids[lane]);
+    if (p.score != COLI_SCORE_SOFTMAX)
+      w = 1.0 / (1.0 + rl_exp(-z));
+    else
+      w = norm.sum > 0.0 ? rl_over(z, norm.top) / norm.sum : rl_over(z, norm.top);
+  }
   if (p.norm_topk) w /= rl_warp_sum(w) + 1e-20;
   if (lane < p.k) {
-    p.idx[(long)t * p.k + lane] = lane < n ? c.id[lane] : -1;
+    p.idx[(long)t * p.k + lane] = lane < n ? ids[lane] : -1;
     p.w[(long)t * p.k + lane] = (float)(w * (double)p.routed_scale);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void rl_route(const RouteLogitsParams &p, int t, const RlCand &c, double *row, int lane) {
+__device__ __forceinline__ void rl_route(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane) {
   if (p.E <= 128)
-    rl_token<T, 4>(p, t, c, row, lane);
+    rl_token<T, 4>(p, t, cand, row, lane);
   else if (p.E <= 256)
-    rl_token<T, 8>(p, t, c, row, lane);
+    rl_token<T, 8>(p, t, cand, row, lane);
   else
-    rl_token<T, 16>(p, t, c, row, lane);
+    rl_token<T, 16>(p, t, cand, row, lane);
 }
 
 // Which of a chunk's tokens chose each expert, one bit each: the number of bits below a token's own is the rank of its
@@ -278,17 +429,15 @@ __device__ __forceinline__ void rl_scan(const int *cnt, int *off, int E, int lan
 
 // One CTA per chunk of tokens: routes them and counts their experts; where the call is one chunk, places them as well.
 template <typename T>
-__global__ void __launch_bounds__(RL_WARPS * 32) k_route_logits(RouteLogitsParams p) {
+__global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid_constant__ RouteLogitsParams p) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char *mine = rl_smem + warp * RL_CAND_BYTES;
-  const RlCand c = {reinterpret_cast<uint64_t *>(mine), reinterpret_cast<double *>(mine + 256), reinterpret_cast<int *>(mine + 512)};
-  unsigned char *after = rl_smem + RL_WARPS * RL_CAND_BYTES;
-  double *row = reinterpret_cast<double *>(after) + (size_t)warp * (p.n_group > 1 ? p.E : 0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  unsigned char *cand = rl_smem + warp * RL_CAND_BYTES;
+  double *row = reinterpret_cast<double *>(rl_smem + warps * RL_CAND_BYTES) + (size_t)warp * (p.n_group > 1 ? p.E : 0);
   coli_grid_dependency_sync();
   const int t0 = blockIdx.x * p.chunk, tokens = min(p.chunk, p.T - t0), words = p.chunk / 32;
-  for (int j = warp; j < tokens; j += RL_WARPS) {
-    rl_route<T>(p, t0 + j, c, row, lane);
+  for (int j = warp; j < tokens; j += warps) {
+    rl_route<T>(p, t0 + j, cand, row, lane);
     __syncwarp();
   }
   __syncthreads();
@@ -316,7 +465,7 @@ __global__ void __launch_bounds__(RL_WARPS * 32) k_route_logits(RouteLogitsParam
 }
 
 // One CTA per chunk: rows of every expert before the chunk from all chunks' counts, then the places of its pairs.
-__global__ void __launch_bounds__(512) k_route_place(RouteLogitsParams p, int chunks) {
+__global__ void __launch_bounds__(512) k_route_place(const __grid_constant__ RouteLogitsParams p, int chunks) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
   const int words = p.chunk / 32;
   uint32_t *mask = reinterpret_cast<uint32_t *>(rl_smem);
@@ -345,22 +494,26 @@ __global__ void __launch_bounds__(512) k_route_place(RouteLogitsParams p, int ch
   for (long i = (long)total + blockIdx.x * blockDim.x + threadIdx.x; i < (long)p.T * p.k; i += (long)gridDim.x * blockDim.x) p.row_token[i] = -1;
 }
 
+template <typename T>
+static int launch_route_typed(const RouteLogitsParams &p, int chunks, int warps, size_t smem, cudaStream_t st) {
+  static ColiPerDeviceOnce attr_once;
+  if (!coli_set_smem_limit(attr_once, k_route_logits<T>, RL_MAX_WARPS * (RL_CAND_BYTES + 512 * 8), "routing shared-memory attribute")) return 0;
+  coli_count_launch(1);
+  return coli_cuda_check(launch_dependent(k_route_logits<T>, dim3(chunks), dim3(warps * 32), smem, st, p), "routing launch") ? 1 : 0;
+}
+
 int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
   p.chunk = route_logits_chunk(p.T);
   const int chunks = (p.T + p.chunk - 1) / p.chunk, words = p.chunk / 32;
+  // a warp per token up to 32; a few more for the tables where there are few tokens
+  const int tokens = p.T < p.chunk ? p.T : p.chunk, warps = tokens < 4 ? 4 : tokens < RL_MAX_WARPS ? tokens : RL_MAX_WARPS;
   const size_t tables = (size_t)p.E * words * 4 + (3 * (size_t)p.E + 1) * 4;
-  size_t smem = RL_WARPS * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));
+  size_t smem = (size_t)warps * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));
   if (smem < tables) smem = tables;
-  coli_count_launch(1);
-  cudaError_t e;
-  if (p.type == COLI_TYPE_F32)
-    e = launch_dependent(k_route_logits<float>, dim3(chunks), dim3(RL_WARPS * 32), smem, st, p);
-  else if (p.type == COLI_TYPE_F16)
-    e = launch_dependent(k_route_logits<__half>, dim3(chunks), dim3(RL_WARPS * 32), smem, st, p);
-  else
-    e = launch_dependent(k_route_logits<__nv_bfloat16>, dim3(chunks), dim3(RL_WARPS * 32), smem, st, p);
-  if (!coli_cuda_check(e, "routing launch")) return 0;
-  if (chunks == 1) return 1;
+  const int ok = p.type == COLI_TYPE_F32   ? launch_route_typed<float>(p, chunks, warps, smem, st)
+                 : p.type == COLI_TYPE_F16 ? launch_route_typed<__half>(p, chunks, warps, smem, st)
+                                           : launch_route_typed<__nv_bfloat16>(p, chunks, warps, smem, st);
+  if (!ok || chunks == 1) return ok;
   coli_count_launch(1);
   return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(512), tables, st, p, chunks), "placement launch") ? 1 : 0;
 }
