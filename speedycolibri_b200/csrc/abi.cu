@@ -1307,7 +1307,7 @@ extern "C" int coli_b200_fp8_check(int device) {
 extern "C" size_t coli_b200_route_logits_workspace(int T, int E) {
   if (T < 1 || E < 1) return 0;
   const int c = colib::route_logits_chunk(T), chunks = (T + c - 1) / c;
-  return chunks == 1 ? 0 : (size_t)chunks * E;
+  return chunks == 1 ? 0 : (size_t)chunks * round_up(E, 4);
 }
 
 extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int type, int64_t stride, const float *select_bias_dev,
@@ -1334,7 +1334,7 @@ extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int ty
   }
   if (stride < 0 || (T > 1 && stride < E) || !aligned_to(logits_dev, es) || !aligned_to(select_bias_dev, 4) || !aligned_to(logit_bias_dev, 4) ||
       !aligned_to(topk_idx_dev, 4) || !aligned_to(topk_w_dev, 4) || !aligned_to(expert_rows_dev, 4) || !aligned_to(slot_dev, 4) ||
-      !aligned_to(row_token_dev, 4)) {
+      !aligned_to(row_token_dev, 4) || !aligned_to(workspace_dev, 4)) {
     coli_set_error("route_logits: row stride %lld for %d experts, or a misaligned pointer", (long long)stride, E);
     return 0;
   }

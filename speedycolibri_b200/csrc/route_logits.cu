@@ -345,9 +345,9 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
   return min(n, p.k);
 }
 
-// One warp routes one token; `row` is E doubles of shared memory of its own (groups only).
+// One warp routes one token; `row` is E doubles of shared memory of its own (groups only).  The experts also go to ids_out.
 template <typename T, int SLOTS>
-__device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane) {
+__device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane, int *ids_out) {
   const T *z0 = (const T *)p.logits + (long)t * p.stride;
   RlNorm norm;
   norm.n = rl_choose32<T, SLOTS>(p, z0, cand, reinterpret_cast<float *>(row), lane, norm);
@@ -364,19 +364,23 @@ __device__ __forceinline__ void rl_token(const RouteLogitsParams &p, int t, unsi
   }
   if (p.norm_topk) w /= rl_warp_sum(w) + 1e-20;
   if (lane < p.k) {
-    p.idx[(long)t * p.k + lane] = lane < n ? ids[lane] : -1;
+    const int id = lane < n ? ids[lane] : -1;
+    ids_out[lane] = id;
+    p.idx[(long)t * p.k + lane] = id;
     p.w[(long)t * p.k + lane] = (float)(w * (double)p.routed_scale);
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void rl_route(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane) {
+__device__ __forceinline__ void rl_route(const RouteLogitsParams &p, int t, unsigned char *cand, double *row, int lane, int *ids_out) {
   if (p.E <= 128)
-    rl_token<T, 4>(p, t, cand, row, lane);
+    rl_token<T, 4>(p, t, cand, row, lane, ids_out);
   else if (p.E <= 256)
-    rl_token<T, 8>(p, t, cand, row, lane);
+    rl_token<T, 8>(p, t, cand, row, lane, ids_out);
+  else if (p.E <= 384)
+    rl_token<T, 12>(p, t, cand, row, lane, ids_out);
   else
-    rl_token<T, 16>(p, t, cand, row, lane);
+    rl_token<T, 16>(p, t, cand, row, lane, ids_out);
 }
 
 // Which of a chunk's tokens chose each expert, one bit each: the number of bits below a token's own is the rank of its
@@ -395,36 +399,23 @@ __device__ __forceinline__ int rl_rank(const uint32_t *m, int words, int j) {
   for (int w = 0; w < words; ++w) r += w < (j >> 5) ? __popc(m[w]) : w == (j >> 5) ? __popc(m[w] & ((1u << (j & 31)) - 1u)) : 0;
   return r;
 }
-
-// A chunk's pairs take the rows base[e] + rank.
-__device__ __forceinline__ void rl_place(const RouteLogitsParams &p, const uint32_t *mask, const int *base, int t0, int tokens) {
-  const int words = p.chunk / 32;
-  for (int i = threadIdx.x; i < tokens * p.k; i += blockDim.x) {
-    const long at = (long)t0 * p.k + i;
-    const int e = p.idx[at], j = i / p.k;
-    int slot = -1;
-    if (e >= 0) {
-      slot = base[e] + rl_rank(mask + e * words, words, j);
-      p.row_token[slot] = t0 + j;
-    }
-    p.slot[at] = slot;
-  }
-}
-// exclusive sums of cnt[0 .. E) into off[0 .. E], by one warp
+// exclusive sums of cnt[0 .. E) into off[0 .. E], by one warp: a run of experts each
 __device__ __forceinline__ void rl_scan(const int *cnt, int *off, int E, int lane) {
-  int total = 0;
-  for (int e0 = 0; e0 < E; e0 += 32) {
-    const int n = e0 + lane < E ? cnt[e0 + lane] : 0;
-    int s = n;
+  const int per = (E + 31) / 32, e0 = lane * per;
+  int n = 0;
+  for (int i = 0; i < per; ++i) n += e0 + i < E ? cnt[e0 + i] : 0;
+  int s = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    if (e0 + lane < E) off[e0 + lane] = total + s - n;
-    total += __shfl_sync(0xffffffffu, s, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
   }
-  if (lane == 0) off[E] = total;
+  if (lane == 31) off[E] = s;
+  s -= n;
+  for (int i = 0; i < per && e0 + i < E; ++i) {
+    off[e0 + i] = s;
+    s += cnt[e0 + i];
+  }
 }
 
 // One CTA per chunk of tokens: routes them and counts their experts; where the call is one chunk, places them as well.
@@ -432,72 +423,115 @@ template <typename T>
 __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid_constant__ RouteLogitsParams p) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  unsigned char *cand = rl_smem + warp * RL_CAND_BYTES;
-  double *row = reinterpret_cast<double *>(rl_smem + warps * RL_CAND_BYTES) + (size_t)warp * (p.n_group > 1 ? p.E : 0);
+  const int t0 = blockIdx.x * p.chunk, tokens = min(p.chunk, p.T - t0), pairs = tokens * p.k, words = p.chunk / 32;
+  int *ids = reinterpret_cast<int *>(rl_smem);  // the chunk's choices, then per-warp memory, later the tables
+  unsigned char *after = rl_smem + (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15);
+  unsigned char *cand = after + warp * RL_CAND_BYTES;
+  double *row = reinterpret_cast<double *>(after + warps * RL_CAND_BYTES) + (size_t)warp * (p.n_group > 1 ? p.E : 0);
   coli_grid_dependency_sync();
-  const int t0 = blockIdx.x * p.chunk, tokens = min(p.chunk, p.T - t0), words = p.chunk / 32;
   for (int j = warp; j < tokens; j += warps) {
-    rl_route<T>(p, t0 + j, cand, row, lane);
+    rl_route<T>(p, t0 + j, cand, row, lane, ids + j * p.k);
     __syncwarp();
   }
   __syncthreads();
-  // (from here the shared memory holds the masks, counts and offsets)
-  uint32_t *mask = reinterpret_cast<uint32_t *>(rl_smem);
-  int *cnt = reinterpret_cast<int *>(mask + p.E * words), *off = cnt + p.E;
-  rl_mark(mask, words, p.idx + (long)t0 * p.k, tokens * p.k, p.k, p.E);
-  const bool only = gridDim.x == 1;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int n = 0;
-    for (int w = 0; w < words; ++w) n += __popc(mask[e * words + w]);
-    if (only) {
-      cnt[e] = n;
-      p.expert_rows[e] = n;
-    } else {
-      p.chunk_rows[(size_t)blockIdx.x * p.E + e] = (uint8_t)n;
+  if (gridDim.x > 1) {
+    uint32_t *mask = reinterpret_cast<uint32_t *>(after);
+    rl_mark(mask, words, ids, pairs, p.k, p.E);
+    const int pitch = (p.E + 3) & ~3;
+    for (int e = threadIdx.x; e < pitch; e += blockDim.x) {
+      int n = 0;
+      for (int w = 0; w < words; ++w) n += e < p.E ? __popc(mask[e * words + w]) : 0;
+      p.chunk_rows[(size_t)blockIdx.x * pitch + e] = (uint8_t)n;
     }
+    return;
   }
-  if (!only) return;
+  // The only chunk: every pair counts the pairs before it in expert order (a table of the experts would cost a scan over all).
+  int *cnt = reinterpret_cast<int *>(after);
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) cnt[e] = 0;
+  const int padded = (pairs + 3) & ~3;
+  for (int i = pairs + threadIdx.x; i < padded; i += blockDim.x) ids[i] = -1;
   __syncthreads();
-  if (warp == 0) rl_scan(cnt, off, p.E, lane);
-  __syncthreads();
-  rl_place(p, mask, off, t0, tokens);
-  for (int i = off[p.E] + (int)threadIdx.x; i < p.T * p.k; i += blockDim.x) p.row_token[i] = -1;
+  int total = 0;
+  for (int i0 = 0; i0 < pairs; i0 += blockDim.x) {
+    const int i = i0 + (int)threadIdx.x, id = i < pairs ? ids[i] : -1;
+    if (id >= 0) {
+      int rank = 0;
+      for (int j = 0; j < padded; j += 4) {
+        const int4 o = *reinterpret_cast<const int4 *>(ids + j);
+        rank += ((unsigned)o.x < (unsigned)id || (o.x == id && j < i)) + ((unsigned)o.y < (unsigned)id || (o.y == id && j + 1 < i)) +
+                ((unsigned)o.z < (unsigned)id || (o.z == id && j + 2 < i)) + ((unsigned)o.w < (unsigned)id || (o.w == id && j + 3 < i));
+      }
+      atomicAdd(cnt + id, 1);
+      p.slot[i] = rank;
+      p.row_token[rank] = i / p.k;
+    } else if (i < pairs) {
+      p.slot[i] = -1;
+    }
+    total += __syncthreads_count(id >= 0);
+  }
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.expert_rows[e] = cnt[e];
+  for (int i = total + (int)threadIdx.x; i < pairs; i += blockDim.x) p.row_token[i] = -1;
 }
 
 // One CTA per chunk: rows of every expert before the chunk from all chunks' counts, then the places of its pairs.
-__global__ void __launch_bounds__(512) k_route_place(const __grid_constant__ RouteLogitsParams p, int chunks) {
+constexpr int RL_PLACE_THREADS = 512;
+__global__ void __launch_bounds__(RL_PLACE_THREADS) k_route_place(const __grid_constant__ RouteLogitsParams p, int chunks) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
-  const int words = p.chunk / 32;
+  const int words = p.chunk / 32, pitch = (p.E + 3) & ~3;
   uint32_t *mask = reinterpret_cast<uint32_t *>(rl_smem);
-  int *cnt = reinterpret_cast<int *>(mask + p.E * words), *off = cnt + p.E, *before = off + p.E + 1;
+  int *cnt = reinterpret_cast<int *>(mask + p.E * words), *before = cnt + pitch, *off = before + pitch;
+  for (int e = threadIdx.x; e < 2 * pitch; e += blockDim.x) cnt[e] = 0;
+  __syncthreads();
   coli_grid_dependency_sync();
   const int t0 = blockIdx.x * p.chunk, tokens = min(p.chunk, p.T - t0);
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int all = 0, b = 0;
-#pragma unroll 16
-    for (int ch = 0; ch < chunks; ++ch) {
-      const int n = p.chunk_rows[(size_t)ch * p.E + e];
-      all += n;
-      b += ch < (int)blockIdx.x ? n : 0;
+  {
+    // four experts a thread, the chunks shared among as many groups of threads as there are
+    const int quads = pitch / 4, groups = RL_PLACE_THREADS / quads, g = (int)threadIdx.x / quads, q = (int)threadIdx.x % quads;
+    if (g < groups) {
+      int all[4] = {}, b[4] = {};
+#pragma unroll 8
+      for (int ch = g; ch < chunks; ch += groups) {
+        const uint32_t n = __ldcg(reinterpret_cast<const uint32_t *>(p.chunk_rows + (size_t)ch * pitch) + q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v = (int)((n >> (8 * i)) & 255u);
+          all[i] += v;
+          b[i] += ch < (int)blockIdx.x ? v : 0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        atomicAdd(cnt + 4 * q + i, all[i]);
+        atomicAdd(before + 4 * q + i, b[i]);
+      }
     }
-    cnt[e] = all;
-    before[e] = b;
-    if (blockIdx.x == 0) p.expert_rows[e] = all;
   }
-  rl_mark(mask, words, p.idx + (long)t0 * p.k, tokens * p.k, p.k, p.E);
+  const int32_t *idx = p.idx + (long)t0 * p.k;
+  rl_mark(mask, words, idx, tokens * p.k, p.k, p.E);
   if (threadIdx.x < 32) rl_scan(cnt, off, p.E, threadIdx.x);
   __syncthreads();
   const int total = off[p.E];
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) before[e] += off[e];
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    before[e] += off[e];
+    if (blockIdx.x == 0) p.expert_rows[e] = cnt[e];
+  }
   __syncthreads();
-  rl_place(p, mask, before, t0, tokens);
+  for (int i = threadIdx.x; i < tokens * p.k; i += blockDim.x) {
+    const int e = idx[i], j = i / p.k;
+    int slot = -1;
+    if (e >= 0) {
+      slot = before[e] + rl_rank(mask + e * words, words, j);
+      p.row_token[slot] = t0 + j;
+    }
+    p.slot[(long)t0 * p.k + i] = slot;
+  }
   for (long i = (long)total + blockIdx.x * blockDim.x + threadIdx.x; i < (long)p.T * p.k; i += (long)gridDim.x * blockDim.x) p.row_token[i] = -1;
 }
 
 template <typename T>
 static int launch_route_typed(const RouteLogitsParams &p, int chunks, int warps, size_t smem, cudaStream_t st) {
   static ColiPerDeviceOnce attr_once;
-  if (!coli_set_smem_limit(attr_once, k_route_logits<T>, RL_MAX_WARPS * (RL_CAND_BYTES + 512 * 8), "routing shared-memory attribute")) return 0;
+  if (!coli_set_smem_limit(attr_once, k_route_logits<T>, 128 * 32 * 4 + RL_MAX_WARPS * (RL_CAND_BYTES + 512 * 8), "routing shared-memory attribute")) return 0;
   coli_count_launch(1);
   return coli_cuda_check(launch_dependent(k_route_logits<T>, dim3(chunks), dim3(warps * 32), smem, st, p), "routing launch") ? 1 : 0;
 }
@@ -507,15 +541,16 @@ int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
   const int chunks = (p.T + p.chunk - 1) / p.chunk, words = p.chunk / 32;
   // a warp per token up to 32; a few more for the tables where there are few tokens
   const int tokens = p.T < p.chunk ? p.T : p.chunk, warps = tokens < 4 ? 4 : tokens < RL_MAX_WARPS ? tokens : RL_MAX_WARPS;
-  const size_t tables = (size_t)p.E * words * 4 + (3 * (size_t)p.E + 1) * 4;
-  size_t smem = (size_t)warps * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));
-  if (smem < tables) smem = tables;
+  const size_t pitch = (p.E + 3) & ~3, own = (size_t)warps * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));
+  const size_t marks = (size_t)p.E * words * 4;
+  const size_t smem = (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15) + (own > marks ? own : marks);
+  const size_t tables = marks + (2 * pitch + p.E + 1) * 4;
   const int ok = p.type == COLI_TYPE_F32   ? launch_route_typed<float>(p, chunks, warps, smem, st)
                  : p.type == COLI_TYPE_F16 ? launch_route_typed<__half>(p, chunks, warps, smem, st)
                                            : launch_route_typed<__nv_bfloat16>(p, chunks, warps, smem, st);
   if (!ok || chunks == 1) return ok;
   coli_count_launch(1);
-  return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(512), tables, st, p, chunks), "placement launch") ? 1 : 0;
+  return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(RL_PLACE_THREADS), tables, st, p, chunks), "placement launch") ? 1 : 0;
 }
 
 }  // namespace colib
