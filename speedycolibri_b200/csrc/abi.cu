@@ -1385,22 +1385,37 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
   d.y_type = COLI_TYPE_BF16;
   d.y_stride = H;
   d.y_vec = true;  // H is a multiple of 8
-  // what stands between the two products takes the place of the 16-bit h: segments of a few rows leave h in f32, longer ones
-  // its codes and behind them its scales
+  // What stands between the two products takes the place of the 16-bit h: its codes and behind them its scales; segments
+  // of a few rows, whose kernel makes 16 features at a time, leave h in f32 behind those for the row quantiser.
   const bool few = colib::fp8_stream_ok(p);
-  const size_t need = few ? (size_t)rows_cap * I * 4 : (size_t)rows_cap * (h_ld + 4 * ((I + 127) / 128));
+  const int blocks = (I + 127) / 128;
+  const size_t codes_bytes = (size_t)rows_cap * h_ld, scale_bytes = ((size_t)rows_cap * blocks * 4 + 15) / 16 * 16;
+  const size_t need = codes_bytes + scale_bytes + (few ? (size_t)rows_cap * I * 4 : 0);
   if (!ensure_h(m, m->seg_main, (need + 2 * (size_t)I - 1) / (2 * (size_t)I))) return 0;
   uint8_t *h = (uint8_t *)m->seg_main.h;
-  if (few) {
-    p.h32 = d.h32 = (float *)h;
-  } else {
+  float *hs = (float *)(h + codes_bytes);
+  d.codes = h;
+  d.sx = hs;
+  if (!few) {
     p.h_codes = h;
-    p.h_scales = (float *)(h + (size_t)rows_cap * h_ld);
+    p.h_scales = hs;
     p.h_ld = h_ld;
-    d.codes = h;
-    d.sx = p.h_scales;
+    return colib::launch_fp8_mm(p, st) && colib::launch_fp8_mm(d, st);
   }
-  return colib::launch_fp8_mm(p, st) && colib::launch_fp8_mm(d, st);
+  p.h32 = (float *)(h + codes_bytes + scale_bytes);
+  colib::QuantRowsParams q = {};
+  q.x = p.h32;
+  q.type = COLI_TYPE_F32;
+  q.x_stride = I;
+  q.x_vec = true;  // I is a multiple of 8
+  q.T = q.rows = rows_cap;
+  q.K = I;
+  q.codes = h;
+  q.ld = h_ld;
+  q.scales = hs;
+  q.s_row = 1;
+  q.s_blk = rows_cap;
+  return colib::launch_fp8_mm(p, st) && colib::launch_quant_rows(q, st) && colib::launch_fp8_mm(d, st);
 }
 
 extern "C" int coli_b200_moe_experts_fp8_dev(ColiMoe *m, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row, int64_t s_blk,

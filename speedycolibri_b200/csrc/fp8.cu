@@ -715,7 +715,7 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   }
   p.KT = (p.K + 127) / 128;
   p.Op = round_up(p.O, 16);
-  if (p.h32 || fp8_stream_ok(p)) return launch_fp8_stream(p, st);
+  if (fp8_stream_ok(p)) return launch_fp8_stream(p, st);
   const bool gated = p.h_codes != nullptr;
   // Row tiles the call is likely to have, and the most it can have.  Both are functions of the call's shapes alone.
   const int most = p.seg_count ? p.rows / F8_BM + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + F8_BM - 1) / F8_BM;

@@ -36,8 +36,7 @@ struct Fp8MmParams {
   uint8_t *h_codes;          // when not null: h = act(w0 x, w1 x) quantised again: codes [rows, O], h_ld bytes apart,
   float *h_scales;           // and scales [ceil(O / 128)][rows]
   long h_ld;
-  float *h32;                // segments of a few rows: h as it is, f32 [rows, O or K]: written instead of h_codes when w1 is
-                             // given, and otherwise read in place of codes and quantised on the way, behind the call that wrote it
+  float *h32;                // segments of a few rows (fp8_stream_ok) instead: h as it is, f32 [rows, O]
   ActParams act;
   int *status;               // device word for a bounded wait that gave up, or null: the library's own
   // filled in by the launcher
