@@ -1403,6 +1403,7 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
     return colib::launch_fp8_mm(p, st) && colib::launch_fp8_mm(d, st);
   }
   p.h32 = (float *)(h + codes_bytes + scale_bytes);
+  d.behind_gated = true;
   colib::QuantRowsParams q = {};
   q.x = p.h32;
   q.type = COLI_TYPE_F32;

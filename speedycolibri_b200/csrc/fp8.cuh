@@ -37,6 +37,7 @@ struct Fp8MmParams {
   float *h_scales;           // and scales [ceil(O / 128)][rows]
   long h_ld;
   float *h32;                // segments of a few rows (fp8_stream_ok) instead: h as it is, f32 [rows, O]
+  bool behind_gated;         // segments of a few rows: the launches before this one are the gated call's and the row quantiser's
   ActParams act;
   int *status;               // device word for a bounded wait that gave up, or null: the library's own
   // filled in by the launcher

@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // Counts, codes and scales of rows are written by earlier launches; weights are not.  One segment's table needs no counts.
-  const bool early = !p.seg_count;
+  // Behind the gated call and the quantiser the counts are complete: the gated call lets its successor start after its own wait.
+  const bool early = !p.seg_count || p.behind_gated;
   if (!early) coli_grid_wait();
   if (warp == 0) f8_tables<ROWS>(p, row_off, tile_off, lane);
   __syncthreads();
@@ -92,23 +93,39 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   int issued = 0, i_task = first, i_kt = kt0, i_slot = 0, i_rows = 0;
   const uint8_t *q0 = nullptr, *q1 = nullptr, *codes = nullptr;
   const float *scale = nullptr;  // lanes 0 .. ROWS - 1: their row's; the next two: the weights'
-  long scale_step = 0;
   bool both = true, alive = true;
+  // where a task's operands are, looked up a task ahead (the expert's index and its table entry are two reads in a row)
+  struct Task {
+    const uint8_t *q0, *q1;
+    const float *scale;
+    int row0, nrows;
+    bool both;
+  } ahead_task = {};
+  auto look_up = [&](int task) {
+    if (task >= tasks) return;
+    const F8Tile tile = f8_tile<ROWS>(tile_off, row_off, p.nseg, task);
+    const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+    const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
+    const int f0 = tile.nt * (GATED ? 16 : 16 * M);
+    ahead_task.q0 = w0.q + (size_t)f0 * 128;
+    ahead_task.q1 = w1.q + (size_t)f0 * 128;
+    ahead_task.scale = lane < ROWS ? p.sx + (long)(tile.row0 + min(lane, tile.nrows - 1)) * p.s_row
+                                   : reinterpret_cast<const float *>(lane == ROWS ? w0.s : w1.s) + (size_t)(f0 >> 7) * p.KT;
+    ahead_task.row0 = tile.row0;
+    ahead_task.nrows = tile.nrows;
+    ahead_task.both = f0 + 16 * M <= p.Op;
+  };
+  if (works) look_up(first);
+  const long scale_step = lane < ROWS ? p.s_blk : 1;
   auto issue_weights = [&]() {
     if (i_kt == kt0) {
-      const F8Tile tile = f8_tile<ROWS>(tile_off, row_off, p.nseg, i_task);
-      const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
-      const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
-      const int f0 = tile.nt * (GATED ? 16 : 16 * M);
-      q0 = w0.q + (size_t)f0 * 128 + lane * 16;
-      q1 = w1.q + (size_t)f0 * 128 + lane * 16;
-      both = f0 + 16 * M <= p.Op;
-      i_rows = tile.nrows;
-      codes = (const uint8_t *)p.codes + (long)(tile.row0 + (lane >> 3)) * p.ld + (lane & 7) * 16;
-      const bool row = lane < ROWS;
-      scale = row ? p.sx + (long)(tile.row0 + min(lane, i_rows - 1)) * p.s_row
-                  : reinterpret_cast<const float *>(lane == ROWS ? w0.s : w1.s) + (size_t)(f0 >> 7) * p.KT;
-      scale_step = row ? p.s_blk : 1;
+      q0 = ahead_task.q0 + lane * 16;
+      q1 = ahead_task.q1 + lane * 16;
+      both = ahead_task.both;
+      i_rows = ahead_task.nrows;
+      codes = (const uint8_t *)p.codes + (long)(ahead_task.row0 + (lane >> 3)) * p.ld + (lane & 7) * 16;
+      scale = ahead_task.scale;
+      look_up(i_task + stride);
     }
     const uint32_t dst = ring + (uint32_t)i_slot * S::UNIT + (uint32_t)lane * 16;
     const size_t off = (size_t)i_kt * p.Op * 128;
