@@ -533,8 +533,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     tile.nrows = 0;
     uint32_t chunk = 0;  // of scales, so far
     float nx = 0.0f, nw0 = 0.0f, nw1 = 0.0f;
-    // This thread's scales of k-tile kb, requested a k-tile ahead: beside the products' operands a read of shared memory takes
-    // two to three hundred cycles.
+    // this thread's scales of k-tile kb
     auto scales_of = [&](int kb) {
       const uint32_t u = (uint32_t)(kb - kb0) % F8_CHUNK;
       if (u == 0) alive = alive && __all_sync(0xffffffffu, mbar_wait(scaled + 8 * (chunk & 1u), (chunk >> 1) & 1u, abort_flag, status, TC_ERR_EPI_WAIT));
@@ -548,10 +547,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         ++chunk;
       }
     };
-    if (cluster0 < n_tiles) {
-      recall(tile);
-      scales_of(kb0);
-    }
+    if (cluster0 < n_tiles) recall(tile);
     for (int t = cluster0; t < n_tiles; t += clusters) {
       const bool any = (warp & 3) * 32 < tile.nrows;
       float2 acc[NACC / 2];
@@ -559,8 +555,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       for (int i = 0; i < NACC / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t d = it & 1u, dph = (it >> 1) & 1u;
+        scales_of(kb);
         const float s0 = nx * nw0, s1 = GATED ? nx * nw1 : s0;
-        if (kb + 1 < kb1) scales_of(kb + 1);
         alive = alive && __all_sync(0xffffffffu, mbar_wait(dfull + 8 * d, dph, abort_flag, status, TC_ERR_EPI_WAIT));
         tc_fence_after();
         if (any && alive) {
@@ -646,10 +642,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
           f8_store_rows<OutT, NACC>(smem + S::RING + warp * 32 * S::OUT_LD, (OutT *)p.y + (long)(tile.row0 + r0) * p.y_stride + f, p.y_stride, flat,
                                     tile.nrows - r0, p.O - f, p.y_vec, lane);
       }
-      if (t + clusters < n_tiles) {
-        recall(tile);
-        scales_of(kb0);
-      }
+      if (t + clusters < n_tiles) recall(tile);
     }
   }
   tc_fence_before();
