@@ -174,18 +174,21 @@ struct F8Info {
   int nt, row0, nrows, pad;
 };
 constexpr int F8_INFOS = 4;
-constexpr int F8_CHUNK = 8;   // k-tiles whose scales are handed over at once
-template <int BN>
+constexpr int F8_OUT_LD = 64 + 16;  // bytes a row of a warp's staged results: eight rows start in different banks
+constexpr int F8_CHUNK = 4;   // k-tiles whose scales are handed over at once
+// AR: rows of a tile.  The products always take 128: where segments are short, 64 or 32 rows stand two or four times in a stage, so
+// that all four quarters of tensor memory hold them and every summing warp takes a half or a quarter of the features it would.
+template <int BN, int AR>
 struct F8Smem {
+  static constexpr int DUP = F8_BM / AR, PARTS = 2 * DUP;  // copies of the rows; shares of the features
   static constexpr int A_BYTES = F8_BM * 128;
   static constexpr int B_BYTES = BN * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 3 : 5;
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
   static constexpr int RED_LD = BN + 4;  // f32 a row of partial sums: rows start 4 banks apart
   static constexpr int RING = STAGES * STAGE;
-  static_assert(F8_BM * RED_LD * 4 <= RING, "partial sums take the ring's place");
-  static constexpr int OUT_LD = 128 + 16;  // bytes a row of a warp's staged results: rows start 4 banks apart
-  static constexpr int OUT = F8_EPI_WARPS * 32 * OUT_LD;
+  static_assert(AR * RED_LD * 4 <= RING, "partial sums take the ring's place");
+  static constexpr int OUT = F8_EPI_WARPS * 32 * F8_OUT_LD;
   static constexpr int INFOS = F8_INFOS * (int)sizeof(F8Info);
   static constexpr int SCALES = 2 * F8_CHUNK * (F8_BM + 2) * 4;  // two chunks: [k-tile][row] of sx, then [k-tile][block of features] of sw
   static constexpr int BARS = 2 * STAGES + 4 + 2 * F8_INFOS + 4;
@@ -233,29 +236,29 @@ __device__ __forceinline__ void f8_store4(OutT *dst, const float (&v)[4], int va
       if (j < valid) dst[j] = o[j];
   }
 }
-// A warp's 32 rows x N columns, a row in each lane, to y: 128 bytes of every row at a time through shared memory, so that a
-// store instruction writes whole lines of four rows (lane by lane it is 32 lines of 16 bytes: 5600 cycles a tile of 128 x 256,
+// A warp's 32 rows x N columns, a row in each lane, to y: 64 bytes of every row at a time through shared memory, so that a
+// store instruction writes eight rows' whole sectors (lane by lane it is 32 rows' halves: 5600 cycles a tile of 128 x 256,
 // of 16 k-tiles at 1180).
 template <typename OutT, int N>
 __device__ __forceinline__ void f8_store_rows(unsigned char *stage, OutT *y, long stride, const float *acc, int rows, int cols, bool vec, int lane) {
-  constexpr int LD = F8Smem<256>::OUT_LD, PER = 16 / (int)sizeof(OutT), CH = 128 / (int)sizeof(OutT);
+  constexpr int LD = F8_OUT_LD, PER = 16 / (int)sizeof(OutT), CH = 64 / (int)sizeof(OutT);
   const uint32_t at = smem_u32(stage);
 #pragma unroll
   for (int c = 0; c < N / CH; ++c) {
     if (c * CH >= cols) break;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       alignas(16) OutT o[PER];
 #pragma unroll
       for (int j = 0; j < PER; ++j) o[j] = f8_out<OutT>(acc[c * CH + i * PER + j]);
       *reinterpret_cast<uint4 *>(stage + lane * LD + 16 * i) = *reinterpret_cast<const uint4 *>(o);
     }
     __syncwarp();
-    const int col = c * CH + (lane & 7) * PER;
+    const int col = c * CH + (lane & 3) * PER;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3);
-      const uint4 v = lds128(at + (uint32_t)(r * LD + 16 * (lane & 7)));
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      const uint4 v = lds128(at + (uint32_t)(r * LD + 16 * (lane & 3)));
       if (r < rows) {
         OutT *dst = y + (long)r * stride + col;
         if (vec && col + PER <= cols) {
@@ -272,17 +275,6 @@ __device__ __forceinline__ void f8_store_rows(unsigned char *stage, OutT *y, lon
   }
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
 // c += (x, y) * s
 __device__ __forceinline__ void f8_add_scaled(float2 &c, float x, float y, float s) {
   uint64_t cc, v, ss;
@@ -302,7 +294,7 @@ __device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &
   for (int r = 0; r < world; ++r) {
 #pragma unroll
     for (int j = 0; j < BN / 128; ++j) {
-      const float4 u = ld_cluster4(red + (uint32_t)(i * F8Smem<BN>::RED_LD + 128 * j + 4 * lane) * 4u, (uint32_t)r);
+      const float4 u = ld_cluster4(red + (uint32_t)(i * (BN + 4) + 128 * j + 4 * lane) * 4u, (uint32_t)r);
       v[j].x += u.x;
       v[j].y += u.y;
       v[j].z += u.z;
@@ -336,10 +328,10 @@ __device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &
 // GATED: features of two weights, h = act(gate, up), quantised again as rows (one scale per row and 128 features).
 // SPLIT: the CTAs of a cluster share the k-tiles of one tile and join their sums, in rank order, through distributed
 // shared memory: for calls with too few tiles for the SMs.
-template <bool GATED, int BN, bool SPLIT, typename OutT>
+template <bool GATED, int BN, int AR, bool SPLIT, typename OutT>
 __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant__ F8Maps maps, const Fp8MmParams p) {
-  using S = F8Smem<BN>;
-  constexpr int NACC = BN / 2;
+  using S = F8Smem<BN, AR>;
+  constexpr int DUP = S::DUP, PARTS = S::PARTS, NACC = BN / PARTS, HF = NACC / 2;  // a thread's sums; of those, GATED, of gate
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = smem_u32(smem);
@@ -353,7 +345,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *row_off = reinterpret_cast<int *>(after + 8 * S::BARS + 16);
   int *tile_off = row_off + F8_MAX_SEGS + 1;
-  float *amax_s = reinterpret_cast<float *>(tile_off + F8_MAX_SEGS + 1);  // [tile parity][half][row]
+  float *amax_s = reinterpret_cast<float *>(tile_off + F8_MAX_SEGS + 1);  // [tile parity][share][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int *status = p.status;
 
@@ -383,7 +375,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     tc_fence_before();
   }
   coli_grid_dependency_sync();  // (the set-up above overlaps the predecessor's end)
-  if (warp == 0) f8_tables<F8_BM>(p, row_off, tile_off, lane);
+  if (warp == 0) f8_tables<AR>(p, row_off, tile_off, lane);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -421,14 +413,15 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         const uint32_t nb = (uint32_t)min(GATED ? 128 : BN, p.Op - f0) * 128u;
         int box = 0;
         while ((8 << box) < tile.nrows) ++box;
-        const uint32_t bytes = (uint32_t)(8 << box) * 128u + (GATED ? 2 * nb : nb);
+        const uint32_t bytes = (uint32_t)(8 << box) * 128u * DUP + (GATED ? 2 * nb : nb);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u;
           alive = alive && __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
           if (alive && elect_one()) {
             const uint32_t a = ring + s * S::STAGE, b = a + S::A_BYTES, bar = full + 8 * s;
             mbar_expect_tx(bar, bytes);
-            tma_load_2d(a, &maps.m[box], kb * 128, tile.row0, bar);
+#pragma unroll
+            for (int j = 0; j < DUP; ++j) tma_load_2d(a + j * AR * 128, &maps.m[box], kb * 128, tile.row0, bar);
             const size_t at = (size_t)kb * p.Op * 128;
             bulk_load(b, tile.q0 + at, nb, bar);
             if (GATED) bulk_load(b + 128 * 128, tile.q1 + at, nb, bar);
@@ -469,7 +462,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       // ---------------- tiles ahead ----------------
       for (int t = cluster0; t < n_tiles; t += clusters, ++nth) {
         const uint32_t s = nth % F8_INFOS, ph = (nth / F8_INFOS) & 1u;
-        const F8Tile tile = f8_tile<F8_BM>(tile_off, row_off, p.nseg, t);
+        const F8Tile tile = f8_tile<AR>(tile_off, row_off, p.nseg, t);
         const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
         const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
         const int f0 = tile.nt * (GATED ? 128 : BN);
@@ -527,7 +520,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
   } else {
     // ---------------- scaled sums ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_SUM));
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int r0 = (warp & 3) % (AR / 32) * 32, row = r0 + lane, part = (warp >> 2) * DUP + (warp & 3) / (AR / 32);
     const uint32_t tbase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     F8Info tile;
     tile.nrows = 0;
@@ -539,7 +532,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       if (u == 0) alive = alive && __all_sync(0xffffffffu, mbar_wait(scaled + 8 * (chunk & 1u), (chunk >> 1) & 1u, abort_flag, status, TC_ERR_EPI_WAIT));
       const float *at = scales + (chunk & 1u) * (F8_CHUNK * (F8_BM + 2));
       nx = at[u * F8_BM + row];
-      nw0 = at[F8_CHUNK * F8_BM + 2 * u + (GATED || BN == 128 ? 0 : half)];
+      nw0 = at[F8_CHUNK * F8_BM + 2 * u + (GATED ? 0 : (part * NACC) >> 7)];
       if (GATED) nw1 = at[F8_CHUNK * F8_BM + 2 * u + 1];
       if (u == F8_CHUNK - 1 || kb + 1 == kb1) {
         __syncwarp();
@@ -549,7 +542,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     };
     if (cluster0 < n_tiles) recall(tile);
     for (int t = cluster0; t < n_tiles; t += clusters) {
-      const bool any = (warp & 3) * 32 < tile.nrows;
+      const bool any = r0 < tile.nrows;
       float2 acc[NACC / 2];
 #pragma unroll
       for (int i = 0; i < NACC / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
@@ -563,9 +556,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
           // FLY loads of 16 columns at a time, the next ones requested as each is added, so that the buffer goes back to the
           // products after few round trips (with 64 columns on their way the sums no longer fit the registers); two sums an
           // instruction.
-          constexpr int CH = NACC / 16, FLY = CH == 8 ? 3 : 4;
+          constexpr int CH = NACC / 16, FLY = CH == 8 ? 3 : CH;
           uint32_t v[FLY][16];
-          auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < CH / 2 ? 64 * half + 16 * c : 128 + 64 * half + 16 * (c - CH / 2)) : half * NACC + 16 * c); };
+          auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < CH / 2 ? HF * part + 16 * c : 128 + HF * part + 16 * (c - CH / 2)) : part * NACC + 16 * c); };
 #pragma unroll
           for (int c = 0; c < FLY; ++c) tmem_ld16(column(c), v[c]);
 #pragma unroll
@@ -598,7 +591,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         if (mine && alive) {
 #pragma unroll
           for (int c = 0; c < NACC / 4; ++c) {
-            const int col = GATED ? (4 * c < 64 ? 64 * half + 4 * c : 128 + 64 * half + 4 * c - 64) : half * NACC + 4 * c;
+            const int col = GATED ? (4 * c < HF ? HF * part + 4 * c : 128 + HF * part + 4 * c - HF) : part * NACC + 4 * c;
             *reinterpret_cast<float4 *>(red + row * S::RED_LD + col) = make_float4(flat[4 * c], flat[4 * c + 1], flat[4 * c + 2], flat[4 * c + 3]);
           }
         }
@@ -608,38 +601,39 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is copied into again
         meet();
       } else if constexpr (GATED) {
-        // h of 64 features, the row's largest together with the other half's, codes
+        // h of this share's features, the row's largest together with the other shares', codes
         float a = 0.0f;
-        const int left = p.O - tile.nt * 128 - 64 * half;  // features that exist
+        const int f0 = tile.nt * 128 + HF * part, left = p.O - f0;  // features that exist
         if (any) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const float h = coli_act_fast(flat[i], flat[64 + i], p.act);  // (selected, not branched around: the 64 chains overlap)
+          for (int i = 0; i < HF; ++i) {
+            const float h = coli_act_fast(flat[i], flat[HF + i], p.act);  // (selected, not branched around: the chains overlap)
             flat[i] = i < left ? h : 0.0f;
             a = fmaxf(a, fabsf(flat[i]));
           }
         }
-        float *am = amax_s + ((t / clusters) & 1) * 2 * F8_BM;
-        am[half * F8_BM + row] = a;
+        float *am = amax_s + ((t / clusters) & 1) * PARTS * AR + row;
+        am[part * AR] = a;
         asm volatile("bar.sync 1, %0;" ::"n"(F8_EPI_WARPS * 32) : "memory");
-        a = fmaxf(a, am[(half ^ 1) * F8_BM + row]);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) a = fmaxf(a, am[i * AR]);
         const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
         if (mine && alive) {
-          uint8_t *dst = p.h_codes + (size_t)(tile.row0 + row) * p.h_ld + tile.nt * 128 + 64 * half;
+          uint8_t *dst = p.h_codes + (size_t)(tile.row0 + row) * p.h_ld + f0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < HF / 16; ++c) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w[i] = e4m3x4(flat[16 * c + 4 * i] * inv, flat[16 * c + 4 * i + 1] * inv, flat[16 * c + 4 * i + 2] * inv, flat[16 * c + 4 * i + 3] * inv);
-            if (tile.nt * 128 + 64 * half + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (f0 + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (half == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
+          if (part == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
         }
       } else {
-        const int f = tile.nt * BN + half * NACC, r0 = (warp & 3) * 32;
+        const int f = tile.nt * BN + part * NACC;
         if (any && alive && f < p.O)
-          f8_store_rows<OutT, NACC>(smem + S::RING + warp * 32 * S::OUT_LD, (OutT *)p.y + (long)(tile.row0 + r0) * p.y_stride + f, p.y_stride, flat,
+          f8_store_rows<OutT, NACC>(smem + S::RING + warp * 32 * F8_OUT_LD, (OutT *)p.y + (long)(tile.row0 + r0) * p.y_stride + f, p.y_stride, flat,
                                     tile.nrows - r0, p.O - f, p.y_vec, lane);
       }
       if (t + clusters < n_tiles) recall(tile);
@@ -671,15 +665,16 @@ static bool make_codes_map(CUtensorMap *map, const void *base, int rows, int K, 
   return true;
 }
 
-template <bool GATED, int BN, bool SPLIT, typename OutT>
+template <bool GATED, int BN, int AR, bool SPLIT, typename OutT>
 static int launch_f8(const F8Maps &maps, const Fp8MmParams &p, int grid, cudaStream_t st) {
   static ColiPerDeviceOnce attr_once;
-  auto *kernel = k_fp8_mm<GATED, BN, SPLIT, OutT>;
-  if (!coli_set_smem_limit(attr_once, kernel, F8Smem<BN>::BYTES, "fp8 product shared-memory attribute")) return 0;
+  auto *kernel = k_fp8_mm<GATED, BN, AR, SPLIT, OutT>;
+  constexpr int bytes = F8Smem<BN, AR>::BYTES;
+  if (!coli_set_smem_limit(attr_once, kernel, bytes, "fp8 product shared-memory attribute")) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(F8_THREADS);
-  cfg.dynamicSmemBytes = F8Smem<BN>::BYTES;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -692,11 +687,18 @@ static int launch_f8(const F8Maps &maps, const Fp8MmParams &p, int grid, cudaStr
   coli_count_launch(1);
   return coli_cuda_check(cudaLaunchKernelEx(&cfg, kernel, maps, p), "fp8 product launch") ? 1 : 0;
 }
+template <bool GATED, int BN, typename OutT>
+static int launch_f8_rows(const F8Maps &maps, const Fp8MmParams &p, int ar, int grid, cudaStream_t st) {
+  if constexpr (BN == 256)
+    if (ar == 32) return p.split > 1 ? launch_f8<GATED, BN, 32, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 32, false, OutT>(maps, p, grid, st);
+  if (ar <= 64) return p.split > 1 ? launch_f8<GATED, BN, 64, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 64, false, OutT>(maps, p, grid, st);
+  return p.split > 1 ? launch_f8<GATED, BN, 128, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 128, false, OutT>(maps, p, grid, st);
+}
 template <bool GATED, typename OutT>
-static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int grid, cudaStream_t st) {
+static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int ar, int grid, cudaStream_t st) {
   if constexpr (!GATED)
-    if (bn == 128) return p.split > 1 ? launch_f8<false, 128, true, OutT>(maps, p, grid, st) : launch_f8<false, 128, false, OutT>(maps, p, grid, st);
-  return p.split > 1 ? launch_f8<GATED, 256, true, OutT>(maps, p, grid, st) : launch_f8<GATED, 256, false, OutT>(maps, p, grid, st);
+    if (bn == 128) return launch_f8_rows<false, 128, OutT>(maps, p, ar, grid, st);
+  return launch_f8_rows<GATED, 256, OutT>(maps, p, ar, grid, st);
 }
 
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
@@ -710,11 +712,15 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   p.Op = round_up(p.O, 16);
   if (fp8_stream_ok(p)) return launch_fp8_stream(p, st);
   const bool gated = p.h_codes != nullptr;
-  // Row tiles the call is likely to have, and the most it can have.  Both are functions of the call's shapes alone.
-  const int most = p.seg_count ? p.rows / F8_BM + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + F8_BM - 1) / F8_BM;
-  const int likely = p.seg_count ? p.rows_expected / F8_BM + (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : most;
+  // Rows of a tile, row tiles the call is likely to have, and the most it can have.  All are functions of the call's shapes alone.
+  const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
+  const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
+  int ar = mean <= (p.seg_count ? 40 : 64) ? 64 : 128;
+  if (mean <= (p.seg_count ? 16 : 32)) ar = 32;
+  const int most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + ar - 1) / ar;
+  const int likely = p.seg_count ? p.rows_expected / ar + segs : most;
   int bn = 256;
-  if (!gated && (long)likely * ((p.O + 255) / 256) < COLI_SMS) bn = 128;
+  if (!gated && (long)likely * ((p.O + 255) / 256) < COLI_SMS) bn = 128, ar = ar < 64 ? 64 : ar;
   const int fw = gated ? 128 : bn;
   p.n_tiles = (p.O + fw - 1) / fw;
   const long tiles = (long)(likely > 0 ? likely : 1) * p.n_tiles;
@@ -727,16 +733,16 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
     while ((8 << b) < n) ++b;
     return b;
   };
-  const int last = p.rows % F8_BM ? p.rows % F8_BM : F8_BM;
+  const int last = p.rows % ar ? p.rows % ar : ar;
   for (int b = 0; b < F8_MAPS; ++b)
-    if (p.seg_count || b == box_of(last) || (b == F8_MAPS - 1 && p.rows >= F8_BM))
+    if (p.seg_count || b == box_of(last) || (b == box_of(ar) && p.rows >= ar))
       if (!make_codes_map(&maps.m[b], p.codes, p.rows, p.K, p.ld, 8 << b)) return 0;
   const long bound = (long)most * p.n_tiles;
   const int clusters = (int)(bound < COLI_SMS / p.split ? bound : COLI_SMS / p.split);
-  if (gated) return launch_f8_shape<true, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);
-  if (p.y_type == COLI_TYPE_F32) return launch_f8_shape<false, float>(maps, p, bn, clusters * p.split, st);
-  if (p.y_type == COLI_TYPE_F16) return launch_f8_shape<false, __half>(maps, p, bn, clusters * p.split, st);
-  return launch_f8_shape<false, __nv_bfloat16>(maps, p, bn, clusters * p.split, st);
+  if (gated) return launch_f8_shape<true, __nv_bfloat16>(maps, p, bn, ar, clusters * p.split, st);
+  if (p.y_type == COLI_TYPE_F32) return launch_f8_shape<false, float>(maps, p, bn, ar, clusters * p.split, st);
+  if (p.y_type == COLI_TYPE_F16) return launch_f8_shape<false, __half>(maps, p, bn, ar, clusters * p.split, st);
+  return launch_f8_shape<false, __nv_bfloat16>(maps, p, bn, ar, clusters * p.split, st);
 }
 
 // Device address of the current device's status word, looked up once per device (as the routing scratch is).
