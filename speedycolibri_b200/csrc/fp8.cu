@@ -525,19 +525,28 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     F8Info tile;
     tile.nrows = 0;
     uint32_t chunk = 0;  // of scales, so far
-    float nx = 0.0f, nw0 = 0.0f, nw1 = 0.0f;
-    // this thread's scales of k-tile kb
+    // This thread's scales of the next k-tiles, read a chunk at a time: beside the products' operands a read of shared memory
+    // takes some two hundred cycles.
+    float sc0[F8_CHUNK] = {}, sc1[F8_CHUNK] = {};
     auto scales_of = [&](int kb) {
-      const uint32_t u = (uint32_t)(kb - kb0) % F8_CHUNK;
-      if (u == 0) alive = alive && __all_sync(0xffffffffu, mbar_wait(scaled + 8 * (chunk & 1u), (chunk >> 1) & 1u, abort_flag, status, TC_ERR_EPI_WAIT));
-      const float *at = scales + (chunk & 1u) * (F8_CHUNK * (F8_BM + 2));
-      nx = at[u * F8_BM + row];
-      nw0 = at[F8_CHUNK * F8_BM + 2 * u + (GATED ? 0 : (part * NACC) >> 7)];
-      if (GATED) nw1 = at[F8_CHUNK * F8_BM + 2 * u + 1];
-      if (u == F8_CHUNK - 1 || kb + 1 == kb1) {
+      if ((uint32_t)(kb - kb0) % F8_CHUNK == 0) {
+        alive = alive && __all_sync(0xffffffffu, mbar_wait(scaled + 8 * (chunk & 1u), (chunk >> 1) & 1u, abort_flag, status, TC_ERR_EPI_WAIT));
+        const float *at = scales + (chunk & 1u) * (F8_CHUNK * (F8_BM + 2)), *w = at + F8_CHUNK * F8_BM + (GATED ? 0 : (part * NACC) >> 7);
+#pragma unroll
+        for (int u = 0; u < F8_CHUNK; ++u) {
+          const float x = at[u * F8_BM + row];
+          sc0[u] = x * w[2 * u];
+          if (GATED) sc1[u] = x * w[2 * u + 1];
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(unscaled + 8 * (chunk & 1u));
         ++chunk;
+      } else {
+#pragma unroll
+        for (int u = 0; u + 1 < F8_CHUNK; ++u) {
+          sc0[u] = sc0[u + 1];
+          if (GATED) sc1[u] = sc1[u + 1];
+        }
       }
     };
     if (cluster0 < n_tiles) recall(tile);
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t d = it & 1u, dph = (it >> 1) & 1u;
         scales_of(kb);
-        const float s0 = nx * nw0, s1 = GATED ? nx * nw1 : s0;
+        const float s0 = sc0[0], s1 = GATED ? sc1[0] : s0;
         alive = alive && __all_sync(0xffffffffu, mbar_wait(dfull + 8 * d, dph, abort_flag, status, TC_ERR_EPI_WAIT));
         tc_fence_after();
         if (any && alive) {
