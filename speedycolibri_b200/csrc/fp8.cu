@@ -442,16 +442,17 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       for (int t = cluster0; t < n_tiles; t += clusters) {
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t s = it % S::STAGES, ph = (it / S::STAGES) & 1u, d = it & 1u, dph = (it >> 1) & 1u;
-          alive = alive && __all_sync(0xffffffffu, mbar_wait(dempty + 8 * d, dph ^ 1u, abort_flag, status, TC_ERR_MMA_WAIT));
+          // (the buffer last: the sums give it back late, and a look at a barrier takes over a hundred cycles here)
           alive = alive && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, ph, abort_flag, status, TC_ERR_MMA_WAIT));
+          alive = alive && __all_sync(0xffffffffu, mbar_wait(dempty + 8 * d, dph ^ 1u, abort_flag, status, TC_ERR_MMA_WAIT));
           tc_fence_after();
           if (alive && elect_one()) {
             const uint32_t a = ring + s * S::STAGE;
             const uint64_t ad = umma_smem_desc(a), bd = umma_smem_desc(a + S::A_BYTES);
 #pragma unroll
             for (int k = 0; k < 4; ++k) umma_f8(tmem + d * BN, ad + 2 * k, bd + 2 * k, idesc, k != 0);
-            umma_commit(empty + 8 * s);
             umma_commit(dfull + 8 * d);
+            umma_commit(empty + 8 * s);
           }
           __syncwarp();
         }
