@@ -1305,9 +1305,7 @@ extern "C" int coli_b200_fp8_check(int device) {
 }
 
 extern "C" size_t coli_b200_route_logits_workspace(int T, int E) {
-  if (T < 1 || E < 1) return 0;
-  const int c = colib::route_logits_chunk(T), chunks = (T + c - 1) / c;
-  return chunks == 1 ? 0 : (size_t)chunks * round_up(E, 4);
+  return T < 1 || E < 1 ? 0 : colib::route_logits_workspace(T, E);
 }
 
 extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int type, int64_t stride, const float *select_bias_dev,

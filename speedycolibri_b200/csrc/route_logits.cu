@@ -418,12 +418,47 @@ __device__ __forceinline__ void rl_scan(const int *cnt, int *off, int E, int lan
   }
 }
 
-// One CTA per chunk of tokens: routes them and counts their experts; where the call is one chunk, places them as well.
-template <typename T>
+// The pairs of a chunk take their rows: off = rows of all experts below, before = rows of the expert in earlier chunks.
+// cnt and before are summed, off has room for E + 1.
+__device__ __forceinline__ void rl_place(const RouteLogitsParams &p, const uint32_t *mask, int words, const int32_t *ids, const int *cnt, int *before,
+                                         int *off, int t0, int pairs) {
+  if (threadIdx.x < 32) rl_scan(cnt, off, p.E, threadIdx.x);
+  __syncthreads();
+  const int total = off[p.E];
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    before[e] += off[e];
+    if (blockIdx.x == 0) p.expert_rows[e] = cnt[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    const int e = ids[i], j = i / p.k;
+    int slot = -1;
+    if (e >= 0) {
+      slot = before[e] + rl_rank(mask + e * words, words, j);
+      p.row_token[slot] = t0 + j;
+    }
+    p.slot[(long)t0 * p.k + i] = slot;
+  }
+  for (long i = (long)total + blockIdx.x * blockDim.x + threadIdx.x; i < (long)p.T * p.k; i += (long)gridDim.x * blockDim.x) p.row_token[i] = -1;
+}
+__device__ __forceinline__ void rl_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int rl_cluster_load(const int *at, uint32_t rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// One CTA per chunk of tokens: routes them and counts their experts.  Where the call is one chunk it places them as well, and where it
+// is a few (CLUSTER: the chunks are one cluster, which reads one another's counts) they do together; else k_route_place does.
+template <typename T, bool CLUSTER>
 __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid_constant__ RouteLogitsParams p) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int t0 = blockIdx.x * p.chunk, tokens = min(p.chunk, p.T - t0), pairs = tokens * p.k, words = p.chunk / 32;
+  const int t0 = blockIdx.x * p.chunk, tokens = max(0, min(p.chunk, p.T - t0)), pairs = tokens * p.k, words = p.chunk / 32;
   int *ids = reinterpret_cast<int *>(rl_smem);  // the chunk's choices, then per-warp memory, later the tables
   unsigned char *after = rl_smem + (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15);
   unsigned char *cand = after + warp * RL_CAND_BYTES;
@@ -434,6 +469,32 @@ __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid
     __syncwarp();
   }
   __syncthreads();
+  if constexpr (CLUSTER) {
+    const int pitch = (p.E + 3) & ~3;
+    uint32_t *mask = reinterpret_cast<uint32_t *>(after);
+    int *mine = reinterpret_cast<int *>(mask + p.E * words), *cnt = mine + pitch, *before = cnt + pitch, *off = before + pitch;
+    rl_mark(mask, words, ids, pairs, p.k, p.E);
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+      int n = 0;
+      for (int w = 0; w < words; ++w) n += __popc(mask[e * words + w]);
+      mine[e] = n;
+    }
+    rl_cluster_sync();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+      int all = 0, b = 0;
+      for (uint32_t r = 0; r < gridDim.x; ++r) {
+        const int n = rl_cluster_load(mine + e, r);
+        all += n;
+        b += r < blockIdx.x ? n : 0;
+      }
+      cnt[e] = all;
+      before[e] = b;
+    }
+    __syncthreads();
+    rl_place(p, mask, words, ids, cnt, before, off, t0, pairs);
+    rl_cluster_sync();  // (the others have read this CTA's counts)
+    return;
+  }
   if (gridDim.x > 1) {
     uint32_t *mask = reinterpret_cast<uint32_t *>(after);
     rl_mark(mask, words, ids, pairs, p.k, p.E);
@@ -508,32 +569,44 @@ __global__ void __launch_bounds__(RL_PLACE_THREADS) k_route_place(const __grid_c
   }
   const int32_t *idx = p.idx + (long)t0 * p.k;
   rl_mark(mask, words, idx, tokens * p.k, p.k, p.E);
-  if (threadIdx.x < 32) rl_scan(cnt, off, p.E, threadIdx.x);
-  __syncthreads();
-  const int total = off[p.E];
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    before[e] += off[e];
-    if (blockIdx.x == 0) p.expert_rows[e] = cnt[e];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < tokens * p.k; i += blockDim.x) {
-    const int e = idx[i], j = i / p.k;
-    int slot = -1;
-    if (e >= 0) {
-      slot = before[e] + rl_rank(mask + e * words, words, j);
-      p.row_token[slot] = t0 + j;
-    }
-    p.slot[(long)t0 * p.k + i] = slot;
-  }
-  for (long i = (long)total + blockIdx.x * blockDim.x + threadIdx.x; i < (long)p.T * p.k; i += (long)gridDim.x * blockDim.x) p.row_token[i] = -1;
+  rl_place(p, mask, words, idx, cnt, before, off, t0, tokens * p.k);
 }
 
-template <typename T>
-static int launch_route_typed(const RouteLogitsParams &p, int chunks, int warps, size_t smem, cudaStream_t st) {
+template <typename T, bool CLUSTER>
+static int launch_route_typed(const RouteLogitsParams &p, int ctas, int warps, size_t smem, cudaStream_t st) {
   static ColiPerDeviceOnce attr_once;
-  if (!coli_set_smem_limit(attr_once, k_route_logits<T>, 128 * 32 * 4 + RL_MAX_WARPS * (RL_CAND_BYTES + 512 * 8), "routing shared-memory attribute")) return 0;
+  if (!coli_set_smem_limit(attr_once, k_route_logits<T, CLUSTER>, 128 * 32 * 4 + RL_MAX_WARPS * (RL_CAND_BYTES + 512 * 8), "routing shared-memory attribute"))
+    return 0;
+  if (CLUSTER) {  // 16 CTAs are more than every GPU promises, and fit this one
+    static ColiPerDeviceOnce cluster_once;
+    bool done = false;
+    const int dev = cluster_once.current(&done);
+    if (!done) {
+      if (!coli_cuda_check(cudaFuncSetAttribute(k_route_logits<T, CLUSTER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "routing cluster attribute")) return 0;
+      cluster_once.mark(dev);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)warps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
   coli_count_launch(1);
-  return coli_cuda_check(launch_dependent(k_route_logits<T>, dim3(chunks), dim3(warps * 32), smem, st, p), "routing launch") ? 1 : 0;
+  return coli_cuda_check(cudaLaunchKernelEx(&cfg, k_route_logits<T, CLUSTER>, p), "routing launch") ? 1 : 0;
+}
+template <bool CLUSTER>
+static int launch_route_kernel(const RouteLogitsParams &p, int ctas, int warps, size_t smem, cudaStream_t st) {
+  if (p.type == COLI_TYPE_F32) return launch_route_typed<float, CLUSTER>(p, ctas, warps, smem, st);
+  if (p.type == COLI_TYPE_F16) return launch_route_typed<__half, CLUSTER>(p, ctas, warps, smem, st);
+  return launch_route_typed<__nv_bfloat16, CLUSTER>(p, ctas, warps, smem, st);
 }
 
 int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
@@ -542,13 +615,11 @@ int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
   // a warp per token up to 32; a few more for the tables where there are few tokens
   const int tokens = p.T < p.chunk ? p.T : p.chunk, warps = tokens < 4 ? 4 : tokens < RL_MAX_WARPS ? tokens : RL_MAX_WARPS;
   const size_t pitch = (p.E + 3) & ~3, own = (size_t)warps * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));
-  const size_t marks = (size_t)p.E * words * 4;
-  const size_t smem = (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15) + (own > marks ? own : marks);
-  const size_t tables = marks + (2 * pitch + p.E + 1) * 4;
-  const int ok = p.type == COLI_TYPE_F32   ? launch_route_typed<float>(p, chunks, warps, smem, st)
-                 : p.type == COLI_TYPE_F16 ? launch_route_typed<__half>(p, chunks, warps, smem, st)
-                                           : launch_route_typed<__nv_bfloat16>(p, chunks, warps, smem, st);
-  if (!ok || chunks == 1) return ok;
+  const size_t marks = (size_t)p.E * words * 4, tables = marks + (3 * pitch + p.E + 1) * 4;
+  const size_t smem = (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15) + (own > tables ? own : tables);
+  if (chunks == 1) return launch_route_kernel<false>(p, 1, warps, smem, st);
+  if (chunks <= ROUTE_LOGITS_CLUSTER) return launch_route_kernel<true>(p, chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16, warps, smem, st);
+  if (!launch_route_kernel<false>(p, chunks, warps, smem, st)) return 0;
   coli_count_launch(1);
   return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(RL_PLACE_THREADS), tables, st, p, chunks), "placement launch") ? 1 : 0;
 }

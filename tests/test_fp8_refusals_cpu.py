@@ -99,7 +99,7 @@ def test_experts(fake_cuda, handles):
 
 def test_routing(fake_cuda):
     fake = bind(fake_cuda)
-    good = dict(device=0, z=A, ty=0, stride=64, sb=None, lb=None, T=40, E=64, k=4, score=1, norm=1, scale=1.0, G=8, kept=4, idx=B, w=S, rows=W, slot=Y,
+    good = dict(device=0, z=A, ty=0, stride=64, sb=None, lb=None, T=2000, E=64, k=4, score=1, norm=1, scale=1.0, G=8, kept=4, idx=B, w=S, rows=W, slot=Y,
                 token=at(Y, 4096), work=at(Y, 8192))
 
     def call(**kw):
@@ -108,8 +108,8 @@ def test_routing(fake_cuda):
         return fake.coli_b200_route_logits(*[a[n] for n in ("device", "z", "ty", "stride", "sb", "lb", "T", "E", "k", "score", "norm", "scale", "G", "kept", "idx",
                                                             "w", "rows", "slot", "token", "work")], None), fake.fake_queued()
 
-    assert call() == (1, 1) and call(T=32, work=None) == (1, 1) and call(T=0) == (1, 1) and call(T=1, stride=0) == (1, 1)
-    assert fake.coli_b200_route_logits_workspace(32, 64) == 0 and fake.coli_b200_route_logits_workspace(33, 64) == 128
+    assert call() == (1, 1) and call(T=512, work=None) == (1, 1) and call(T=0) == (1, 1) and call(T=1, stride=0) == (1, 1)
+    assert fake.coli_b200_route_logits_workspace(512, 64) == 0 and fake.coli_b200_route_logits_workspace(513, 66) == 17 * 68
     for bad in (dict(T=-1), dict(E=0), dict(E=513, G=1, kept=1), dict(k=0), dict(k=33), dict(G=1, kept=1, E=3, k=4), dict(ty=5), dict(score=2), dict(G=0),
                 dict(kept=0), dict(kept=9), dict(G=7), dict(G=64, kept=32), dict(G=16, kept=1, k=5), dict(z=None), dict(idx=None), dict(w=None),
                 dict(rows=None), dict(slot=None), dict(token=None), dict(work=None), dict(stride=63), dict(stride=-1), dict(z=at(A, 2)),
