@@ -344,7 +344,7 @@ int coli_b200_fp8_check(int device);
  * For the chosen pairs in expert order (ascending expert, then token): expert_rows_dev [E] pairs of each expert, slot_dev
  * [T,k] the row of each pair or -1, row_token_dev [T*k] the token of each row, -1 behind the last: what
  * coli_b200_quantize_rows_fp8, the expert calls and coli_b200_moe_combine_partial_dev take (with every
- * expert resident).  E <= 512, k <= 32, at most 32 groups.
+ * expert resident).  T <= 2^20, E <= 512, k <= 32, at most 32 groups.
  * workspace_dev: coli_b200_route_logits_workspace(T, E) bytes that no other call in flight uses (NULL where that is 0).
  * The same call gives the same bits.  (The block's own router compares f32 scores, as the reference does,
  * and takes expert 0 where nothing can be chosen.) */

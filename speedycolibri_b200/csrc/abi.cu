@@ -1237,7 +1237,7 @@ extern "C" int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_
   if (!check_fp8_rows("quantize_rows_fp8", codes_dev, ld, scales_dev, s_row, s_blk, rows, K)) return 0;
   OnDevice on(device);
   if (!on.ok) return 0;
-  colib::QuantRowsParams p;
+  colib::QuantRowsParams p = {};
   p.x = x_dev;
   p.type = x_type;
   p.x_stride = (long)x_stride;
@@ -1313,8 +1313,8 @@ extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int ty
                                       int n_group, int topk_group, int32_t *topk_idx_dev, float *topk_w_dev, int32_t *expert_rows_dev,
                                       int32_t *slot_dev, int32_t *row_token_dev, void *workspace_dev, void *stream) {
   const size_t es = type_size(type);
-  if (T < 0 || E < 1 || E > 512 || k < 1 || k > 32 || k > E || es == 0 || (int64_t)T * k > INT32_MAX) {
-    coli_set_error("route_logits: unsupported shape T=%d E=%d k=%d type=%d (E <= 512, k <= min(32, E), T * k below 2^31)", T, E, k, type);
+  if (T < 0 || T > 1 << 20 || E < 1 || E > 512 || k < 1 || k > 32 || k > E || es == 0) {
+    coli_set_error("route_logits: unsupported shape T=%d E=%d k=%d type=%d (T <= 2^20, E <= 512, k <= min(32, E))", T, E, k, type);
     return 0;
   }
   if (score != COLI_SCORE_SOFTMAX && score != COLI_SCORE_SIGMOID) {
@@ -1388,7 +1388,7 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
   const bool few = colib::fp8_stream_ok(p);
   const int blocks = (I + 127) / 128;
   const size_t codes_bytes = (size_t)rows_cap * h_ld, scale_bytes = ((size_t)rows_cap * blocks * 4 + 15) / 16 * 16;
-  const size_t need = codes_bytes + scale_bytes + (few ? (size_t)rows_cap * I * 4 : 0);
+  const size_t need = codes_bytes + scale_bytes + (few ? (size_t)rows_cap * I * 4 + 16 : 0);
   if (!ensure_h(m, m->seg_main, (need + 2 * (size_t)I - 1) / (2 * (size_t)I))) return 0;
   uint8_t *h = (uint8_t *)m->seg_main.h;
   float *hs = (float *)(h + codes_bytes);
@@ -1401,6 +1401,7 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
     return colib::launch_fp8_mm(p, st) && colib::launch_fp8_mm(d, st);
   }
   p.h32 = (float *)(h + codes_bytes + scale_bytes);
+  p.rows_used = (int32_t *)(p.h32 + (size_t)rows_cap * I);
   d.behind_gated = true;
   colib::QuantRowsParams q = {};
   q.x = p.h32;
@@ -1408,6 +1409,7 @@ static int run_segments_fp8(ColiMoe *m, const int32_t *seg_expert_dev, const voi
   q.x_stride = I;
   q.x_vec = true;  // I is a multiple of 8
   q.T = q.rows = rows_cap;
+  q.rows_used = p.rows_used;
   q.K = I;
   q.codes = h;
   q.ld = h_ld;

@@ -80,14 +80,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
   const int lane = threadIdx.x & 31, sub = lane & 7;
   const int c0 = blockIdx.y * QR_COLS + (lane >> 3) * 128 + sub * P::VEC;
   const int step = gridDim.x * 8;
+  const int rows = p.rows_used ? min(p.rows, *p.rows_used) : p.rows;
   // source of a row; outside [0, T): none
-  auto source = [&](long r) { return r < p.rows ? (p.row_token ? __ldg(p.row_token + r) : (int)r) : -1; };
+  auto source = [&](long r) { return r < rows ? (p.row_token ? __ldg(p.row_token + r) : (int)r) : -1; };
   auto valid = [&](int src) { return (unsigned)src < (unsigned)p.T; };
   long r = blockIdx.x * 8 + (threadIdx.x >> 5);
   P now, next;
   int src = source(r), src_next = source(r + step);
   if (valid(src)) qr_request<T>(now, p, src, c0);
-  for (; r < p.rows; r += step) {
+  for (; r < rows; r += step) {
     const int src_after = source(r + 2 * (long)step);
     if (valid(src_next)) qr_request<T>(next, p, src_next, c0);
     if (valid(src)) {  // (no token: the row is left as it was)
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_REGS_OTHER));
     if (warp == F8_EPI_WARPS) {
       // ---------------- copies ----------------
+      asm volatile("fence.proxy.async.global;" ::: "memory");  // (the codes may be an earlier launch's ordinary stores)
       for (int t = cluster0; t < n_tiles; t += clusters) {
         F8Info tile;
         recall(tile);

@@ -11,6 +11,7 @@ struct QuantRowsParams {
   bool x_vec;                // every row starts on 16 bytes
   const int32_t *row_token;  // [rows] source row of each row (outside [0, T): none, the row is left as it was), or null: the row itself
   int T, rows, K;
+  const int32_t *rows_used = nullptr;  // device word: rows from it on are none
   uint8_t *codes;            // [rows, K], rows `ld` bytes apart (a multiple of 16); bytes K .. round_up(K, 16) become zero
   long ld;
   float *scales;             // scale of (row, block) at row * s_row + block * s_blk
@@ -37,6 +38,7 @@ struct Fp8MmParams {
   float *h_scales;           // and scales [ceil(O / 128)][rows]
   long h_ld;
   float *h32;                // segments of a few rows (fp8_stream_ok) instead: h as it is, f32 [rows, O]
+  int32_t *rows_used;        // with h32: device word that receives the rows of all segments
   bool behind_gated;         // segments of a few rows: the launches before this one are the gated call's and the row quantiser's
   ActParams act;
   int *status;               // device word for a bounded wait that gave up, or null: the library's own

@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   if (warp == 0) f8_tables<ROWS>(p, row_off, tile_off, lane);
   __syncthreads();
   const int tasks = tile_off[p.nseg], ks = p.split;
+  if (GATED && blockIdx.x == 0 && threadIdx.x == 0) *p.rows_used = row_off[p.nseg];
   // as many of the warps at work as make the rounds come out even, and the ring shared among those
   const int most = FS_WARPS / ks, rounds = (tasks + (int)gridDim.x * most - 1) / ((int)gridDim.x * most);
   const int groups = rounds > 0 ? min(most, (tasks + (int)gridDim.x * rounds - 1) / ((int)gridDim.x * rounds)) : 0;

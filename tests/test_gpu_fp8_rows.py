@@ -137,12 +137,13 @@ def test_product_at_odd_strides(gpu_backend):
     assert torch.equal(y[:, 7 : 7 + O], want) and (y[:, :7] == 5).all() and (y[:, 7 + O :] == 5).all()
 
 
-def test_nan_and_infinity_reach_their_row_only(gpu_backend):
-    x = rows(5, 256, 9)
+@pytest.mark.parametrize("T", [5, 40, 200])
+def test_nan_and_infinity_reach_their_row_only(gpu_backend, T):
+    x = rows(T, 256, 9)
     x[1, 200], x[3, 4] = torch.nan, -torch.inf
     w, _ = weight(gpu_backend, 300, 256, 10)
     y = gpu_backend.matmul_fp8_dev(w, *gpu_backend.quantize_rows_fp8_dev(x))
-    assert y[[1, 3]].isnan().all() and y[[0, 2, 4]].isfinite().all()
+    assert y[[1, 3]].isnan().all() and y[0].isfinite().all() and y[2].isfinite().all() and y[4:].isfinite().all()
 
 
 def test_no_rows(gpu_backend):
@@ -211,7 +212,7 @@ def test_experts(gpu_backend, E, H, I, counts):
     block.close()
 
 
-@pytest.mark.parametrize("expected", [1, 6, 10000])
+@pytest.mark.parametrize("expected", [0, 1, 6, 10000])
 def test_rows_behind_the_last_segment_stay(gpu_backend, expected):
     counts, H = [2, 0, 4], 256
     block, _ = expert_layer(gpu_backend, 3, H, 128, 300)
@@ -239,4 +240,102 @@ def test_counts_past_the_buffer_are_cut(gpu_backend, counts, expected):
     block.experts_fp8_dev(q, s, torch.tensor(cut, dtype=torch.int32, device="cuda"), expected, want)
     block.check()
     assert torch.equal(y, want) and (y[R - left :] == 3.0).all()
+    block.close()
+
+
+def test_offsets_past_32_bits(gpu_backend):
+    T, K, O = 270000, 8192, 24  # 2.2 GB of codes
+    x = torch.empty((T, K), dtype=torch.bfloat16, device="cuda")
+    x[:1000], x[-1000:] = rows(1000, K, 50), rows(1000, K, 51)
+    x[1000:-1000] = 1.0
+    w, _ = weight(gpu_backend, O, K, 52)
+    q, s = gpu_backend.quantize_rows_fp8_dev(x)
+    y = gpu_backend.matmul_fp8_dev(w, q, s, out_dtype=torch.float32)
+    for cut in (slice(0, 1000), slice(T - 1000, T)):
+        qc, sc = gpu_backend.quantize_rows_fp8_dev(x[cut])
+        assert torch.equal(qc, q[cut]) and torch.equal(sc, s[cut])
+        want = (qc.view(E4M3).double() * spread(sc.double(), K)) @ weight_values(w, O, K).t()
+        assert ((y[cut].double() - want).abs() <= product_bound(qc, sc, weight_values(w, O, K), want, torch.float32)).all()
+
+
+def weight_values(w, O, K):
+    """A handle's values in f64, through its export."""
+    q, s, _ = w.export()
+    return torch.from_numpy(q).cuda().view(E4M3).double() * spread(torch.from_numpy(s).cuda().double(), K).repeat_interleave(128, 0)[:O]
+
+
+@pytest.mark.parametrize("T", [3, 100])
+def test_streams_and_graphs(gpu_backend, T):
+    """Calls on several streams at once, and captured ones replayed on other inputs."""
+    K, O = 700, 600
+    w, _ = weight(gpu_backend, O, K, 60)
+    xs = [rows(T, K, 61 + i).to(torch.bfloat16) for i in range(3)]
+    want = [gpu_backend.matmul_fp8_dev(w, *gpu_backend.quantize_rows_fp8_dev(x)) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], []
+    for x, st in zip(xs, streams):
+        with torch.cuda.stream(st):
+            for _ in range(4):
+                y = gpu_backend.matmul_fp8_dev(w, *gpu_backend.quantize_rows_fp8_dev(x))
+        got.append(y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = xs[0].clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = gpu_backend.matmul_fp8_dev(w, *gpu_backend.quantize_rows_fp8_dev(x))
+    for i in (1, 2, 0):
+        x.copy_(xs[i])
+        g.replay()
+        assert torch.equal(y, want[i])
+    gpu_backend.fp8_check()
+
+
+def test_two_handles_at_once(gpu_backend):
+    """Each handle has its own workspace: their calls may overlap."""
+    H, I, counts = 512, 256, [3, 0, 70, 1]
+    R = sum(counts)
+    made = [expert_layer(gpu_backend, 4, H, I, R, seed=70 + 20 * i) for i in range(2)]
+    seg = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    q, s = gpu_backend.quantize_rows_fp8_dev(rows(R, H, 80))
+    want = [torch.empty((R, H), dtype=torch.bfloat16, device="cuda") for _ in made]
+    for (block, _), y in zip(made, want):
+        block.experts_fp8_dev(q, s, seg, R, y)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    got = [torch.empty_like(y) for y in want]
+    for _ in range(5):
+        for (block, _), y, st in zip(made, got, streams):
+            block.experts_fp8_dev(q, s, seg, R, y, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for block, _ in made:
+        block.check()
+        block.close()
+
+
+def test_refusals(gpu_backend):
+    b, cuda = gpu_backend, "cuda"
+    w, _ = weight(b, 64, 128, 90)
+    q, s = b.quantize_rows_fp8_dev(torch.ones((4, 128), device=cuda))
+    x = torch.ones((4, 128), device=cuda)
+    for bad in (lambda: b.quantize_rows_fp8_dev(x.double()), lambda: b.quantize_rows_fp8_dev(x[0]), lambda: b.quantize_rows_fp8_dev(x.t()),
+                lambda: b.quantize_rows_fp8_dev(x.cpu()), lambda: b.quantize_rows_fp8_dev(x, torch.zeros(4, dtype=torch.int64, device=cuda)),
+                lambda: b.quantize_rows_fp8_dev(x, torch.zeros(4, dtype=torch.int32)), lambda: b.quantize_rows_fp8_dev(x, out=(q[:3], s[:3])),
+                lambda: b.quantize_rows_fp8_dev(x, out=(q, s.double())), lambda: b.quantize_rows_fp8_dev(x, out=(q[:, :64], s)),
+                lambda: b.matmul_fp8_dev(w, q[:, :64], s), lambda: b.matmul_fp8_dev(w, q, s[:3]), lambda: b.matmul_fp8_dev(w, q.cpu(), s),
+                lambda: b.matmul_fp8_dev(w, q, s, out=torch.empty((4, 63), device=cuda)), lambda: b.matmul_fp8_dev(w, q, s, out_dtype=torch.float64),
+                lambda: b.matmul_fp8_dev(w, q, s, out=torch.empty((64, 4), device=cuda).t()),
+                lambda: b.matmul_fp8_dev(w, q, s, out_dtype=torch.float16, out=torch.empty((4, 64), device=cuda))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(b.CudaError):  # rows of codes off the 16-byte grid
+        b.matmul_fp8_dev(w, torch.zeros((4, 150), dtype=torch.uint8, device=cuda)[:, :128], s)
+    block, _ = expert_layer(b, 2, 128, 64, 4)
+    y, seg = torch.empty((4, 128), dtype=torch.bfloat16, device=cuda), torch.tensor([2, 2], dtype=torch.int32, device=cuda)
+    for bad in (lambda: block.experts_fp8_dev(q, s, seg, 4, y.float()), lambda: block.experts_fp8_dev(q, s, seg[:1], 4, y),
+                lambda: block.experts_fp8_dev(q, s, seg.long(), 4, y), lambda: block.experts_fp8_dev(q, s, seg.cpu(), 4, y),
+                lambda: block.experts_fp8_dev(q, s, seg, 4, y[:3])):
+        with pytest.raises(ValueError):
+            bad()
     block.close()

@@ -174,3 +174,17 @@ def test_calls_on_two_streams_and_in_graphs(gpu_backend):
     torch.cuda.synchronize()
     for r, w in zip(outs, want):
         assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+def test_refusals(gpu_backend):
+    z = torch.zeros((4, 16), device="cuda")
+    out = gpu_backend.route_logits_dev(z, 2)
+    for bad in (lambda: gpu_backend.route_logits_dev(z.double(), 2), lambda: gpu_backend.route_logits_dev(z[0], 2), lambda: gpu_backend.route_logits_dev(z.cpu(), 2),
+                lambda: gpu_backend.route_logits_dev(z.t(), 2), lambda: gpu_backend.route_logits_dev(z, 2, select_bias=torch.zeros(15, device="cuda")),
+                lambda: gpu_backend.route_logits_dev(z, 2, logit_bias=torch.zeros(16)), lambda: gpu_backend.route_logits_dev(z, 3, out=out),
+                lambda: gpu_backend.route_logits_dev(z, 2, out=out._replace(w=out.idx))):
+        with pytest.raises(ValueError):
+            bad()
+    for kw in (dict(k=17), dict(k=0), dict(k=2, score=5), dict(k=2, n_group=3), dict(k=9, n_group=4, topk_group=2)):
+        with pytest.raises(gpu_backend.CudaError):
+            gpu_backend.route_logits_dev(z, **kw)
