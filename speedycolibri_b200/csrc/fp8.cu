@@ -162,6 +162,7 @@ constexpr int F8_EPI_WARPS = 8;
 constexpr int F8_THREADS = (F8_EPI_WARPS + 4) * 32;  // (two warps stand by: registers are moved between whole warpgroups)
 // 168 registers a thread at launch are 64512; the summing warps take 208 of them each, the others keep 88: all of them.
 constexpr int F8_REGS_SUM = 208, F8_REGS_OTHER = 88;
+constexpr int F8_MAX_SPLIT = 4;  // CTAs that share a tile's k-tiles (clusters of 8 start late: 24 rows x 2048 x 2048 11.4 us, with 4 6.5)
 constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
 struct F8Maps {
   CUtensorMap m[F8_MAPS];
@@ -289,19 +290,25 @@ __device__ __forceinline__ void f8_add_scaled(float2 &c, float x, float y, float
 // One warp sums row i of the tile over the CTAs of the cluster and writes what becomes of it.
 template <bool GATED, int BN, typename OutT>
 __device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &tile, uint32_t red, int world, int i, int lane) {
-  float4 v[BN / 128];
+  // (all CTAs' sums are requested before the first is added)
+  float4 v[BN / 128], u[F8_MAX_SPLIT][BN / 128];
 #pragma unroll
-  for (int j = 0; j < BN / 128; ++j) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int r = 0; r < world; ++r) {
+  for (int r = 0; r < F8_MAX_SPLIT; ++r)
 #pragma unroll
-    for (int j = 0; j < BN / 128; ++j) {
-      const float4 u = ld_cluster4(red + (uint32_t)(i * (BN + 4) + 128 * j + 4 * lane) * 4u, (uint32_t)r);
-      v[j].x += u.x;
-      v[j].y += u.y;
-      v[j].z += u.z;
-      v[j].w += u.w;
-    }
-  }
+    for (int j = 0; j < BN / 128; ++j)
+      if (r < world) u[r][j] = ld_cluster4(red + (uint32_t)(i * (BN + 4) + 128 * j + 4 * lane) * 4u, (uint32_t)r);
+#pragma unroll
+  for (int j = 0; j < BN / 128; ++j) v[j] = u[0][j];
+#pragma unroll
+  for (int r = 1; r < F8_MAX_SPLIT; ++r)
+#pragma unroll
+    for (int j = 0; j < BN / 128; ++j)
+      if (r < world) {
+        v[j].x += u[r][j].x;
+        v[j].y += u[r][j].y;
+        v[j].z += u[r][j].z;
+        v[j].w += u[r][j].w;
+      }
   if constexpr (GATED) {
     const int f = tile.nt * 128 + 4 * lane;
     const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
@@ -727,8 +734,11 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   // Rows of a tile, row tiles the call is likely to have, and the most it can have.  All are functions of the call's shapes alone.
   const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
   const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
-  int ar = mean <= (p.seg_count ? 40 : 64) ? 64 : 128;
-  if (mean <= (p.seg_count ? 16 : 32)) ar = 32;
+  // 128 rows where segments are long and their tiles fill the SMs (with 64 rows, us a call: 100 rows x 2048 x 2048 14.7 -> 7.6, 200 x
+  // 4096 x 1024 15.5 -> 9.1; 4096 rows on 128 experts, H 2048, I 768, 158 -> 127)
+  const long full = ((mean + 127) / 128) * (segs > 0 ? segs : 1) * ((p.O + 127) / 128);
+  int ar = mean <= (p.seg_count ? 40 : 64) || full <= COLI_SMS ? 64 : 128;
+  if (mean <= (p.seg_count ? 20 : 32)) ar = 32;  // (64-row tiles: 600 rows on 32 experts, H 2048, I 768, 49.6 us, with 32 rows 46.0)
   const int most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + ar - 1) / ar;
   const int likely = p.seg_count ? p.rows_expected / ar + segs : most;
   int bn = 256;
@@ -737,7 +747,7 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   p.n_tiles = (p.O + fw - 1) / fw;
   const long tiles = (long)(likely > 0 ? likely : 1) * p.n_tiles;
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= COLI_SMS && p.split * 2 <= p.KT) p.split *= 2;
+  while (p.split < F8_MAX_SPLIT && tiles * p.split * 2 <= COLI_SMS && p.split * 2 <= p.KT) p.split *= 2;
   F8Maps maps;
   // One segment has full boxes and a last one; behind counts on the device any may come (an encoding takes 0.3 us).
   auto box_of = [](int n) {
