@@ -45,11 +45,14 @@ struct Fp8MmParams {
   // filled in by the launcher
   int KT, Op, n_tiles, split;
 };
-// Whether segments are short enough for the streaming kernel (fp8_stream.cu).  A function of shapes alone.
+// Whether segments are short enough for the streaming kernel (fp8_stream.cu), a task of which takes up to 8 rows.  One segment up to
+// 8 rows (streaming / tcgen05, us a call: 8 rows x 2048 x 2048 4.5 / 5.9, x 7168 x 4096 8.9 / 9.9); experts while
+// segments have two rows on average (H 4096, I 1024, 32 experts: 32 rows 53 / 67, 128 rows 100 / 78; H 2048, I 768, 128 experts: 300
+// rows 109 / 104, 512 rows 153 / 114).  A function of shapes alone.
 static inline bool fp8_stream_ok(const Fp8MmParams &p) {
-  if (!p.seg_count) return p.rows <= 16;
+  if (!p.seg_count) return p.rows <= 8;
   const int segs = p.rows_expected < p.nseg ? p.rows_expected : p.nseg;
-  return p.rows_expected <= 6L * segs;
+  return p.rows_expected <= 2L * segs;
 }
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st);
 int launch_fp8_stream(Fp8MmParams p, cudaStream_t st);  // called by launch_fp8_mm

@@ -19,11 +19,13 @@ namespace colib {
 constexpr int FS_WARPS = 16;
 constexpr int FS_THREADS = FS_WARPS * 32;
 
-template <int M, int NT>
+constexpr int FS_ROWS = 8;  // of a task
+
+template <int M>
 struct FsSmem {
-  static constexpr int ROWS = M * 2048, SCALES = ROWS + NT * 1024;  // a slot: slabs, rows' codes, scales (sx, then sw)
+  static constexpr int ROWS = M * 2048, SCALES = ROWS + FS_ROWS * 128;  // a slot: slabs, rows' codes, scales (sx, then sw)
   static constexpr int UNIT = SCALES + 128;
-  static constexpr int RED = FS_WARPS * M * NT * 512;  // partial sums of warps that share a task
+  static constexpr int RED = FS_WARPS * M * 512;  // partial sums of warps that share a task
   static constexpr int RING = (218 * 1024 - RED) / UNIT * UNIT;
   static constexpr int SLOTS = RING / UNIT;
   static constexpr int TABLES = 2 * (F8_MAX_SEGS + 1) * 4;
@@ -50,11 +52,10 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// GATED: units hold a slab of gate and one of up.  M: slabs of a unit.  NT: groups of 8 rows.
-template <bool GATED, int M, int NT, typename OutT>
+// GATED: units hold a slab of gate and one of up.  M: slabs of a unit.
+template <bool GATED, int M, typename OutT>
 __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_constant__ Fp8MmParams p) {
-  using S = FsSmem<M, NT>;
-  constexpr int ROWS = 8 * NT;
+  using S = FsSmem<M>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
   float *red = reinterpret_cast<float *>(smem + S::RING);
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   // Behind the gated call and the quantiser the counts are complete: the gated call lets its successor start after its own wait.
   const bool early = !p.seg_count || p.behind_gated;
   if (!early) coli_grid_wait();
-  if (warp == 0) f8_tables<ROWS>(p, row_off, tile_off, lane);
+  if (warp == 0) f8_tables<FS_ROWS>(p, row_off, tile_off, lane);
   __syncthreads();
   const int tasks = tile_off[p.nseg], ks = p.split;
   if (GATED && blockIdx.x == 0 && threadIdx.x == 0) *p.rows_used = row_off[p.nseg];
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   // the copies: unit u is k-tile kt0 + u % per_task of the warp's task u / per_task
   int issued = 0, i_task = first, i_kt = kt0, i_slot = 0, i_rows = 0;
   const uint8_t *q0 = nullptr, *q1 = nullptr, *codes = nullptr;
-  const float *scale = nullptr;  // lanes 0 .. ROWS - 1: their row's; the next two: the weights'
+  const float *scale = nullptr;  // lanes 0 .. 7: their row's; the next two: the weights'
   bool both = true, alive = true;
   // where a task's operands are, looked up a task ahead (the expert's index and its table entry are two reads in a row)
   struct Task {
@@ -104,20 +105,20 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   } ahead_task = {};
   auto look_up = [&](int task) {
     if (task >= tasks) return;
-    const F8Tile tile = f8_tile<ROWS>(tile_off, row_off, p.nseg, task);
+    const F8Tile tile = f8_tile<FS_ROWS>(tile_off, row_off, p.nseg, task);
     const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
     const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
     const int f0 = tile.nt * (GATED ? 16 : 16 * M);
     ahead_task.q0 = w0.q + (size_t)f0 * 128;
     ahead_task.q1 = w1.q + (size_t)f0 * 128;
-    ahead_task.scale = lane < ROWS ? p.sx + (long)(tile.row0 + min(lane, tile.nrows - 1)) * p.s_row
-                                   : reinterpret_cast<const float *>(lane == ROWS ? w0.s : w1.s) + (size_t)(f0 >> 7) * p.KT;
+    ahead_task.scale = lane < FS_ROWS ? p.sx + (long)(tile.row0 + min(lane, tile.nrows - 1)) * p.s_row
+                                   : reinterpret_cast<const float *>(lane == FS_ROWS ? w0.s : w1.s) + (size_t)(f0 >> 7) * p.KT;
     ahead_task.row0 = tile.row0;
     ahead_task.nrows = tile.nrows;
     ahead_task.both = f0 + 16 * M <= p.Op;
   };
   if (works) look_up(first);
-  const long scale_step = lane < ROWS ? p.s_blk : 1;
+  const long scale_step = lane < FS_ROWS ? p.s_blk : 1;
   auto issue_weights = [&]() {
     if (i_kt == kt0) {
       q0 = ahead_task.q0 + lane * 16;
@@ -142,11 +143,11 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
     const uint32_t dst = ring + (uint32_t)i_slot * S::UNIT, c0 = (uint32_t)(lane & 7);
     const int left = p.K - i_kt * 128 - (lane & 7) * 16;
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {  // rows 4 i + lane / 8; a missing row and columns past K are zeros
+    for (int i = 0; i < FS_ROWS / 4; ++i) {  // rows 4 i + lane / 8; a missing row and columns past K are zeros
       const int r = 4 * i + (lane >> 3), n = r < i_rows ? max(0, min(16, left)) : 0;
       cp_async_part(dst + S::ROWS + (uint32_t)r * 128 + ((c0 ^ (uint32_t)(r & 7)) << 4), n ? codes + 4 * i * p.ld + (long)i_kt * 128 : codes, n);
     }
-    if (lane < ROWS + 2) cp_async_word(dst + S::SCALES + (uint32_t)lane * 4, scale + (long)i_kt * scale_step, 4);
+    if (lane < FS_ROWS + 2) cp_async_word(dst + S::SCALES + (uint32_t)lane * 4, scale + (long)i_kt * scale_step, 4);
     // the lane's copies count once they have landed
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar + 8u * (uint32_t)i_slot) : "memory");
     if (++i_slot == depth) i_slot = 0;
@@ -177,38 +178,28 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
   int used = 0, slot = 0;
   uint32_t phase = 0;
   for (int task = first; works && task < tasks; task += stride) {
-    const F8Tile tile = f8_tile<ROWS>(tile_off, row_off, p.nseg, task);
+    const F8Tile tile = f8_tile<FS_ROWS>(tile_off, row_off, p.nseg, task);
     const int f0 = tile.nt * (GATED ? 16 : 16 * M);
-    float acc[M][NT][4] = {};
+    float acc[M][4] = {};
     for (int kt = kt0; kt < kt1; ++kt, ++used) {
       alive = alive && __all_sync(0xffffffffu, mbar_wait(bar + 8u * (uint32_t)slot, phase, abort_flag, status, TC_ERR_TMA_WAIT));
       const uint32_t unit = ring + (uint32_t)slot * S::UNIT, c0 = (uint32_t)(t ^ g) * 16, c1 = (uint32_t)((t + 4) ^ g) * 16;
-      uint4 lo[NT], hi[NT];
-      float sx[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint32_t r = unit + S::ROWS + (uint32_t)(8 * n + g) * 128;
-        lo[n] = lds128(r + c0);
-        hi[n] = lds128(r + c1);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) sx[n][i] = lds32(unit + S::SCALES + (uint32_t)(8 * n + 2 * t + i) * 4);
-      }
-      const float s0 = lds32(unit + S::SCALES + ROWS * 4), s1 = GATED ? lds32(unit + S::SCALES + ROWS * 4 + 4) : s0;
+      const uint32_t r = unit + S::ROWS + (uint32_t)g * 128;
+      const uint4 lo = lds128(r + c0), hi = lds128(r + c1);
+      const float sx[2] = {lds32(unit + S::SCALES + (uint32_t)t * 8), lds32(unit + S::SCALES + (uint32_t)t * 8 + 4)};
+      const float s0 = lds32(unit + S::SCALES + FS_ROWS * 4), s1 = GATED ? lds32(unit + S::SCALES + FS_ROWS * 4 + 4) : s0;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const uint32_t at = unit + (uint32_t)g * 128 + m * 2048;
         const uint4 a0 = lds128(at + c0), a1 = lds128(at + 1024 + c0), a2 = lds128(at + c1), a3 = lds128(at + 1024 + c1);
         const float sw = m == 0 || !GATED ? s0 : s1;
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_e4m3(d, a0.x, a1.x, a2.x, a3.x, lo.x, hi.x);
+        mma_e4m3(d, a0.y, a1.y, a2.y, a3.y, lo.y, hi.y);
+        mma_e4m3(d, a0.z, a1.z, a2.z, a3.z, lo.z, hi.z);
+        mma_e4m3(d, a0.w, a1.w, a2.w, a3.w, lo.w, hi.w);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_e4m3(d, a0.x, a1.x, a2.x, a3.x, lo[n].x, hi[n].x);
-          mma_e4m3(d, a0.y, a1.y, a2.y, a3.y, lo[n].y, hi[n].y);
-          mma_e4m3(d, a0.z, a1.z, a2.z, a3.z, lo[n].z, hi[n].z);
-          mma_e4m3(d, a0.w, a1.w, a2.w, a3.w, lo[n].w, hi[n].w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(d[i], sx[n][i & 1] * sw, acc[m][n][i]);
-        }
+        for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(d[i], sx[i & 1] * sw, acc[m][i]);
       }
       if (++slot == depth) {
         slot = 0;
@@ -219,77 +210,72 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
     }
     if (ks > 1) {
       // join the sums of the warps that share the task, in their order
-      constexpr int N = M * NT * 4;
+      constexpr int N = M * 4;
       float *mine = red + (size_t)warp * N * 32;
 #pragma unroll
-      for (int i = 0; i < N; ++i) mine[i * 32 + lane] = acc[i / (4 * NT)][i / 4 % NT][i % 4];
+      for (int i = 0; i < N; ++i) mine[i * 32 + lane] = acc[i / 4][i % 4];
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(ks * 32) : "memory");
       if (sub == 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           float s = mine[i * 32 + lane];
           for (int w = 1; w < ks; ++w) s += mine[(size_t)w * N * 32 + i * 32 + lane];
-          acc[i / (4 * NT)][i / 4 % NT][i % 4] = s;
+          acc[i / 4][i % 4] = s;
         }
       }
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(ks * 32) : "memory");
     }
     if (sub == 0 && alive) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < 4; ++i) {
+        const int r = 2 * t + (i & 1);
+        if (r >= tile.nrows) continue;
+        if constexpr (GATED) {
+          const int f = f0 + g + 8 * (i >> 1);
+          if (f < p.O) p.h32[(long)(tile.row0 + r) * p.O + f] = coli_act_fast(acc[0][i], acc[1][i], p.act);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * n + 2 * t + (i & 1);
-          if (r >= tile.nrows) continue;
-          if constexpr (GATED) {
-            const int f = f0 + g + 8 * (i >> 1);
-            if (f < p.O) p.h32[(long)(tile.row0 + r) * p.O + f] = coli_act_fast(acc[0][n][i], acc[1][n][i], p.act);
-          } else {
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-              const int f = f0 + 16 * m + g + 8 * (i >> 1);
-              if (f < p.O) ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f] = f8_out<OutT>(acc[m][n][i]);
-            }
+          for (int m = 0; m < M; ++m) {
+            const int f = f0 + 16 * m + g + 8 * (i >> 1);
+            if (f < p.O) ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f] = f8_out<OutT>(acc[m][i]);
           }
         }
+      }
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");  // (none are left unless a wait gave up)
 }
 
-template <bool GATED, int M, int NT, typename OutT>
+template <bool GATED, int M, typename OutT>
 static int launch_fs(const Fp8MmParams &p, int grid, cudaStream_t st) {
   static ColiPerDeviceOnce attr_once;
-  auto *kernel = k_fp8_stream<GATED, M, NT, OutT>;
-  constexpr int bytes = FsSmem<M, NT>::BYTES;
+  auto *kernel = k_fp8_stream<GATED, M, OutT>;
+  constexpr int bytes = FsSmem<M>::BYTES;
   if (!coli_set_smem_limit(attr_once, kernel, bytes, "fp8 stream shared-memory attribute")) return 0;
   coli_count_launch(1);
   return coli_cuda_check(launch_dependent(kernel, dim3((unsigned)grid), dim3(FS_THREADS), bytes, st, p), "fp8 stream launch") ? 1 : 0;
 }
 template <typename OutT>
-static int launch_fs_shape(const Fp8MmParams &p, int m, int nt, int grid, cudaStream_t st) {
-  if (m == 2) return nt == 1 ? launch_fs<false, 2, 1, OutT>(p, grid, st) : launch_fs<false, 2, 2, OutT>(p, grid, st);
-  return nt == 1 ? launch_fs<false, 1, 1, OutT>(p, grid, st) : launch_fs<false, 1, 2, OutT>(p, grid, st);
+static int launch_fs_slabs(const Fp8MmParams &p, int m, int grid, cudaStream_t st) {
+  return m == 2 ? launch_fs<false, 2, OutT>(p, grid, st) : launch_fs<false, 1, OutT>(p, grid, st);
 }
 
 int launch_fp8_stream(Fp8MmParams p, cudaStream_t st) {
   const bool gated = p.w1 != nullptr;
   const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
-  // rows of a task: 8, or 16 where many segments have more than 8
-  const int nt = p.rows_expected <= (p.seg_count ? 3L : 8L) * segs ? 1 : 2, rows = 8 * nt;
-  const long chunks = p.seg_count ? segs + p.rows_expected / rows : (p.rows + rows - 1) / rows;
+  const long chunks = p.seg_count ? segs + p.rows_expected / FS_ROWS : 1;
   // two slabs a unit where that still leaves every warp a task
   const int m = gated || chunks * ((p.O + 31) / 32) >= (long)COLI_SMS * FS_WARPS ? 2 : 1;
   p.n_tiles = (p.O + (gated ? 16 : 16 * m) - 1) / (gated ? 16 : 16 * m);
   const long tasks = (chunks > 0 ? chunks : 1) * p.n_tiles;
   p.split = 1;
   while (p.split < FS_WARPS && tasks * p.split * 2 <= (long)COLI_SMS * FS_WARPS && p.split * 2 <= p.KT) p.split *= 2;
-  const long most = p.seg_count ? (p.rows / rows + (p.rows < p.nseg ? p.rows : p.nseg)) * (long)p.n_tiles : tasks;
+  const long most = p.seg_count ? (p.rows / FS_ROWS + (p.rows < p.nseg ? p.rows : p.nseg)) * (long)p.n_tiles : tasks;
   const int grid = (int)(most < COLI_SMS ? most : COLI_SMS);
-  if (gated) return nt == 1 ? launch_fs<true, 2, 1, float>(p, grid, st) : launch_fs<true, 2, 2, float>(p, grid, st);
-  if (p.y_type == COLI_TYPE_F32) return launch_fs_shape<float>(p, m, nt, grid, st);
-  if (p.y_type == COLI_TYPE_F16) return launch_fs_shape<__half>(p, m, nt, grid, st);
-  return launch_fs_shape<__nv_bfloat16>(p, m, nt, grid, st);
+  if (gated) return launch_fs<true, 2, float>(p, grid, st);
+  if (p.y_type == COLI_TYPE_F32) return launch_fs_slabs<float>(p, m, grid, st);
+  if (p.y_type == COLI_TYPE_F16) return launch_fs_slabs<__half>(p, m, grid, st);
+  return launch_fs_slabs<__nv_bfloat16>(p, m, grid, st);
 }
 
 }  // namespace colib
