@@ -16,24 +16,27 @@ namespace colib {
 //   a = largest |x| of a block's non-NaN values, s = 1 if a == 0 else max(a / 448, 2^-126), code = e4m3(x / s)
 // to nearest even, saturating; a NaN keeps a NaN code, and an infinity makes s infinite and its own code NaN, so
 // that either shows in every product with the row.
-// Eight lanes share a block, 16 columns each in pieces of 16 bytes; a warp takes QR_STEPS times four blocks of a row and
-// goes through the rows with the next one's pieces already requested; the warps of a CTA take neighbouring rows, whose
-// scales of a block lie side by side.
-constexpr int QR_STEPS = 2, QR_COLS = QR_STEPS * 512;
-template <typename T>
+// LANES lanes share a block, in pieces of 16 bytes; a warp takes QR_COLS columns of a row and goes through the rows with the next
+// one's pieces already requested; the warps of a CTA take neighbouring rows, whose scales of a block lie side by side.  Four lanes
+// halve what a block's scale costs (32768 gathered rows of 7168 bf16 99.7 -> 90.4 us, with eight lanes and two quotients an
+// instruction; rows as they are 112 -> 108.5, 6.5 TB/s); values read one by one, off the 16-byte grid, and f32, whose codes would be
+// stored half a sector at a time, keep eight (5000 rows of 1111 f16 11.0 us, with four 16.4).
+constexpr int QR_COLS = 1024;
+template <typename T, int LANES>
 struct QrPieces {
-  static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 16 / VEC;
-  uint4 q[QR_STEPS][LOADS];
+  static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 128 / LANES / VEC, COLS = 32 / LANES * 128, STEPS = QR_COLS / COLS;
+  uint4 q[STEPS][LOADS];
 };
-template <typename T>
-__device__ __forceinline__ void qr_request(QrPieces<T> &d, const QuantRowsParams &p, int src, int c0) {
-  constexpr int VEC = QrPieces<T>::VEC;
+template <typename T, int LANES>
+__device__ __forceinline__ void qr_request(QrPieces<T, LANES> &d, const QuantRowsParams &p, int src, int c0) {
+  using P = QrPieces<T, LANES>;
+  constexpr int VEC = P::VEC, STEPS = P::STEPS, COLS = P::COLS;
   const T *x = (const T *)p.x + (long)src * p.x_stride;
 #pragma unroll
-  for (int j = 0; j < QR_STEPS; ++j)
+  for (int j = 0; j < STEPS; ++j)
 #pragma unroll
-    for (int l = 0; l < QrPieces<T>::LOADS; ++l) {
-      const int c = c0 + 512 * j + 8 * VEC * l;
+    for (int l = 0; l < P::LOADS; ++l) {
+      const int c = c0 + COLS * j + LANES * VEC * l;
       if (p.x_vec && c + VEC <= p.K) {
         d.q[j][l] = __ldg(reinterpret_cast<const uint4 *>(x + c));
       } else {
@@ -72,13 +75,14 @@ struct QrMax<__nv_bfloat16> {
   using type = __nv_bfloat162;
 };
 
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(QuantRowsParams p) {
-  using P = QrPieces<T>;
+  using P = QrPieces<T, LANES>;
+  constexpr int STEPS = P::STEPS, COLS = P::COLS;
   coli_grid_dependency_sync();
   const int kp = (p.K + 15) & ~15;
-  const int lane = threadIdx.x & 31, sub = lane & 7;
-  const int c0 = blockIdx.y * QR_COLS + (lane >> 3) * 128 + sub * P::VEC;
+  const int lane = threadIdx.x & 31, sub = lane % LANES;
+  const int c0 = blockIdx.y * QR_COLS + lane / LANES * 128 + sub * P::VEC;
   const int step = gridDim.x * 8;
   const int rows = p.rows_used ? min(p.rows, *p.rows_used) : p.rows;
   // source of a row; outside [0, T): none
@@ -87,38 +91,39 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
   long r = blockIdx.x * 8 + (threadIdx.x >> 5);
   P now, next;
   int src = source(r), src_next = source(r + step);
-  if (valid(src)) qr_request<T>(now, p, src, c0);
+  if (valid(src)) qr_request<T, LANES>(now, p, src, c0);
   for (; r < rows; r += step) {
     const int src_after = source(r + 2 * (long)step);
-    if (valid(src_next)) qr_request<T>(next, p, src_next, c0);
+    if (valid(src_next)) qr_request<T, LANES>(next, p, src_next, c0);
     if (valid(src)) {  // (no token: the row is left as it was)
 #pragma unroll
-      for (int j = 0; j < QR_STEPS; ++j) {
+      for (int j = 0; j < STEPS; ++j) {
         typename QrMax<T>::type m;
         qr_zero(m);
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) m = qr_amax(qr_amax(qr_amax(qr_amax(m, now.q[j][l].x, T()), now.q[j][l].y, T()), now.q[j][l].z, T()), now.q[j][l].w, T());
         float a = qr_amax_out(m);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
         const float s = row_scale(a), y = __frcp_rn(s);
         const float b = s <= 3.4028235e38f ? s : 0.0f;  // (x times the reciprocal of an infinite s as it is)
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) {
-          const int c = c0 + 512 * j + 8 * P::VEC * l;
+          const int c = c0 + COLS * j + LANES * P::VEC * l;
           const uint4 q = now.q[j][l];
           uint8_t *dst = p.codes + (size_t)r * p.ld + c;
           if constexpr (sizeof(T) == 4) {
-            const uint32_t w = e4m3x4(quotients(make_float2(__uint_as_float(q.x), __uint_as_float(q.y)), b, y),
-                                      quotients(make_float2(__uint_as_float(q.z), __uint_as_float(q.w)), b, y));
+            const uint32_t w = e4m3x4(quotient(__uint_as_float(q.x), b, y), quotient(__uint_as_float(q.y), b, y),
+                                      quotient(__uint_as_float(q.z), b, y), quotient(__uint_as_float(q.w), b, y));
             if (c < kp) *reinterpret_cast<uint32_t *>(dst) = w;
           } else {
-            const uint2 w = make_uint2(e4m3x4(quotients(qr_pair(q.x, T()), b, y), quotients(qr_pair(q.y, T()), b, y)),
-                                       e4m3x4(quotients(qr_pair(q.z, T()), b, y), quotients(qr_pair(q.w, T()), b, y)));
+            const float2 v0 = qr_pair(q.x, T()), v1 = qr_pair(q.y, T()), v2 = qr_pair(q.z, T()), v3 = qr_pair(q.w, T());
+            const uint2 w = make_uint2(e4m3x4(quotient(v0.x, b, y), quotient(v0.y, b, y), quotient(v1.x, b, y), quotient(v1.y, b, y)),
+                                       e4m3x4(quotient(v2.x, b, y), quotient(v2.y, b, y), quotient(v3.x, b, y), quotient(v3.y, b, y)));
             if (c < kp) *reinterpret_cast<uint2 *>(dst) = w;
           }
         }
-        const int block = (c0 + 512 * j) >> 7;
+        const int block = (c0 + COLS * j) >> 7;
         if (sub == 0 && block * 128 < p.K) p.scales[r * p.s_row + (long)block * p.s_blk] = s;
       }
     }
@@ -142,11 +147,11 @@ int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
   coli_count_launch(1);
   cudaError_t e;
   if (p.type == COLI_TYPE_F32)
-    e = launch_dependent(k_quant_rows<float>, grid, dim3(256), 0, st, p);
+    e = launch_dependent(k_quant_rows<float, 8>, grid, dim3(256), 0, st, p);
   else if (p.type == COLI_TYPE_F16)
-    e = launch_dependent(k_quant_rows<__half>, grid, dim3(256), 0, st, p);
+    e = launch_dependent(p.x_vec ? k_quant_rows<__half, 4> : k_quant_rows<__half, 8>, grid, dim3(256), 0, st, p);
   else
-    e = launch_dependent(k_quant_rows<__nv_bfloat16>, grid, dim3(256), 0, st, p);
+    e = launch_dependent(p.x_vec ? k_quant_rows<__nv_bfloat16, 4> : k_quant_rows<__nv_bfloat16, 8>, grid, dim3(256), 0, st, p);
   return coli_cuda_check(e, "row quantiser launch") ? 1 : 0;
 }
 

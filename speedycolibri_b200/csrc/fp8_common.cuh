@@ -14,19 +14,6 @@ __device__ __forceinline__ float quotient(float a, float b, float y) {
   const float q = a * y;
   return fmaf(fmaf(-q, b, a), y, q);
 }
-// two quotients by the same b at once
-__device__ __forceinline__ float2 quotients(float2 a, float b, float y) {
-  uint64_t q, r, a2, nb, y2;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(a2) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(nb) : "f"(-b));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(y2) : "f"(y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(a2), "l"(y2));
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(nb), "l"(a2));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(r), "l"(y2));
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(q));
-  return d;
-}
 __device__ __forceinline__ float row_scale(float a) {
   constexpr float TINY = 1.17549435e-38f;              // 2^-126
   const float s = fmaxf(quotient(a, 448.0f, 1.0f / 448.0f), TINY);
@@ -40,7 +27,6 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return d;
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
-__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) { return e4m3x4(a.x, a.y, b.x, b.y); }
 
 // `bytes` (a multiple of 16) in a row, global -> shared memory, counted by the barrier
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
