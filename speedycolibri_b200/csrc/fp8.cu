@@ -739,10 +739,11 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   // Rows of a tile, row tiles the call is likely to have, and the most it can have.  All are functions of the call's shapes alone.
   const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
   const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
-  // 128 rows where segments are long and their tiles fill the SMs (with 64 rows, us a call: 100 rows x 2048 x 2048 14.7 -> 7.6, 200 x
-  // 4096 x 1024 15.5 -> 9.1; 4096 rows on 128 experts, H 2048, I 768, 158 -> 127)
+  // 128 rows where segments are long and their tiles fill the SMs.  Us a call, 128 / 64 rows: one segment of 100 rows x 2048 x 2048
+  // 14.7 / 7.6, of 200 x 4096 x 1024 15.5 / 9.1; experts of H 7168, I 2048, 32 of them, 53 rows each 274 / 249, 64 rows 279 / 312
+  // (their weights pass twice for a segment of more than 64); H 2048, I 768, 64 experts, 64 rows 100 / 82, 94 rows 103 / 103.
   const long full = ((mean + 127) / 128) * (segs > 0 ? segs : 1) * ((p.O + 127) / 128);
-  int ar = mean <= (p.seg_count ? 40 : 64) || full <= COLI_SMS ? 64 : 128;
+  int ar = mean <= (p.seg_count && p.KT > 32 ? 56 : 64) || full <= COLI_SMS ? 64 : 128;
   if (mean <= (p.seg_count ? 20 : 32)) ar = 32;  // (64-row tiles: 600 rows on 32 experts, H 2048, I 768, 49.6 us, with 32 rows 46.0)
   const int most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + ar - 1) / ar;
   const int likely = p.seg_count ? p.rows_expected / ar + segs : most;
