@@ -261,22 +261,19 @@ __device__ __forceinline__ void f8_store_rows(unsigned char *stage, OutT *y, lon
       *reinterpret_cast<uint4 *>(stage + lane * LD + 16 * i) = *reinterpret_cast<const uint4 *>(o);
     }
     __syncwarp();
-    const int col = c * CH + (lane & 3) * PER;
+    if (vec && (c + 1) * CH <= cols) {
+      const int col = c * CH + (lane & 3) * PER;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      const uint4 v = lds128(at + (uint32_t)(r * LD + 16 * (lane & 3)));
-      if (r < rows) {
-        OutT *dst = y + (long)r * stride + col;
-        if (vec && col + PER <= cols) {
-          *reinterpret_cast<uint4 *>(dst) = v;
-        } else {
-          const OutT *o = reinterpret_cast<const OutT *>(&v);
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (col + j < cols) dst[j] = o[j];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        const uint4 v = lds128(at + (uint32_t)(r * LD + 16 * (lane & 3)));
+        if (r < rows) *reinterpret_cast<uint4 *>(y + (long)r * stride + col) = v;
       }
+    } else {  // off the 16-byte grid, or the last features: value by value, a row's next to each other
+      const int e = lane % CH, col = c * CH + e;
+#pragma unroll 8
+      for (int r = lane / CH; r < 32; r += 32 / CH)
+        if (r < rows && col < cols) y[(long)r * stride + col] = *reinterpret_cast<const OutT *>(stage + r * LD + e * (int)sizeof(OutT));
     }
     __syncwarp();
   }
@@ -725,6 +722,13 @@ static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int
   return launch_f8_rows<GATED, 256, OutT>(maps, p, ar, grid, st);
 }
 
+// Us a k-tile, for the ends of a tile, and for joining the sums of CTAs that share one: fitted to K 512 to 7168 on 64 to 148 CTAs.
+struct F8Shape {
+  int ar, bn;
+  double kt_us, end_us, join_us;
+};
+static const F8Shape F8_SHAPES[] = {{128, 256, 0.60, 3.3, 3.2}, {128, 128, 0.42, 1.7, 2.4}, {64, 256, 0.46, 1.9, 2.4}, {64, 128, 0.40, 0.9, 2.1}, {32, 256, 0.44, 1.7, 2.2}};
+
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   if (p.rows == 0 || p.nseg == 0) return 1;
   if (!p.status && !(p.status = fp8_status_word())) return 0;
@@ -736,24 +740,33 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   p.Op = round_up(p.O, 16);
   if (fp8_stream_ok(p)) return launch_fp8_stream(p, st);
   const bool gated = p.h_codes != nullptr;
-  // Rows of a tile, row tiles the call is likely to have, and the most it can have.  All are functions of the call's shapes alone.
+  // The tile and the CTAs that share one, all functions of the call's shapes alone: the cheapest of what was measured.  Experts'
+  // rows of a tile follow from their average segment (a tile passes the weights once more): 32 up to 20 rows, 64 up to 56, 128
+  // from there where their tiles fill the SMs.  Us a call, 128 / 64 rows: H 7168, I 2048, 32 experts, 53 rows each 274 / 249,
+  // 64 rows 279 / 312; H 2048, I 768, 64 experts, 64 rows 100 / 82, 94 rows 103 / 103; 64 / 32 rows: 32 experts, 19 rows 49.6 / 46.0.
   const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
   const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
-  // 128 rows where segments are long and their tiles fill the SMs.  Us a call, 128 / 64 rows: one segment of 100 rows x 2048 x 2048
-  // 14.7 / 7.6, of 200 x 4096 x 1024 15.5 / 9.1; experts of H 7168, I 2048, 32 of them, 53 rows each 274 / 249, 64 rows 279 / 312
-  // (their weights pass twice for a segment of more than 64); H 2048, I 768, 64 experts, 64 rows 100 / 82, 94 rows 103 / 103.
   const long full = ((mean + 127) / 128) * (segs > 0 ? segs : 1) * ((p.O + 127) / 128);
-  int ar = mean <= (p.seg_count && p.KT > 32 ? 56 : 64) || full <= COLI_SMS ? 64 : 128;
-  if (mean <= (p.seg_count ? 20 : 32)) ar = 32;  // (64-row tiles: 600 rows on 32 experts, H 2048, I 768, 49.6 us, with 32 rows 46.0)
-  const int most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : (p.rows + ar - 1) / ar;
-  const int likely = p.seg_count ? p.rows_expected / ar + segs : most;
-  int bn = 256;
-  if (!gated && (long)likely * ((p.O + 255) / 256) < COLI_SMS) bn = 128, ar = ar < 64 ? 64 : ar;
-  const int fw = gated ? 128 : bn;
-  p.n_tiles = (p.O + fw - 1) / fw;
-  const long tiles = (long)(likely > 0 ? likely : 1) * p.n_tiles;
-  p.split = 1;
-  while (p.split < F8_MAX_SPLIT && tiles * p.split * 2 <= COLI_SMS && p.split * 2 <= p.KT) p.split *= 2;
+  const int wanted = !p.seg_count ? 0 : mean <= 20 ? 32 : mean <= (p.KT > 32 ? 56 : 64) || full <= COLI_SMS ? 64 : 128;
+  int ar = 0, bn = 0, most = 0;
+  double best = 0.0;
+  for (const F8Shape &f : F8_SHAPES) {
+    if ((wanted && f.ar != wanted) || (gated && f.bn != 256)) continue;
+    const int fw = gated ? 128 : f.bn;
+    const int row_tiles = p.seg_count ? p.rows_expected / f.ar + segs : (p.rows + f.ar - 1) / f.ar;
+    const long tiles = (long)(row_tiles > 0 ? row_tiles : 1) * ((p.O + fw - 1) / fw);
+    for (int split = 1; split <= F8_MAX_SPLIT && split <= p.KT && (split == 1 || tiles * split <= COLI_SMS); split *= 2) {
+      const long rounds = (tiles * split + COLI_SMS - 1) / COLI_SMS;
+      const double us = rounds * ((p.KT + split - 1) / split * f.kt_us + f.end_us) + (split > 1 ? f.join_us : 0.0);
+      if (ar && us >= best) continue;
+      best = us;
+      ar = f.ar;
+      bn = f.bn;
+      p.split = split;
+      p.n_tiles = (p.O + fw - 1) / fw;
+      most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : row_tiles;
+    }
+  }
   F8Maps maps;
   // One segment has full boxes and a last one; behind counts on the device any may come (an encoding takes 0.3 us).
   auto box_of = [](int n) {
