@@ -286,10 +286,12 @@ int coli_b200_moe_experts_dev(ColiMoe *moe, const void *rows_dev, const int32_t 
 /* The same experts in 8-bit arithmetic (handles of format 8 only; the calls of "8-bit rows" below make
  * the rows): codes_dev / scales_dev are expert-contiguous rows of H columns, seg_count_dev[n_local] the
  * rows of each resident expert (counts that run past rows_cap are cut there).  h = act(gate x, up x) is
- * quantised again, one scale per row and 128 features, by the rule of coli_b200_quantize_rows_fp8; both
+ * quantised again, one scale per row and 128 features, by the rule of coli_b200_quantize_rows_fp8 (with a
+ * rounded reciprocal of the scale where 128 features are made at once); both
  * products are those of coli_b200_matmul_fp8_dev; y_dev is bf16 [rows, H] (16-byte aligned), written
  * for the rows of the segments only: what lies behind the last one stays as it was.  rows_expected
- * only selects how the work is cut, as above.  Uses the handle's workspace like the call above. */
+ * only selects how the work is cut, as above.  Uses the handle's workspace like the call above; the first
+ * call of a size may enlarge it (which synchronises, and a stream capture does not allow). */
 int coli_b200_moe_experts_fp8_dev(ColiMoe *moe, const void *codes_dev, int64_t ld, const float *scales_dev, int64_t s_row,
                                   int64_t s_blk, const int32_t *seg_count_dev, int rows_cap, int rows_expected, void *y_dev,
                                   void *stream);
@@ -307,7 +309,8 @@ int coli_b200_moe_finish_dev(ColiMoe *moe, const float *partial_dev, const void 
 /* ---- 8-bit rows: DEVICE pointers, asynchronous on `stream`, no handle, no workspace ----------------
  * A matrix of rows in 8 bits is e4m3 codes [rows, K], `ld` bytes from row to row (a multiple of 16, at
  * least K rounded up to 16; 16-byte aligned), and an f32 scale for each row and 128 columns, the scale
- * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.
+ * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.  Results must not
+ * overlap what a call reads.  The calls leave the caller's current device as it was.
  *
  * Quantises rows x_dev of x_type (COLI_TYPE_*), x_stride elements apart: row r of the result is row r of
  * x (rows <= T), or with row_token_dev [rows] row row_token_dev[r] of it; an entry outside [0,T) is no
