@@ -90,8 +90,9 @@ def test_experts(fake_cuda, handles):
         return fake.coli_b200_moe_experts_fp8_dev(a["m"], a["codes"], a["ld"], a["scales"], a["sr"], a["sb"], a["counts"], a["cap"], a["expected"], a["y"],
                                                   None), fake.fake_queued()
 
-    # gate/up and down, and between them the row quantiser where segments have a few rows
-    assert call() == (1, 3) and call(cap=0) == (1, 0) and call(expected=0) == (1, 3) and call(cap=1000, expected=1000) == (1, 2)
+    # gate/up and down, and between them the row quantiser where segments have two rows on average or fewer
+    assert call() == (1, 2) and call(expected=2 * E) == (1, 3) and call(cap=0) == (1, 0) and call(expected=0) == (1, 3)
+    assert call(cap=1000, expected=1000) == (1, 2)
     for bad in (dict(m=None), dict(m=handles[4]), dict(codes=None), dict(codes=at(A, 8)), dict(ld=24), dict(scales=None), dict(counts=None),
                 dict(counts=at(W, 1)), dict(cap=-1), dict(expected=-1), dict(y=None), dict(y=at(Y, 8)), dict(sr=-2)):
         assert call(**bad) == (0, 0), bad
