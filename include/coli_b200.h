@@ -339,7 +339,9 @@ int coli_b200_fp8_check(int device);
  * logits_dev [T,E] of `type` (COLI_TYPE_*), `stride` elements from row to row.  With z = logit + logit_bias (may be
  * NULL) an expert takes part where z > -inf: -inf and NaN close it to that token, a row of them is no token.
  *   score  softmax over the open experts, or sigmoid
- *   choice score + select_bias (may be NULL), compared in 64 bits; ties go to the lowest expert.  With n_group > 1 only
+ *   choice score + select_bias (may be NULL), compared in 64 bits (arguments of exp beyond +-708 count as that); without
+ *          biases and groups the logits themselves; ties go to the lowest expert, and what a bias makes -inf or
+ *          NaN is not chosen.  With n_group > 1 only
  *          experts of the topk_group best groups (contiguous; a group's mark is the sum of its two best choices, or
  *          its only one; ties to the lowest)
  *   weight score of the chosen, divided by their sum + 1e-20 if norm_topk, times routed_scale

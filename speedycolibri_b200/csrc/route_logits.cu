@@ -322,14 +322,15 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
       const int e = lane + 32 * s;
       choice[s] = softmax ? (z[s] == m ? 1.0f : __expf(z[s] - m)) * inv : __fdividef(1.0f, 1.0f + __expf(fminf(-z[s], 80.0f)));
       if (p.select_bias && e < p.E) choice[s] += __ldg(p.select_bias + e);
+      if (key[s]) key[s] = choice[s] > NEG_INF ? rl_key32(choice[s]) : 0u;
       if (key[s]) {
-        key[s] = choice[s] > NEG_INF ? rl_key32(choice[s]) : 0u;
         size = fmaxf(size, fabsf(choice[s]));
         arg = fmaxf(arg, fminf(fabsf(z[s]), 128.0f));
       }
     }
     size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size)));
     arg = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(arg)));
+    if (!(size <= 1.0e38f)) return -1;  // (the sum of two may leave f32)
     apart = 2.0f * (1.9e-6f + 2.4e-7f * size + (p.logit_bias ? 1.2e-7f * arg : 0.0f));
     if (p.n_group > 1) {
       const float gap = rl_groups<SLOTS, uint32_t, float>(p, key, choice, NEG_INF, row, reinterpret_cast<float *>(cand), lane);

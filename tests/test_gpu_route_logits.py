@@ -122,6 +122,24 @@ def test_ties_infinities_and_lowest_values(gpu_backend):
     assert got.idx[0].tolist() == list(range(8)) and got.idx[1, :3].tolist() == [4, 33, 90]
 
 
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+def test_biases_of_the_lowest_value(gpu_backend, score):
+    # groups 0 and 1 are closed, 2 has one open expert, and two choices of group 3 leave f32 when added
+    lowest = torch.finfo(torch.float32).min
+    z = logits(6, 8, 8)
+    z[:, :4] = -math.inf
+    z[:, 5] = -math.inf
+    bias = torch.zeros(8, device="cuda")
+    bias[6:] = lowest
+    check(gpu_backend, z, 2, score, select_bias=bias, G=4, kept=3)
+    bias[6] = -math.inf  # (the plain form keeps what can be chosen alone)
+    got = gpu_backend.route_logits_dev(z, 2, score, select_bias=bias, n_group=4, topk_group=3)
+    assert (got.idx.cpu() == torch.tensor([4, 7])).all()
+    bias[7], bias[4] = -math.inf, 1.0
+    got = gpu_backend.route_logits_dev(z, 2, score, select_bias=bias, n_group=4, topk_group=3)
+    assert (got.idx.cpu() == torch.tensor([4, -1])).all()
+
+
 def test_scores_that_32_bits_do_not_tell_apart(gpu_backend):
     z = torch.full((1, 64), 20.0, device="cuda")
     z[0, 50], z[0, 13] = 20.00001, 20.000002  # sigmoids all 1 in f32
