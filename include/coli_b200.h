@@ -309,7 +309,8 @@ int coli_b200_moe_finish_dev(ColiMoe *moe, const float *partial_dev, const void 
 /* ---- 8-bit rows: DEVICE pointers, asynchronous on `stream`, no handle, no workspace ----------------
  * A matrix of rows in 8 bits is e4m3 codes [rows, K], `ld` bytes from row to row (a multiple of 16, at
  * least K rounded up to 16; 16-byte aligned), and an f32 scale for each row and 128 columns, the scale
- * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.  Results must not
+ * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.  At most 2^30 rows;
+ * what lies behind a row's K codes is not read.  Results must not
  * overlap what a call reads.  The calls leave the caller's current device as it was.
  *
  * Quantises rows x_dev of x_type (COLI_TYPE_*), x_stride elements apart: row r of the result is row r of

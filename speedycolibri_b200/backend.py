@@ -226,12 +226,14 @@ def _rows_fp8(what: str, codes, scales, K: int):
     if len(shape) != 2 or shape[1] != K or codes.element_size() != 1 or (K > 1 and stride[1] != 1):
         raise ValueError(f"{what}: codes must be one byte each, [rows, {K}], columns next to each other")
     R = shape[0]
+    if R > 1 << 30:  # (before ctypes cuts it to 32 bits)
+        raise ValueError(f"{what}: {R} rows (at most 2^30)")
     if scales.shape != (R, (K + 127) // 128) or scales.dtype != _torch_().f32:
         raise ValueError(f"{what}: scales must be f32 [{R}, {(K + 127) // 128}], not {scales.dtype} {tuple(scales.shape)}")
     s_row, s_blk = scales.stride()
     ld = stride[0]
     if R < 2:  # (a single row may say anything)
-        ld = max(ld, (K + 15) // 16 * 16)
+        ld = (K + 15) // 16 * 16
     return R, ld, s_row, s_blk
 
 
@@ -245,6 +247,8 @@ def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     if ty is None or len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and xs[1] != 1):
         raise ValueError("quantize_rows_fp8_dev: x must be f32, f16 or bf16 [T,K], columns next to each other")
     T, K = shape
+    if T >= 1 << 31 or K >= 1 << 31:
+        raise ValueError(f"quantize_rows_fp8_dev: x [{T}, {K}] is past 32 bits")
     if row_token is None:
         R, take = T, None
     elif row_token.dtype != th.i32 or row_token.dim() != 1 or not row_token.is_contiguous():
@@ -259,6 +263,8 @@ def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     rows, ld, s_row, s_blk = _rows_fp8("quantize_rows_fp8_dev", codes, scales, K)
     if rows != R:
         raise ValueError(f"quantize_rows_fp8_dev: out has {rows} rows, not {R}")
+    if out is not None and K % 16 and rows and codes.storage_offset() + (rows - 1) * ld + (K + 15) // 16 * 16 > codes.untyped_storage().nbytes():
+        raise ValueError("quantize_rows_fp8_dev: out's codes need room up to a multiple of 16 bytes behind the last row")
     device = x.get_device()
     _same_gpu("quantize_rows_fp8_dev", device, codes, scales, row_token)
     if not _lib_().coli_b200_quantize_rows_fp8(device, x.data_ptr(), ty, xs[0], take, T, R, K, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk,
@@ -313,6 +319,8 @@ def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=Non
     if ty is None or len(shape) != 2 or (shape[1] > 1 and zs[1] != 1):
         raise ValueError("route_logits_dev: logits must be f32, f16 or bf16 [T,E], experts next to each other")
     T, E = shape
+    if T > 1 << 20 or E > 512:
+        raise ValueError(f"route_logits_dev: logits [{T}, {E}] (T <= 2^20, E <= 512)")
     for name, b in (("select_bias", select_bias), ("logit_bias", logit_bias)):
         if b is not None and (b.dtype != th.f32 or b.numel() != E or not b.is_contiguous()):
             raise ValueError(f"route_logits_dev: {name} must be contiguous f32 [{E}]")

@@ -1206,8 +1206,8 @@ size_t type_size(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYP
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 // Codes are copied by TMA (16-byte rows), scales read one by one.
 bool check_fp8_rows(const char *who, const void *codes, int64_t ld, const float *scales, int64_t s_row, int64_t s_blk, int rows, int K) {
-  if (rows < 0 || (rows > 0 && (!codes || !scales))) {
-    coli_set_error("%s: bad row count %d or null pointer", who, rows);
+  if (rows < 0 || rows > 1 << 30 || (rows > 0 && (!codes || !scales))) {  // (tables add a tile's rows to them)
+    coli_set_error("%s: bad row count %d (at most 2^30) or null pointer", who, rows);
     return false;
   }
   if (ld < round_up(K, 16) || ld % 16 || !aligned_to(codes, 16) || !aligned_to(scales, 4)) {

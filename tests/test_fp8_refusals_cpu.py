@@ -43,7 +43,7 @@ def test_quantise(fake_cuda):
 
     assert call() == (1, 1) and call(take=W, rows=9) == (1, 1) and call(x=at(A, 2), stride=41) == (1, 1) and call(rows=0) == (1, 1)
     for bad in (dict(ty=3), dict(ty=-1), dict(K=0), dict(T=-1), dict(rows=-1), dict(rows=6), dict(x=None), dict(codes=None), dict(scales=None),
-                dict(x=at(A, 1)), dict(ty=0, x=at(A, 2)), dict(stride=-1), dict(ld=47), dict(ld=32), dict(ld=56), dict(codes=at(B, 8)),
+                dict(take=W, rows=2**30 + 1), dict(x=at(A, 1)), dict(ty=0, x=at(A, 2)), dict(stride=-1), dict(ld=47), dict(ld=32), dict(ld=56), dict(codes=at(B, 8)),
                 dict(scales=at(S, 2)), dict(sr=-1), dict(sb=-1), dict(take=at(W, 2)), dict(device=3)):
         assert call(**bad) == (0, 0), bad
 
@@ -60,7 +60,7 @@ def test_product(fake_cuda):
                                              None), fake.fake_queued()
 
     assert call() == (1, 1) and call(y=at(Y, 2), ys=33) == (1, 1) and call(rows=1, ys=0) == (1, 1)
-    for bad in (dict(w=None), dict(w=row_scaled), dict(codes=None), dict(codes=at(A, 4)), dict(ld=40), dict(ld=50), dict(scales=None), dict(rows=-1),
+    for bad in (dict(w=None), dict(w=row_scaled), dict(codes=None), dict(codes=at(A, 4)), dict(ld=40), dict(ld=50), dict(scales=None), dict(rows=-1), dict(rows=2**30 + 1),
                 dict(y=None), dict(y=at(Y, 1)), dict(ty=0, y=at(Y, 2)), dict(ty=9), dict(ys=23), dict(sr=-1), dict(sb=-1), dict(ld=1 << 41)):
         assert call(**bad) == (0, 0), bad
 
@@ -94,7 +94,7 @@ def test_experts(fake_cuda, handles):
     assert call() == (1, 2) and call(expected=2 * E) == (1, 3) and call(cap=0) == (1, 0) and call(expected=0) == (1, 3)
     assert call(cap=1000, expected=1000) == (1, 2)
     for bad in (dict(m=None), dict(m=handles[4]), dict(codes=None), dict(codes=at(A, 8)), dict(ld=24), dict(scales=None), dict(counts=None),
-                dict(counts=at(W, 1)), dict(cap=-1), dict(expected=-1), dict(y=None), dict(y=at(Y, 8)), dict(sr=-2)):
+                dict(counts=at(W, 1)), dict(cap=-1), dict(cap=2**31 - 1), dict(expected=-1), dict(y=None), dict(y=at(Y, 8)), dict(sr=-2)):
         assert call(**bad) == (0, 0), bad
 
 

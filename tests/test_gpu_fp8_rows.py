@@ -329,6 +329,14 @@ def test_refusals(gpu_backend):
                 lambda: b.matmul_fp8_dev(w, q, s, out_dtype=torch.float16, out=torch.empty((4, 64), device=cuda))):
         with pytest.raises(ValueError):
             bad()
+    one = torch.zeros(128, dtype=torch.uint8, device=cuda)  # a row of 100 codes that ends with its storage's
+    for part, fits in ((one[28:].view(1, 100), False), (one[16:116].view(1, 100), True)):
+        if not fits:
+            with pytest.raises(ValueError):
+                b.quantize_rows_fp8_dev(x[:1, :100], out=(part, s[:1]))
+        else:
+            b.quantize_rows_fp8_dev(x[:1, :100], out=(part, s[:1]))
+            assert (part == 0x7E).all() and (one[116:] == 0).all()  # 1 = 448 / 448, the largest code
     with pytest.raises(b.CudaError):  # rows of codes off the 16-byte grid
         b.matmul_fp8_dev(w, torch.zeros((4, 150), dtype=torch.uint8, device=cuda)[:, :128], s)
     block, _ = expert_layer(b, 2, 128, 64, 4)
