@@ -459,7 +459,7 @@ template <typename T, bool CLUSTER>
 __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid_constant__ RouteLogitsParams p) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int t0 = blockIdx.x * p.chunk, tokens = max(0, min(p.chunk, p.T - t0)), pairs = tokens * p.k, words = p.chunk / 32;
+  const int t0 = blockIdx.x * p.chunk, tokens = max(0, min(p.chunk, p.T - t0)), pairs = tokens * p.k, words = (p.chunk + 31) / 32;
   int *ids = reinterpret_cast<int *>(rl_smem);  // the chunk's choices, then per-warp memory, later the tables
   unsigned char *after = rl_smem + (((size_t)p.chunk * p.k * 4 + 15) & ~(size_t)15);
   unsigned char *cand = after + warp * RL_CAND_BYTES;
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid
 constexpr int RL_PLACE_THREADS = 512;
 __global__ void __launch_bounds__(RL_PLACE_THREADS) k_route_place(const __grid_constant__ RouteLogitsParams p, int chunks) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
-  const int words = p.chunk / 32, pitch = (p.E + 3) & ~3;
+  const int words = (p.chunk + 31) / 32, pitch = (p.E + 3) & ~3;
   uint32_t *mask = reinterpret_cast<uint32_t *>(rl_smem);
   int *cnt = reinterpret_cast<int *>(mask + p.E * words), *before = cnt + pitch, *off = before + pitch;
   for (int e = threadIdx.x; e < 2 * pitch; e += blockDim.x) cnt[e] = 0;
@@ -612,7 +612,7 @@ static int launch_route_kernel(const RouteLogitsParams &p, int ctas, int warps, 
 
 int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
   p.chunk = route_logits_chunk(p.T);
-  const int chunks = (p.T + p.chunk - 1) / p.chunk, words = p.chunk / 32;
+  const int chunks = (p.T + p.chunk - 1) / p.chunk, words = (p.chunk + 31) / 32;
   // a warp per token up to 32; a few more for the tables where there are few tokens
   const int tokens = p.T < p.chunk ? p.T : p.chunk, warps = tokens < 4 ? 4 : tokens < RL_MAX_WARPS ? tokens : RL_MAX_WARPS;
   const size_t pitch = (p.E + 3) & ~3, own = (size_t)warps * (RL_CAND_BYTES + (p.n_group > 1 ? (size_t)p.E * 8 : 0));

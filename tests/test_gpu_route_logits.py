@@ -79,7 +79,7 @@ def test_sizes_and_types(gpu_backend, dtype, score, T, E, k):
     check(gpu_backend, logits(T, E, 1, dtype), k, score, norm=bool(T % 2), scale=2.5)
 
 
-@pytest.mark.parametrize("T", [33, 64, 65, 97, 129, 256, 257, 512, 513, 1024, 1025, 4736, 4737, 9472, 9473])
+@pytest.mark.parametrize("T", [33, 64, 65, 97, 129, 256, 257, 512, 513, 1024, 1025, 4736, 4737, 9472, 9473, 18944, 18945])
 def test_chunk_lines(gpu_backend, T):
     check(gpu_backend, logits(T, 16, 2), 2, SOFTMAX)
 
