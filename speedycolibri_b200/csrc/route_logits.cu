@@ -535,8 +535,12 @@ __global__ void __launch_bounds__(RL_MAX_WARPS * 32) k_route_logits(const __grid
   for (int i = total + (int)threadIdx.x; i < pairs; i += blockDim.x) p.row_token[i] = -1;
 }
 
-// One CTA per chunk: rows of every expert before the chunk from all chunks' counts, then the places of its pairs.
-constexpr int RL_PLACE_THREADS = 512;
+// One CTA per chunk: rows of every expert before the chunk from all chunks' counts, then the places of its pairs.  Its CTAs wait for
+// one another's memory most of the time: as large as they may be (16384 tokens, 384 experts, both kernels: 36.8 us with 512
+// threads, 30.4 with 1024), and where they are no more than the SMs one on each, by the shared memory that they ask for: launched
+// early, they would pack onto the SMs that their predecessor leaves first (27.5 us; 20000 tokens in 295 chunks 32.9, without 30.8).
+constexpr int RL_PLACE_THREADS = 1024;
+constexpr int RL_PLACE_ALONE = 116 * 1024;  // more than half of an SM's
 __global__ void __launch_bounds__(RL_PLACE_THREADS) k_route_place(const __grid_constant__ RouteLogitsParams p, int chunks) {
   extern __shared__ __align__(16) unsigned char rl_smem[];
   const int words = (p.chunk + 31) / 32, pitch = (p.E + 3) & ~3;
@@ -621,8 +625,11 @@ int launch_route_logits(RouteLogitsParams p, cudaStream_t st) {
   if (chunks == 1) return launch_route_kernel<false>(p, 1, warps, smem, st);
   if (chunks <= ROUTE_LOGITS_CLUSTER) return launch_route_kernel<true>(p, chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16, warps, smem, st);
   if (!launch_route_kernel<false>(p, chunks, warps, smem, st)) return 0;
+  static ColiPerDeviceOnce place_once;
+  if (!coli_set_smem_limit(place_once, k_route_place, RL_PLACE_ALONE, "placement shared-memory attribute")) return 0;
+  const size_t place = chunks <= COLI_SMS ? (size_t)RL_PLACE_ALONE : tables;  // (tables: 17 KB at most)
   coli_count_launch(1);
-  return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(RL_PLACE_THREADS), tables, st, p, chunks), "placement launch") ? 1 : 0;
+  return coli_cuda_check(launch_dependent(k_route_place, dim3(chunks), dim3(RL_PLACE_THREADS), place, st, p, chunks), "placement launch") ? 1 : 0;
 }
 
 }  // namespace colib
