@@ -18,16 +18,18 @@ namespace colib {
 // that either shows in every product with the row.
 // LANES lanes share a block, in pieces of 16 bytes; a warp takes QR_COLS columns of a row and goes through the rows with the next
 // one's pieces already requested; the warps of a CTA take neighbouring rows, whose scales of a block lie side by side.  Four lanes
-// halve what a block's scale costs (32768 gathered rows of 7168 bf16 99.7 -> 90.4 us, with eight lanes and two quotients an
+// halve what a block's scale costs (32768 gathered rows of 7168 bf16 99.7 -> 90.4 us before WHOLE, with eight lanes and two quotients an
 // instruction; rows as they are 112 -> 108.5, 6.5 TB/s); values read one by one, off the 16-byte grid, and f32, whose codes would be
-// stored half a sector at a time, keep eight (5000 rows of 1111 f16 11.0 us, with four 16.4).
+// stored half a sector at a time, keep eight (5000 rows of 1111 f16 11.0 us, with four 16.4).  WHOLE: gathered rows of whole pieces,
+// which the L2 has as a rule and the instructions bound, are read without a branch per piece (the gathered rows 92.0 -> 83.8 us);
+// rows as they are come faster from HBM with the branches, 108.7 against 131.
 constexpr int QR_COLS = 1024;
 template <typename T, int LANES>
 struct QrPieces {
   static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 128 / LANES / VEC, COLS = 32 / LANES * 128, STEPS = QR_COLS / COLS;
   uint4 q[STEPS][LOADS];
 };
-template <typename T, int LANES>
+template <typename T, int LANES, bool WHOLE>
 __device__ __forceinline__ void qr_request(QrPieces<T, LANES> &d, const QuantRowsParams &p, int src, int c0) {
   using P = QrPieces<T, LANES>;
   constexpr int VEC = P::VEC, STEPS = P::STEPS, COLS = P::COLS;
@@ -37,7 +39,9 @@ __device__ __forceinline__ void qr_request(QrPieces<T, LANES> &d, const QuantRow
 #pragma unroll
     for (int l = 0; l < P::LOADS; ++l) {
       const int c = c0 + COLS * j + LANES * VEC * l;
-      if (p.x_vec && c + VEC <= p.K) {
+      if constexpr (WHOLE) {
+        d.q[j][l] = c < p.K ? __ldg(reinterpret_cast<const uint4 *>(x + c)) : make_uint4(0u, 0u, 0u, 0u);
+      } else if (p.x_vec && c + VEC <= p.K) {
         d.q[j][l] = __ldg(reinterpret_cast<const uint4 *>(x + c));
       } else {
         alignas(16) T raw[VEC];
@@ -75,7 +79,7 @@ struct QrMax<__nv_bfloat16> {
   using type = __nv_bfloat162;
 };
 
-template <typename T, int LANES>
+template <typename T, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(QuantRowsParams p) {
   using P = QrPieces<T, LANES>;
   constexpr int STEPS = P::STEPS, COLS = P::COLS;
@@ -91,10 +95,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
   long r = blockIdx.x * 8 + (threadIdx.x >> 5);
   P now, next;
   int src = source(r), src_next = source(r + step);
-  if (valid(src)) qr_request<T, LANES>(now, p, src, c0);
+  if (valid(src)) qr_request<T, LANES, WHOLE>(now, p, src, c0);
   for (; r < rows; r += step) {
     const int src_after = source(r + 2 * (long)step);
-    if (valid(src_next)) qr_request<T, LANES>(next, p, src_next, c0);
+    if (valid(src_next)) qr_request<T, LANES, WHOLE>(next, p, src_next, c0);
     if (valid(src)) {  // (no token: the row is left as it was)
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
@@ -145,13 +149,13 @@ int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
   const int each = fit / chunks > 0 ? fit / chunks : 1;
   const dim3 grid((unsigned)(groups < each ? groups : each), (unsigned)chunks);
   coli_count_launch(1);
-  cudaError_t e;
-  if (p.type == COLI_TYPE_F32)
-    e = launch_dependent(k_quant_rows<float, 8>, grid, dim3(256), 0, st, p);
-  else if (p.type == COLI_TYPE_F16)
-    e = launch_dependent(p.x_vec ? k_quant_rows<__half, 4> : k_quant_rows<__half, 8>, grid, dim3(256), 0, st, p);
-  else
-    e = launch_dependent(p.x_vec ? k_quant_rows<__nv_bfloat16, 4> : k_quant_rows<__nv_bfloat16, 8>, grid, dim3(256), 0, st, p);
+  const bool whole = p.x_vec && p.row_token && p.K % 8 == 0;
+  auto of16 = [&](auto t) {
+    using T = decltype(t);
+    return whole ? k_quant_rows<T, 4, true> : p.x_vec ? k_quant_rows<T, 4, false> : k_quant_rows<T, 8, false>;
+  };
+  auto *kernel = p.type == COLI_TYPE_F32 ? k_quant_rows<float, 8, false> : p.type == COLI_TYPE_F16 ? of16(__half()) : of16(__nv_bfloat16());
+  const cudaError_t e = launch_dependent(kernel, grid, dim3(256), 0, st, p);
   return coli_cuda_check(e, "row quantiser launch") ? 1 : 0;
 }
 

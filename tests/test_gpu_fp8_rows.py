@@ -91,6 +91,21 @@ def test_quantiser_gathers(gpu_backend):
             assert (codes[r] == 0x33).all() and (scales[r] == -1.0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K", [8, 136, 1000, 1032, 2048])
+def test_gathered_rows_of_whole_pieces(gpu_backend, dtype, K):
+    x = rows(70, K, 4).to(dtype)
+    take = torch.arange(500, dtype=torch.int32, device="cuda") * 37 % 73  # (some past the last row)
+    codes = torch.full((500, (K + 15) // 16 * 16), 0x33, dtype=torch.uint8, device="cuda")[:, :K]
+    scales = torch.full((500, (K + 127) // 128), -1.0, device="cuda")
+    gpu_backend.quantize_rows_fp8_dev(x, take, out=(codes, scales))
+    want = gpu_backend.quantize_rows_fp8_dev(x)
+    some = take < 70
+    at = take[some].long()
+    assert torch.equal(codes[some], want[0][at]) and torch.equal(scales[some], want[1][at])
+    assert (codes[~some] == 0x33).all() and (scales[~some] == -1.0).all()
+
+
 def test_quantiser_of_special_values(gpu_backend):
     x = torch.zeros((5, 256), device="cuda")
     x[1, 3], x[1, 4], x[1, 200] = torch.nan, 2.0, 1.0
