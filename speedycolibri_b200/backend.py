@@ -211,6 +211,13 @@ def _torch_() -> _Torch:
     return _torch
 
 
+def _on(stream: int, device):
+    """The current stream is `stream` (a raw handle) inside: what a call allocates there is handed out in that stream's order."""
+    import torch
+
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device))
+
+
 def _same_gpu(what: str, device: int, *tensors) -> None:
     """Raises unless every given tensor is on GPU `device` (-1: the host)."""
     for t in tensors:
@@ -239,9 +246,12 @@ def _rows_fp8(what: str, codes, scales, K: int):
 
 def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     """coli_b200_quantize_rows_fp8: rows of x (f32, f16 or bf16 [T,K] on the GPU, any row stride) -> (codes u8 [R,K],
-    scales f32 [R, ceil(K/128)]), on the current torch stream.  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
+    scales f32 [R, ceil(K/128)]), on the current torch stream or on `stream` (a raw handle).  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
     outside [0,T) leaves the row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16
     bytes and a block's scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
+    if stream is not None and x.is_cuda:
+        with _on(stream, x.device):
+            return quantize_rows_fp8_dev(x, row_token, out)
     th = _torch or _torch_()
     ty, shape, xs = th.types.get(x.dtype), x.shape, x.stride()
     if ty is None or len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and xs[1] != 1):
@@ -268,14 +278,17 @@ def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     device = x.get_device()
     _same_gpu("quantize_rows_fp8_dev", device, codes, scales, row_token)
     if not _lib_().coli_b200_quantize_rows_fp8(device, x.data_ptr(), ty, xs[0], take, T, R, K, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk,
-                                               th.stream(device) if stream is None else stream):
+                                               th.stream(device)):
         _check(0, "coli_b200_quantize_rows_fp8")
     return codes, scales
 
 
 def matmul_fp8_dev(w: CudaTensor, codes, scales, out_dtype=None, out=None, stream=None):
     """coli_b200_matmul_fp8_dev: 8-bit rows [R, w.I] times a resident weight of format 8 -> [R, w.O] as `out_dtype` (bf16
-    unless given) or into `out` (f32, f16 or bf16, any row stride), on the current torch stream."""
+    unless given) or into `out` (f32, f16 or bf16, any row stride), on the current torch stream or on `stream`."""
+    if stream is not None and codes.is_cuda:
+        with _on(stream, codes.device):
+            return matmul_fp8_dev(w, codes, scales, out_dtype, out)
     th = _torch or _torch_()
     R, ld, s_row, s_blk = _rows_fp8("matmul_fp8_dev", codes, scales, w.I)
     O = w.O
@@ -289,7 +302,7 @@ def matmul_fp8_dev(w: CudaTensor, codes, scales, out_dtype=None, out=None, strea
     if device != w.device:
         raise ValueError(f"matmul_fp8_dev: the weight is on cuda:{w.device}, the rows on cuda:{device}")
     if not _lib_().coli_b200_matmul_fp8_dev(w.handle, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk, R, out.data_ptr(), ty, stride[0],
-                                            th.stream(device) if stream is None else stream):
+                                            th.stream(device)):
         _check(0, "coli_b200_matmul_fp8_dev")
     return out
 
@@ -313,7 +326,11 @@ class Routing(NamedTuple):
 def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=None, logit_bias=None, norm_topk: bool = False,
                      routed_scale: float = 1.0, n_group: int = 1, topk_group: int = 1, out=None, stream=None) -> Routing:
     """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing, on the current torch
-    stream.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are written in place."""
+    stream or on `stream`.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are
+    written in place."""
+    if stream is not None and logits.is_cuda:
+        with _on(stream, logits.device):
+            return route_logits_dev(logits, k, score, select_bias, logit_bias, norm_topk, routed_scale, n_group, topk_group, out)
     th = _torch or _torch_()
     ty, shape, zs = th.types.get(logits.dtype), logits.shape, logits.stride()
     if ty is None or len(shape) != 2 or (shape[1] > 1 and zs[1] != 1):
@@ -339,14 +356,10 @@ def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=Non
     lib = _lib_()
     n = lib.coli_b200_route_logits_workspace(T, E)
     work = th.empty(n, dtype=th.u8, device=logits.device) if n else None
-    if work is not None and stream is not None:
-        import torch
-
-        work.record_stream(torch.cuda.ExternalStream(stream, device=logits.device))
     if not lib.coli_b200_route_logits(device, logits.data_ptr(), ty, zs[0] if T > 1 else E, None if select_bias is None else select_bias.data_ptr(),
                                       None if logit_bias is None else logit_bias.data_ptr(), T, E, k, score, norm_topk, routed_scale, n_group,
                                       topk_group, out.idx.data_ptr(), out.w.data_ptr(), out.expert_rows.data_ptr(), out.slot.data_ptr(),
-                                      out.row_token.data_ptr(), None if work is None else work.data_ptr(), th.stream(device) if stream is None else stream):
+                                      out.row_token.data_ptr(), None if work is None else work.data_ptr(), th.stream(device)):
         _check(0, "coli_b200_route_logits")
     return out
 

@@ -21,6 +21,27 @@ def run(backend, block, logits, x, k, out, **kw):
     return r, codes, scales
 
 
+def test_calls_on_a_given_stream(gpu_backend):
+    # results and the router's counts come from the given stream's memory, so that calls in turn on two streams share none in flight
+    b, side = gpu_backend, [torch.cuda.Stream() for _ in range(2)]
+    x, z = torch.randn((5000, 512), device="cuda"), torch.randn((5000, 64), device="cuda")
+    codes, scales = b.quantize_fp8_b128_dev(torch.randn((256, 512), device="cuda"))
+    w = b.CudaTensor.from_device(8, codes, scales, 1.0, 512, 256)
+    want = [*b.route_logits_dev(z, 4), *b.quantize_rows_fp8_dev(x)]
+    want.append(b.matmul_fp8_dev(w, want[5], want[6]))
+    torch.cuda.synchronize()
+    got = []
+    for i in range(24):
+        s = 0 if i % 3 == 2 else side[i % 3].cuda_stream
+        r, (q, sx) = b.route_logits_dev(z, 4, stream=s), b.quantize_rows_fp8_dev(x, stream=s)
+        got.append([*r, q, sx, b.matmul_fp8_dev(w, q, sx, stream=s)])
+    torch.cuda.synchronize()
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+    for r in got:
+        assert all(torch.equal(a, v) for a, v in zip(r, want))
+    w.free()
+
+
 @pytest.mark.parametrize("T,E,k,H,I,pad", [(1, 8, 2, 256, 128, 0), (7, 8, 1, 128, 64, 2), (40, 16, 4, 512, 264, 3), (300, 8, 2, 640, 256, 50)])
 def test_the_operators_in_a_row(gpu_backend, T, E, k, H, I, pad):
     from speedycolibri_b200.configs import FMT_FP8_B128
