@@ -1,7 +1,8 @@
 // Routing from given logits: scores, choice of experts, weights, and the rows the chosen pairs take in expert order.
 // The rules are those of the block's own router (crates/colibri-engine/src/moe.rs:1047-1132; groups and the logit bias
 // as in routing.cu), with two differences that a caller's own logits make necessary: the choice is made on scores in 64
-// bits, so that experts whose scores 32 bits do not tell apart still come in the order of their logits, and an expert whose
+// bits (by the logits themselves, where neither a bias nor groups ask for scores), so that experts whose scores 32 bits
+// do not tell apart still come in the order of their logits, and an expert whose
 // logit is -inf or NaN is not chosen at all (a closed expert, a padded token), where the block's router falls back to expert 0.
 #include "route_logits.cuh"
 
