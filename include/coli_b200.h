@@ -306,7 +306,8 @@ int coli_b200_moe_combine_partial_dev(ColiMoe *moe, const void *y_rows_dev, cons
 int coli_b200_moe_finish_dev(ColiMoe *moe, const float *partial_dev, const void *shared_y_dev, void *out_dev, int T,
                              void *stream);
 
-/* ---- 8-bit rows: DEVICE pointers, asynchronous on `stream`, no handle, no workspace ----------------
+/* ---- 8-bit rows: DEVICE pointers, asynchronous on `stream`, no handle of their own, no workspace -----
+ * (coli_b200_quantize_rows_fp8 and coli_b200_route_logits may come before coli_cuda_init, or without it.)
  * A matrix of rows in 8 bits is e4m3 codes [rows, K], `ld` bytes from row to row (a multiple of 16, at
  * least K rounded up to 16; 16-byte aligned), and an f32 scale for each row and 128 columns, the scale
  * of (row, block) at scales[row * s_row + block * s_blk].  It stands for scale * code.  At most 2^30 rows;

@@ -246,7 +246,7 @@ def _rows_fp8(what: str, codes, scales, K: int):
 
 def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     """coli_b200_quantize_rows_fp8: rows of x (f32, f16 or bf16 [T,K] on the GPU, any row stride) -> (codes u8 [R,K],
-    scales f32 [R, ceil(K/128)]), on the current torch stream or on `stream` (a raw handle).  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
+    scales f32 [R, ceil(K/128)]), on the current torch stream or on `stream` (a raw handle); `init` need not come first.  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
     outside [0,T) leaves the row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16
     bytes and a block's scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
     if stream is not None and x.is_cuda:
@@ -326,7 +326,7 @@ class Routing(NamedTuple):
 def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=None, logit_bias=None, norm_topk: bool = False,
                      routed_scale: float = 1.0, n_group: int = 1, topk_group: int = 1, out=None, stream=None) -> Routing:
     """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing, on the current torch
-    stream or on `stream`.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are
+    stream or on `stream`; `init` need not come first.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are
     written in place."""
     if stream is not None and logits.is_cuda:
         with _on(stream, logits.device):

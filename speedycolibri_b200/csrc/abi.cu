@@ -65,6 +65,18 @@ bool coli_select_ctx(DeviceContext *c) { return c && coli_cuda_check(cudaSetDevi
 static DeviceContext *find_ctx(int device) { return coli_find_ctx(device); }
 static bool select_ctx(DeviceContext *c) { return coli_select_ctx(c); }
 
+// Whether `device` is one of the `n` visible ones, and of the architecture that the kernels are built for.
+static bool usable_device(int device, int n) {
+  cudaDeviceProp prop;
+  if (device < 0 || device >= n) {
+    coli_set_error("device %d is not one of the %d visible ones", device, n);
+    return false;
+  }
+  if (!coli_cuda_check(cudaGetDeviceProperties(&prop, device), "device properties")) return false;
+  if (prop.major != 10) coli_set_error("device %d is sm_%d%d; this library is built for sm_100a only", device, prop.major, prop.minor);
+  return prop.major == 10;
+}
+
 extern "C" int coli_cuda_init(const int *devices, int count) {
   std::lock_guard<std::mutex> lk(g_init_mu);
   for (int i = 0; devices && i < count && i < COLI_CUDA_MAX_DEVICES; ++i)  // a repeated ordinal is refused, backend_cuda.cu:2636-2640
@@ -93,15 +105,8 @@ extern "C" int coli_cuda_init(const int *devices, int count) {
     if (!same) coli_set_error("coli_cuda_init: already initialised with a different device set");
     return same ? 1 : 0;
   }
-  for (int i = 0; i < count; ++i) {
-    cudaDeviceProp prop;
-    if (devices[i] < 0 || devices[i] >= n || !coli_cuda_check(cudaGetDeviceProperties(&prop, devices[i]), "device properties"))
-      return 0;
-    if (prop.major != 10) {
-      coli_set_error("device %d is sm_%d%d; this library is built for sm_100a only", devices[i], prop.major, prop.minor);
-      return 0;
-    }
-  }
+  for (int i = 0; i < count; ++i)
+    if (!usable_device(devices[i], n)) return 0;
   for (int i = 0; i < count; ++i) {
     DeviceContext *c = new DeviceContext();
     c->device = devices[i];
@@ -1191,15 +1196,34 @@ namespace {
 struct OnDevice {
   int before = -1;
   bool ok = false, back = false;
-  explicit OnDevice(int device) {
-    DeviceContext *c = find_ctx(device);
-    if (!c) return;
+  explicit OnDevice(int device) { enter(device, find_ctx(device) != nullptr); }
+  void enter(int device, bool usable) {
+    if (!usable) return;
     if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-    ok = before == device || select_ctx(c);
+    ok = before == device || coli_cuda_check(cudaSetDevice(device), "cudaSetDevice");
     back = ok && before >= 0 && before != device;
   }
   ~OnDevice() {
     if (back) cudaSetDevice(before);
+  }
+
+ protected:
+  OnDevice() = default;
+};
+// The same for a call that keeps nothing between calls (no handle, no workspace of the library's): it may be a program's first
+// one, before coli_cuda_init or without it.  Looked at once per device.
+struct OnAnyDevice : OnDevice {
+  explicit OnAnyDevice(int device) {
+    static unsigned seen = 0;  // bit d: device d is usable
+    const unsigned bit = device >= 0 && device < 32 ? 1u << device : 0u;
+    bool usable = (__atomic_load_n(&seen, __ATOMIC_ACQUIRE) & bit) != 0;
+    if (!usable) {
+      int n = 0;
+      if (!coli_cuda_check(cudaGetDeviceCount(&n), "device count")) return;
+      usable = usable_device(device, n);
+      if (usable) __atomic_fetch_or(&seen, bit, __ATOMIC_RELEASE);
+    }
+    enter(device, usable);
   }
 };
 size_t type_size(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYPE_F16 || type == COLI_TYPE_BF16 ? 2 : 0; }
@@ -1235,7 +1259,7 @@ extern "C" int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_
     return 0;
   }
   if (!check_fp8_rows("quantize_rows_fp8", codes_dev, ld, scales_dev, s_row, s_blk, rows, K)) return 0;
-  OnDevice on(device);
+  OnAnyDevice on(device);
   if (!on.ok) return 0;
   colib::QuantRowsParams p = {};
   p.x = x_dev;
@@ -1336,7 +1360,7 @@ extern "C" int coli_b200_route_logits(int device, const void *logits_dev, int ty
     coli_set_error("route_logits: row stride %lld for %d experts, or a misaligned pointer", (long long)stride, E);
     return 0;
   }
-  OnDevice on(device);
+  OnAnyDevice on(device);
   if (!on.ok) return 0;
   if (T == 0) return coli_cuda_check(cudaMemsetAsync(expert_rows_dev, 0, sizeof(int32_t) * E, (cudaStream_t)stream), "count clear") ? 1 : 0;
   colib::RouteLogitsParams p = {};
