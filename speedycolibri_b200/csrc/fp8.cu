@@ -176,7 +176,6 @@ constexpr int F8_EPI_WARPS = 8;
 constexpr int F8_THREADS = (F8_EPI_WARPS + 4) * 32;  // (two warps stand by: registers are moved between whole warpgroups)
 // 168 registers a thread at launch are 64512; the summing warps take 208 of them each, the others keep 88: all of them.
 constexpr int F8_REGS_SUM = 208, F8_REGS_OTHER = 88;
-constexpr int F8_MAX_SPLIT = 4;  // CTAs that share a tile's k-tiles (clusters of 8 start late: 24 rows x 2048 x 2048 11.4 us, with 4 6.5)
 constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
 struct F8Maps {
   CUtensorMap m[F8_MAPS];
@@ -722,7 +721,9 @@ static int launch_f8_rows(const F8Maps &maps, const Fp8MmParams &p, int ar, int 
   if constexpr (BN == 256)
     if (ar == 32) return p.split > 1 ? launch_f8<GATED, BN, 32, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 32, false, OutT>(maps, p, grid, st);
   if (ar <= 64) return p.split > 1 ? launch_f8<GATED, BN, 64, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 64, false, OutT>(maps, p, grid, st);
-  return p.split > 1 ? launch_f8<GATED, BN, 128, true, OutT>(maps, p, grid, st) : launch_f8<GATED, BN, 128, false, OutT>(maps, p, grid, st);
+  if constexpr (!GATED)
+    if (p.split > 1) return launch_f8<false, BN, 128, true, OutT>(maps, p, grid, st);
+  return launch_f8<GATED, BN, 128, false, OutT>(maps, p, grid, st);
 }
 template <bool GATED, typename OutT>
 static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int ar, int grid, cudaStream_t st) {
@@ -730,13 +731,6 @@ static int launch_f8_shape(const F8Maps &maps, const Fp8MmParams &p, int bn, int
     if (bn == 128) return launch_f8_rows<false, 128, OutT>(maps, p, ar, grid, st);
   return launch_f8_rows<GATED, 256, OutT>(maps, p, ar, grid, st);
 }
-
-// Us a k-tile, for the ends of a tile, and for joining the sums of CTAs that share one: fitted to K 512 to 7168 on 64 to 148 CTAs.
-struct F8Shape {
-  int ar, bn;
-  double kt_us, end_us, join_us;
-};
-static const F8Shape F8_SHAPES[] = {{128, 256, 0.60, 3.3, 3.2}, {128, 128, 0.42, 1.7, 2.4}, {64, 256, 0.46, 1.9, 2.4}, {64, 128, 0.40, 0.9, 2.1}, {32, 256, 0.44, 1.7, 2.2}};
 
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   if (p.rows == 0 || p.nseg == 0) return 1;
@@ -749,33 +743,10 @@ int launch_fp8_mm(Fp8MmParams p, cudaStream_t st) {
   p.Op = round_up(p.O, 16);
   if (fp8_stream_ok(p)) return launch_fp8_stream(p, st);
   const bool gated = p.h_codes != nullptr;
-  // The tile and the CTAs that share one, all functions of the call's shapes alone: the cheapest of what was measured.  Experts'
-  // rows of a tile follow from their average segment (a tile passes the weights once more): 32 up to 20 rows, 64 up to 56, 128
-  // from there where their tiles fill the SMs.  Us a call, 128 / 64 rows: H 7168, I 2048, 32 experts, 53 rows each 274 / 249,
-  // 64 rows 279 / 312; H 2048, I 768, 64 experts, 64 rows 100 / 82, 94 rows 103 / 103; 64 / 32 rows: 32 experts, 19 rows 49.6 / 46.0.
-  const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
-  const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
-  const long full = ((mean + 127) / 128) * (segs > 0 ? segs : 1) * ((p.O + 127) / 128);
-  const int wanted = !p.seg_count ? 0 : mean <= 20 ? 32 : mean <= (p.KT > 32 ? 56 : 64) || full <= COLI_SMS ? 64 : 128;
-  int ar = 0, bn = 0, most = 0;
-  double best = 0.0;
-  for (const F8Shape &f : F8_SHAPES) {
-    if ((wanted && f.ar != wanted) || (gated && f.bn != 256)) continue;
-    const int fw = gated ? 128 : f.bn;
-    const int row_tiles = p.seg_count ? p.rows_expected / f.ar + segs : (p.rows + f.ar - 1) / f.ar;
-    const long tiles = (long)(row_tiles > 0 ? row_tiles : 1) * ((p.O + fw - 1) / fw);
-    for (int split = 1; split <= F8_MAX_SPLIT && split <= p.KT && (split == 1 || tiles * split <= COLI_SMS); split *= 2) {
-      const long rounds = (tiles * split + COLI_SMS - 1) / COLI_SMS;
-      const double us = rounds * ((p.KT + split - 1) / split * f.kt_us + f.end_us) + (split > 1 ? f.join_us : 0.0);
-      if (ar && us >= best) continue;
-      best = us;
-      ar = f.ar;
-      bn = f.bn;
-      p.split = split;
-      p.n_tiles = (p.O + fw - 1) / fw;
-      most = p.seg_count ? p.rows / ar + (p.rows < p.nseg ? p.rows : p.nseg) : row_tiles;
-    }
-  }
+  const Fp8Plan plan = fp8_plan(p);
+  const int ar = plan.ar, bn = plan.bn, most = plan.most;
+  p.split = plan.split;
+  p.n_tiles = plan.n_tiles;
   F8Maps maps;
   // One segment has full boxes and a last one; behind counts on the device any may come (an encoding takes 0.3 us).
   auto box_of = [](int n) {

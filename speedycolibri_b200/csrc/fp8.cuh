@@ -54,6 +54,49 @@ static inline bool fp8_stream_ok(const Fp8MmParams &p) {
   const int segs = p.rows_expected < p.nseg ? p.rows_expected : p.nseg;
   return p.rows_expected <= 2L * segs;
 }
+
+// How the tensor-memory kernel cuts a product, all functions of the call's shapes alone: the cheapest of what was measured.
+constexpr int F8_MAX_SPLIT = 4;  // CTAs that share a tile's k-tiles (clusters of 8 start late: 24 rows x 2048 x 2048 11.4 us, with 4 6.5)
+// Us a k-tile, for the ends of a tile, and for joining the sums of CTAs that share one: fitted to K 512 to 7168 on 64 to 148 CTAs.
+struct F8Shape {
+  int ar, bn;
+  double kt_us, end_us, join_us;
+};
+static const F8Shape F8_SHAPES[] = {{128, 256, 0.60, 3.3, 3.2}, {128, 128, 0.42, 1.7, 2.4}, {64, 256, 0.46, 1.9, 2.4}, {64, 128, 0.40, 0.9, 2.1}, {32, 256, 0.44, 1.7, 2.2}};
+
+struct Fp8Plan {
+  int ar, bn;   // rows and columns of a tile (gated: the columns are 128 features of gate and of up)
+  int split;    // CTAs that share a tile
+  int n_tiles;  // tiles over the features
+  int most;     // tiles over the rows, at most
+};
+// Experts' rows of a tile follow from their average segment (a tile passes the weights once more): 32 up to 20 rows, 64 up to 56, 128
+// from there where their tiles fill the SMs.  Us a call, 128 / 64 rows: H 7168, I 2048, 32 experts, 53 rows each 274 / 249,
+// 64 rows 279 / 312; H 2048, I 768, 64 experts, 64 rows 100 / 82, 94 rows 103 / 103; 64 / 32 rows: 32 experts, 19 rows 49.6 / 46.0.
+// (128-row tiles of gate and up are never shared: that they are taken says that there are more of them than SMs.)
+static inline Fp8Plan fp8_plan(const Fp8MmParams &p) {
+  const bool gated = p.h_codes != nullptr;
+  const int segs = p.seg_count ? (p.rows_expected < p.nseg ? p.rows_expected : p.nseg) : 1;
+  const long mean = p.seg_count ? ((long)p.rows_expected + segs - 1) / (segs > 0 ? segs : 1) : p.rows;
+  const long full = ((mean + 127) / 128) * (segs > 0 ? segs : 1) * ((p.O + 127) / 128);
+  const int wanted = !p.seg_count ? 0 : mean <= 20 ? 32 : mean <= (p.KT > 32 ? 56 : 64) || full <= COLI_SMS ? 64 : 128;
+  Fp8Plan plan = {};
+  double best = 0.0;
+  for (const F8Shape &f : F8_SHAPES) {
+    if ((wanted && f.ar != wanted) || (gated && f.bn != 256)) continue;
+    const int fw = gated ? 128 : f.bn;
+    const int row_tiles = p.seg_count ? p.rows_expected / f.ar + segs : (p.rows + f.ar - 1) / f.ar;
+    const long tiles = (long)(row_tiles > 0 ? row_tiles : 1) * ((p.O + fw - 1) / fw);
+    for (int split = 1; split <= F8_MAX_SPLIT && split <= p.KT && (split == 1 || tiles * split <= COLI_SMS); split *= 2) {
+      const long rounds = (tiles * split + COLI_SMS - 1) / COLI_SMS;
+      const double us = rounds * ((p.KT + split - 1) / split * f.kt_us + f.end_us) + (split > 1 ? f.join_us : 0.0);
+      if (plan.ar && us >= best) continue;
+      best = us;
+      plan = {f.ar, f.bn, split, (p.O + fw - 1) / fw, p.seg_count ? p.rows / f.ar + (p.rows < p.nseg ? p.rows : p.nseg) : row_tiles};
+    }
+  }
+  return plan;
+}
 int launch_fp8_mm(Fp8MmParams p, cudaStream_t st);
 int launch_fp8_stream(Fp8MmParams p, cudaStream_t st);  // called by launch_fp8_mm
 int *fp8_status_word();          // the library's own status word on the current device
