@@ -508,18 +508,19 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       for (int t = cluster0; t < n_tiles; t += clusters) {
         F8Info tile;
         recall(tile);
-        // (a second block past the end has no scales, and is not stored)
+        // (a second block past the end has no scales, and is not stored; a tile that was not waited for is not known: no address of it
+        // is used once a wait has given up)
         const float *sw = (lane & 1) == 0 ? tile.s0 : GATED ? tile.s1 : BN == 256 && tile.nt * BN + 128 < p.O ? tile.s0 + p.KT : tile.s0;
         const float *sx[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) sx[j] = p.sx + (long)(tile.row0 + min(lane + 32 * j, max(tile.nrows, 1) - 1)) * p.s_row;
         for (int kb = kb0; kb < kb1; kb += F8_CHUNK, ++it) {
           float x[F8_CHUNK][4];
-          const float w = lane < 2 * F8_CHUNK ? __ldg(sw + min(kb + (lane >> 1), kb1 - 1)) : 0.0f;
+          const float w = alive && lane < 2 * F8_CHUNK ? __ldg(sw + min(kb + (lane >> 1), kb1 - 1)) : 0.0f;
 #pragma unroll
           for (int u = 0; u < F8_CHUNK; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[u][j] = kb + u < kb1 ? __ldg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
+            for (int j = 0; j < 4; ++j) x[u][j] = alive && kb + u < kb1 ? __ldg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
           const uint32_t s = it & 1u, ph = (it >> 1) & 1u;
           alive = alive && __all_sync(0xffffffffu, mbar_wait(unscaled + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
           if (alive) {
