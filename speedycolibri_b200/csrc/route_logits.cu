@@ -282,14 +282,22 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
   const RlCand<uint32_t> c = {reinterpret_cast<uint32_t *>(cand), reinterpret_cast<int *>(cand + 256)};
   const bool softmax = p.score == COLI_SCORE_SOFTMAX;
   const bool scored = p.select_bias || p.logit_bias || p.n_group > 1;
+  if (softmax && p.logit_bias) return -1;  // (top and sum are wanted to 64 bits)
   float z[SLOTS];
   uint32_t key[SLOTS];
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) z[s] = lane + 32 * s < p.E ? (float)rl_load<T>(z0 + lane + 32 * s) : NEG_INF;
   if (p.logit_bias) {
+    // two finite values may leave f32: an expert that is open all the same
+    bool leaves = false;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s)
-      if (lane + 32 * s < p.E) z[s] += __ldg(p.logit_bias + lane + 32 * s);
+      if (lane + 32 * s < p.E) {
+        const float b = __ldg(p.logit_bias + lane + 32 * s), sum = z[s] + b;
+        leaves |= isinf(sum) && isfinite(z[s]) && isfinite(b);
+        z[s] = sum;
+      }
+    if (__any_sync(0xffffffffu, leaves)) return -1;
   }
   uint32_t top = 0u;
 #pragma unroll
@@ -302,8 +310,6 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
   if (top == 0u) return 0;  // every expert is closed
   const float m = rl_value32(top);
   if (softmax) {
-    // an infinite sum of z and its bias may be a rounded one
-    if (p.logit_bias && !(fabsf(m) <= 3.0e38f)) return -1;
     norm.top = (double)m;
     // (where the weights are divided by their own sum, and that holds the largest, the sum over all experts drops out)
     if (!p.norm_topk || scored) {
@@ -315,7 +321,6 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
   }
   float apart = 0.0f;  // how far two choices must lie apart
   if (scored) {
-    if (p.logit_bias && softmax) return -1;  // (top and sum are wanted to 64 bits)
     const float inv = softmax ? (float)(1.0 / norm.sum) : 0.0f;
     float choice[SLOTS], size = 0.0f, arg = 0.0f;
 #pragma unroll
