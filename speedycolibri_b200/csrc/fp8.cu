@@ -6,6 +6,8 @@
 //   product  y[r,o] = sum_b sx[r,b] * sw[o/128,b] * ( sum_{k in b} q[r,k] * qw[o,k] )
 //
 // (crates/colibri-engine/src/convert.rs:731-741 has the weights' half of it; the reference multiplies f32 activations.)
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "fp8_common.cuh"
 #include "tc_common.cuh"
@@ -66,6 +68,14 @@ __device__ __forceinline__ void qr_zero(__nv_bfloat162 &a) { a = __nv_bfloat162(
 __device__ __forceinline__ float2 qr_pair(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 __device__ __forceinline__ float2 qr_pair(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
+// a piece's values times 2^64, exactly
+__device__ __forceinline__ float qr_lift(float v) { return v * 18446744073709551616.0f; }
+__device__ __forceinline__ uint32_t qr_lift(uint32_t w, float) { return __float_as_uint(qr_lift(__uint_as_float(w))); }
+__device__ __forceinline__ uint32_t qr_lift(uint32_t w, __nv_bfloat16 t) {
+  const float2 v = qr_pair(w, t);
+  return __float_as_uint(qr_lift(v.x)) >> 16 | (__float_as_uint(qr_lift(v.y)) & 0xffff0000u);
+}
+
 template <typename T>
 struct QrMax {
   using type = float;
@@ -109,8 +119,21 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
         float a = qr_amax_out(m);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const float s = row_scale(a), y = __frcp_rn(s);
-        const float b = s <= 3.4028235e38f ? s : 0.0f;  // (x times the reciprocal of an infinite s as it is)
+        const float s = row_scale(a);
+        float d = s;
+        // The remainder of a quotient of 2^-10 (below it the code is 0) or more is exact while s is 2^-93 or more; smaller blocks are
+        // divided 2^64 times as large (16-bit floats have none: 2^-24 / 448)
+        if constexpr (!std::is_same<T, __half>::value) {
+          if (s < 8.0779356694631609e-28f) {  // 2^-90
+            d = qr_lift(s);
+#pragma unroll
+            for (int l = 0; l < P::LOADS; ++l) {
+              uint4 &q = now.q[j][l];
+              q = make_uint4(qr_lift(q.x, T()), qr_lift(q.y, T()), qr_lift(q.z, T()), qr_lift(q.w, T()));
+            }
+          }
+        }
+        const float y = __frcp_rn(d), b = d <= 3.4028235e38f ? d : 0.0f;  // (x times the reciprocal of an infinite s as it is)
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) {
           const int c = c0 + COLS * j + LANES * P::VEC * l;
