@@ -326,7 +326,8 @@ int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_type, int64
                                 int64_t s_blk, void *stream);
 /* y[r,o] = sum over blocks b of 128 columns of scale[r,b] * w_scale[o / 128, b] * (the product of the codes
  * over the block): rows in 8 bits times a resident weight of format 8, y_dev [rows, O] of y_type, y_stride
- * elements apart.  Products of codes are exact, sums are f32, each result is rounded once to y_type.  A
+ * elements apart.  Products of codes are exact, sums are f32, each result is rounded once to y_type.  Scales
+ * may be any f32: a row whose scale times a block's leaves f32's normal range is summed apart, slowly.  A
  * weight code of 0x7F or 0xFF is a NaN here (the 16-bit expert calls read it as 480).  The same call gives
  * the same bits; calls with another number of rows may share K among CTAs differently and differ in the
  * last f32 bits. */

@@ -320,9 +320,52 @@ __device__ __forceinline__ void f8_add_scaled(float2 &c, float x, float y, float
   asm("mov.b64 {%0, %1}, %2;" : "=f"(c.x), "=f"(c.y) : "l"(cc));
 }
 
+// Row `row` of tile t from its codes, for scales that the tile's sums do not hold (f8_ordinary).
+template <bool GATED, int BN, int AR>
+struct F8Row {
+  const uint8_t *codes, *q[2];
+  const float *sx, *sw[2];  // sw: of all blocks of the feature's weight
+  int f0;                   // the tile's first feature
+  __device__ __forceinline__ F8Row(const Fp8MmParams &p, const int *row_off, const int *tile_off, int t, int row) {
+    const F8Tile tile = f8_tile<AR>(tile_off, row_off, p.nseg, t);
+    const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+    const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
+    codes = (const uint8_t *)p.codes + (long)(tile.row0 + row) * p.ld;
+    sx = p.sx + (long)(tile.row0 + row) * p.s_row;
+    q[0] = w0.q;
+    q[1] = w1.q;
+    sw[0] = reinterpret_cast<const float *>(w0.s);
+    sw[1] = reinterpret_cast<const float *>(w1.s);
+    f0 = tile.nt * (GATED ? 128 : BN);
+  }
+  __device__ __forceinline__ bool asks(const Fp8MmParams &p) const {
+    const float *s0 = sw[0] + (size_t)(f0 >> 7) * p.KT;
+    return f8_again(sx, p.s_blk, s0, GATED ? sw[1] + (size_t)(f0 >> 7) * p.KT : BN == 256 && f0 + 128 < p.O ? s0 + p.KT : s0, 0, p.KT);
+  }
+  __device__ __forceinline__ float sum(const Fp8MmParams &p, int f, int up) const {
+    return f < p.O ? f8_sum_again(codes, sx, p.s_blk, p.K, q[up] + (size_t)f * 128, (size_t)p.Op * 128, f & 7, sw[up] + (size_t)(f >> 7) * p.KT, 0, p.KT) : 0.0f;
+  }
+};
+// Four neighbouring features of one row of h by each lane of a warp: its scale and codes.
+__device__ __forceinline__ void f8_store_h(const Fp8MmParams &p, const float (&g)[4], const float (&u)[4], long r, int nt, int lane) {
+  const int f = nt * 128 + 4 * lane;
+  float h[4], a = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = f + j < p.O ? coli_act_fast(g[j], u[j], p.act) : 0.0f;
+    a = fmaxf(a, fabsf(h[j]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
+  if (f < p.h_ld) *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)r * p.h_ld + f) = e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+  if (lane == 0) p.h_scales[(size_t)nt * p.rows + r] = s;
+}
+
 // One warp sums row i of the tile over the CTAs of the cluster and writes what becomes of it.
-template <bool GATED, int BN, typename OutT>
-__device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &tile, uint32_t red, int world, int i, int lane) {
+template <bool GATED, int BN, int AR, typename OutT>
+__device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &tile, const int *row_off, const int *tile_off, int t, uint32_t red, int world, int i,
+                                            int lane) {
   // (all CTAs' sums are requested before the first is added)
   float4 v[BN / 128], u[F8_MAX_SPLIT][BN / 128];
 #pragma unroll
@@ -342,20 +385,21 @@ __device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &
         v[j].z += u[r][j].z;
         v[j].w += u[r][j].w;
       }
-  if constexpr (GATED) {
-    const int f = tile.nt * 128 + 4 * lane;
-    const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-    float h[4], a = 0.0f;
+  const float first = __shfl_sync(0xffffffffu, v[0].x, 0);  // (columns behind the last feature hold anything)
+  if (first != first) {
+    const F8Row<GATED, BN, AR> row(p, row_off, tile_off, t, i);
+    if (row.asks(p)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h[j] = f + j < p.O ? coli_act_fast(g[j], u[j], p.act) : 0.0f;
-      a = fmaxf(a, fabsf(h[j]));
+      for (int j = 0; j < BN / 128; ++j) {
+        const int f = row.f0 + (GATED ? 0 : 128 * j) + 4 * lane;
+        v[j] = make_float4(row.sum(p, f, GATED ? j : 0), row.sum(p, f + 1, GATED ? j : 0), row.sum(p, f + 2, GATED ? j : 0), row.sum(p, f + 3, GATED ? j : 0));
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
-    if (f < p.h_ld) *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)(tile.row0 + i) * p.h_ld + f) = e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-    if (lane == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + i] = s;
+    __syncwarp();
+  }
+  if constexpr (GATED) {
+    const float g[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+    f8_store_h(p, g, u, tile.row0 + i, tile.nt, lane);
   } else {
 #pragma unroll
     for (int j = 0; j < BN / 128; ++j) {
@@ -544,6 +588,30 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
           for (int u = 0; u < F8_CHUNK; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[u][j] = alive && kb + u < kb1 ? __ldg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
+          // A row with a pair that is not f8_ordinary becomes NaN, and the summing warps look closer at those.  (The chunk's extremes first:
+          // the pairs one by one would make this warp the slowest.)
+          float most = fabsf(x[0][0]), least = most;
+#pragma unroll
+          for (int u = 0; u < F8_CHUNK; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              most = fmaxf(most, fabsf(x[u][j]));
+              least = fminf(least, kb + u < kb1 ? fabsf(x[u][j]) : least);
+            }
+          const uint32_t wbits = __float_as_uint(fabsf(w));
+          const float wmost = __uint_as_float(__reduce_max_sync(0xffffffffu, wbits)), wleast = __uint_as_float(__reduce_min_sync(0xffffffffu, lane < 2 * F8_CHUNK ? wbits : 0x7fffffffu));
+          if (!__all_sync(0xffffffffu, f8_ordinary(most, wmost) && f8_ordinary(least, wleast) && least > 0.0f && wleast > 0.0f)) {
+            bool again[4] = {};
+#pragma unroll
+            for (int u = 0; u < F8_CHUNK; ++u) {
+              const float w0 = __shfl_sync(0xffffffffu, w, 2 * u), w1 = __shfl_sync(0xffffffffu, w, 2 * u + 1);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) again[j] = again[j] || (kb + u < kb1 && (!f8_ordinary(x[u][j], w0) || !f8_ordinary(x[u][j], w1)));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (again[j]) x[0][j] = __uint_as_float(0x7fffffffu);
+          }
           const uint32_t s = it & 1u, ph = (it >> 1) & 1u;
           alive = alive && __all_sync(0xffffffffu, mbar_wait(unscaled + 8 * s, ph ^ 1u, abort_flag, status, TC_ERR_TMA_WAIT));
           if (alive) {
@@ -638,6 +706,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
       }
       float *flat = reinterpret_cast<float *>(acc);
       const bool mine = row < tile.nrows;
+      // a NaN: the row's own, or the scales' warp's (looked at once the sums are stored; columns behind the last feature hold anything)
+      const bool none = mine && alive && flat[0] != flat[0] && tile.nt * (GATED ? 128 : BN) + (GATED ? HF : NACC) * part < p.O;
       if constexpr (SPLIT) {
         // partial sums into the ring's place: its last copies have been multiplied
         float *red = reinterpret_cast<float *>(smem);
@@ -650,7 +720,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         }
         meet();
         alive = alive && !*abort_flag;
-        for (int i = (int)rank + world * warp; alive && i < tile.nrows; i += world * F8_EPI_WARPS) f8_join_row<GATED, BN, OutT>(p, tile, ring, world, i, lane);
+        for (int i = (int)rank + world * warp; alive && i < tile.nrows; i += world * F8_EPI_WARPS) f8_join_row<GATED, BN, AR, OutT>(p, tile, row_off, tile_off, t, ring, world, i, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring is copied into again
         meet();
       } else if constexpr (GATED) {
@@ -671,7 +741,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) a = fmaxf(a, am[i * AR]);
         const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
-        if (mine && alive) {
+        const bool again = none && F8Row<GATED, BN, AR>(p, row_off, tile_off, t, row).asks(p);  // (every share of the row sees it)
+        if (mine && alive && !again) {
           uint8_t *dst = p.h_codes + (size_t)(tile.row0 + row) * p.h_ld + f0;
 #pragma unroll
           for (int c = 0; c < HF / 16; ++c) {
@@ -683,11 +754,30 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
           }
           if (part == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
         }
+        for (uint32_t left = part == 0 ? __ballot_sync(0xffffffffu, again) : 0u; left; left &= left - 1u) {
+          const int r = r0 + __ffs(left) - 1;
+          const F8Row<GATED, BN, AR> one(p, row_off, tile_off, t, r);
+          float g[4], u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            g[j] = one.sum(p, one.f0 + 4 * lane + j, 0);
+            u[j] = one.sum(p, one.f0 + 4 * lane + j, 1);
+          }
+          __syncwarp();
+          f8_store_h(p, g, u, tile.row0 + r, tile.nt, lane);
+        }
       } else {
         const int f = tile.nt * BN + part * NACC;
         if (any && alive && f < p.O)
           f8_store_rows<OutT, NACC>(smem + S::RING + warp * 32 * F8_OUT_LD, (OutT *)p.y + (long)(tile.row0 + r0) * p.y_stride + f, p.y_stride, flat,
                                     tile.nrows - r0, p.O - f, p.y_vec, lane);
+        for (uint32_t left = __ballot_sync(0xffffffffu, none); left; left &= left - 1u) {
+          const int r = r0 + __ffs(left) - 1;
+          const F8Row<GATED, BN, AR> one(p, row_off, tile_off, t, r);
+          if (!one.asks(p)) continue;
+          for (int i = lane; i < NACC && f + i < p.O; i += 32) ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f + i] = f8_out<OutT>(one.sum(p, f + i, 0));
+        }
+        __syncwarp();
       }
       if (t + clusters < n_tiles) recall(tile);
     }

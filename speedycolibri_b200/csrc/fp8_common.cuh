@@ -28,6 +28,63 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) { return e4m3x2(a, b) | (e4m3x2(c, d) << 16); }
 
+// The two scales of a k-tile are any f32.  They are multiplied with each other first, which is right while the product is a normal number
+// (or one of them is 0): outside, scale x scale x sum may be one all the same (1e-38 and 1e-6 leave three bits of the product, 1e36
+// and 1e5 none, and a sum of 0 becomes NaN).  A row with such a pair is summed again, by f8_sum_again: a branch among the additions, or
+// one shared-memory read more a k-tile, costs every call 5 to 15 % (4096 x 7168 x 4096: 149.5 -> 157.7 and 170.7 us).
+__device__ __forceinline__ bool f8_ordinary(float x, float w) {
+  const float product = fabsf(x * w);
+  return (product >= 1.17549435e-38f && product <= 3.4028235e38f) || x == 0.0f || w == 0.0f;
+}
+// sum * x * w, however far apart: factors of 2^64 keep what is on the way in range
+__device__ __forceinline__ float f8_scaled(float sum, float x, float w) {
+  if (f8_ordinary(x, w) || !(fabsf(x) <= 3.4028235e38f && fabsf(w) <= 3.4028235e38f)) return sum * (x * w);
+  constexpr float UP = 18446744073709551616.0f, DOWN = 1.0f / UP;
+  return fabsf(x * w) < 1.0f ? sum * ((x * UP) * (w * UP)) * DOWN * DOWN : sum * ((x * DOWN) * (w * DOWN)) * UP * UP;
+}
+// Whether a row has such a pair in k-tiles kb0 .. kb1 - 1, with either of two blocks of features
+__device__ __forceinline__ bool f8_again(const float *sx, long s_blk, const float *sw0, const float *sw1, int kb0, int kb1) {
+  bool again = false;
+#pragma unroll 1
+  for (int kb = kb0; kb < kb1; ++kb) again = again || !f8_ordinary(sx[kb * s_blk], sw0[kb]) || !f8_ordinary(sx[kb * s_blk], sw1[kb]);
+  return again;
+}
+// One result over k-tiles kb0 .. kb1 - 1, code by code: the row's codes, and the feature's, whose k-tiles lie w_step bytes apart
+// (feature f, f & 7 = f7, with its chunks permuted).  Slow, and reached only by rows with scales as above.
+static __device__ __noinline__ float f8_sum_again(const uint8_t *codes, const float *sx, long s_blk, int K, const uint8_t *w, size_t w_step, int f7,
+                                                  const float *sw, int kb0, int kb1) {
+  auto pair = [](uint32_t two) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  };
+  float y = 0.0f;
+  for (int kb = kb0; kb < kb1; ++kb) {
+    float sum = 0.0f;
+#pragma unroll 2
+    for (int c = 0; c < 8; ++c) {
+      const int k = kb * 128 + c * 16;
+      uint32_t a[4] = {};
+      if (k + 16 <= K) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(codes + k);
+        a[0] = q.x, a[1] = q.y, a[2] = q.z, a[3] = q.w;
+      } else {  // (nothing behind a row's last code is read)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a[i >> 2] |= (k + i < K ? (uint32_t)codes[k + i] : 0u) << (8 * (i & 3));
+      }
+      const uint4 q = *reinterpret_cast<const uint4 *>(w + kb * w_step + (size_t)((c ^ f7) << 4));
+      const uint32_t b[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 u = pair(a[i >> 1] >> (16 * (i & 1))), v = pair(b[i >> 1] >> (16 * (i & 1)));
+        sum = fmaf(u.y, v.y, fmaf(u.x, v.x, sum));
+      }
+    }
+    y += f8_scaled(sum, sx[kb * s_blk], sw[kb]);
+  }
+  return y;
+}
+
 // `bytes` (a multiple of 16) in a row, global -> shared memory, counted by the barrier
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)

@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
     const F8Tile tile = f8_tile<FS_ROWS>(tile_off, row_off, p.nseg, task);
     const int f0 = tile.nt * (GATED ? 16 : 16 * M);
     float acc[M][4] = {};
+    float least = 1.0f;  // product of scales so far (one that is too large shows in the sums)
     for (int kt = kt0; kt < kt1; ++kt, ++used) {
       alive = alive && __all_sync(0xffffffffu, mbar_wait(bar + 8u * (uint32_t)slot, phase, abort_flag, status, TC_ERR_TMA_WAIT));
       const uint32_t unit = ring + (uint32_t)slot * S::UNIT, c0 = (uint32_t)(t ^ g) * 16, c1 = (uint32_t)((t + 4) ^ g) * 16;
@@ -200,6 +201,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
         mma_e4m3(d, a0.w, a1.w, a2.w, a3.w, lo.w, hi.w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(d[i], sx[i & 1] * sw, acc[m][i]);
+        if (m == 0 || GATED) least = fminf(least, fminf(fabsf(sx[0] * sw), fabsf(sx[1] * sw)));
       }
       if (++slot == depth) {
         slot = 0;
@@ -208,6 +210,20 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
       __syncwarp();  // the slot has been read
       if (alive && issued < n_units) issue();
     }
+    if (alive && !(least >= 1.17549435e-38f)) {
+      // too small a product, or a scale of 0: NaN where it asks for a closer look at the end
+      const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+      const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
+      const size_t sw = (size_t)(f0 >> 7) * p.KT;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (f8_again(p.sx + (long)(tile.row0 + min(2 * t + j, tile.nrows - 1)) * p.s_row, p.s_blk, reinterpret_cast<const float *>(w0.s) + sw,
+                     reinterpret_cast<const float *>(w1.s) + sw, kt0, kt1)) {
+#pragma unroll
+          for (int m = 0; m < M; ++m) acc[m][j] = acc[m][j + 2] = __uint_as_float(0x7fffffffu);
+        }
+    }
+    __syncwarp();
     if (ks > 1) {
       // join the sums of the warps that share the task, in their order
       constexpr int N = M * 4;
@@ -226,21 +242,49 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(ks * 32) : "memory");
     }
     if (sub == 0 && alive) {
+      auto store = [&](int r, int m, int f, float v) {
+        if constexpr (GATED)
+          p.h32[(long)(tile.row0 + r) * p.O + f] = v;
+        else
+          ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f + 16 * m] = f8_out<OutT>(v);
+      };
+      bool look = false;
+#pragma unroll
+      for (int i = 0; i < 4 * M; ++i) look = look || !(fabsf(acc[i / 4][i % 4]) <= 3.4028235e38f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 2 * t + (i & 1);
+        const int r = 2 * t + (i & 1), f = f0 + g + 8 * (i >> 1);
         if (r >= tile.nrows) continue;
         if constexpr (GATED) {
-          const int f = f0 + g + 8 * (i >> 1);
-          if (f < p.O) p.h32[(long)(tile.row0 + r) * p.O + f] = coli_act_fast(acc[0][i], acc[1][i], p.act);
+          if (f < p.O) store(r, 0, f, coli_act_fast(acc[0][i], acc[1][i], p.act));
         } else {
 #pragma unroll
-          for (int m = 0; m < M; ++m) {
-            const int f = f0 + 16 * m + g + 8 * (i >> 1);
-            if (f < p.O) ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f] = f8_out<OutT>(acc[m][i]);
+          for (int m = 0; m < M; ++m)
+            if (f + 16 * m < p.O) store(r, m, f, acc[m][i]);
+        }
+      }
+      if (look) {
+        // a sum is infinite or none: where scales whose product is no normal number are the reason, the lane's results from their codes
+        const int ex = p.seg_expert ? p.seg_expert[tile.seg] : tile.seg;
+        const WeightRef w0 = p.w0 ? p.w0[ex] : p.one, w1 = GATED ? p.w1[ex] : w0;
+        const size_t sw = (size_t)(f0 >> 7) * p.KT;
+        const float *s0 = reinterpret_cast<const float *>(w0.s) + sw, *s1 = reinterpret_cast<const float *>(w1.s) + sw;
+#pragma unroll 1
+        for (int r = 2 * t; r < min(2 * t + 2, tile.nrows); ++r) {
+          const uint8_t *q = (const uint8_t *)p.codes + (long)(tile.row0 + r) * p.ld;
+          const float *sr = p.sx + (long)(tile.row0 + r) * p.s_row;
+          if (!f8_again(sr, p.s_blk, s0, s1, 0, p.KT)) continue;
+          auto sum = [&](const uint8_t *w, const float *s, int f) {
+            return f8_sum_again(q, sr, p.s_blk, p.K, w + (size_t)f * 128, (size_t)p.Op * 128, f & 7, s, 0, p.KT);
+          };
+#pragma unroll 1
+          for (int f = f0 + g; f < min(f0 + (GATED ? 16 : 16 * M), p.O); f += 8) {
+            const float v = sum(w0.q, s0, f);
+            store(r, 0, f, GATED ? coli_act_fast(v, sum(w1.q, s1, f), p.act) : v);
           }
         }
       }
+      __syncwarp();
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");  // (none are left unless a wait gave up)
