@@ -286,8 +286,7 @@ int coli_b200_moe_experts_dev(ColiMoe *moe, const void *rows_dev, const int32_t 
 /* The same experts in 8-bit arithmetic (handles of format 8 only; the calls of "8-bit rows" below make
  * the rows): codes_dev / scales_dev are expert-contiguous rows of H columns, seg_count_dev[n_local] the
  * rows of each resident expert (counts that run past rows_cap are cut there).  h = act(gate x, up x) is
- * quantised again, one scale per row and 128 features, by the rule of coli_b200_quantize_rows_fp8 (with a
- * rounded reciprocal of the scale where 128 features are made at once); both
+ * quantised again, one scale per row and 128 features, by the rule of coli_b200_quantize_rows_fp8; both
  * products are those of coli_b200_matmul_fp8_dev; y_dev is bf16 [rows, H] (16-byte aligned), written
  * for the rows of the segments only: what lies behind the last one stays as it was.  rows_expected
  * only selects how the work is cut, as above.  Uses the handle's workspace like the call above; the first

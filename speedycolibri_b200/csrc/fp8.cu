@@ -69,7 +69,7 @@ __device__ __forceinline__ float2 qr_pair(uint32_t w, __half) { return __half22f
 __device__ __forceinline__ float2 qr_pair(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 // a piece's values times 2^64, exactly
-__device__ __forceinline__ float qr_lift(float v) { return v * 18446744073709551616.0f; }
+__device__ __forceinline__ float qr_lift(float v) { return v * RowDivisor::UP; }
 __device__ __forceinline__ uint32_t qr_lift(uint32_t w, float) { return __float_as_uint(qr_lift(__uint_as_float(w))); }
 __device__ __forceinline__ uint32_t qr_lift(uint32_t w, __nv_bfloat16 t) {
   const float2 v = qr_pair(w, t);
@@ -119,13 +119,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
         float a = qr_amax_out(m);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const float s = row_scale(a);
-        float d = s;
-        // The remainder of a quotient of 2^-10 (below it the code is 0) or more is exact while s is 2^-93 or more; smaller blocks are
-        // divided 2^64 times as large (16-bit floats have none: 2^-24 / 448)
-        if constexpr (!std::is_same<T, __half>::value) {
-          if (s < 8.0779356694631609e-28f) {  // 2^-90
-            d = qr_lift(s);
+        const RowDivisor by(row_scale(a));
+        if constexpr (!std::is_same<T, __half>::value) {  // (16-bit floats have no such blocks: 2^-24 / 448)
+          if (by.up != 1.0f) {
 #pragma unroll
             for (int l = 0; l < P::LOADS; ++l) {
               uint4 &q = now.q[j][l];
@@ -133,25 +129,24 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
             }
           }
         }
-        const float y = __frcp_rn(d), b = d <= 3.4028235e38f ? d : 0.0f;  // (x times the reciprocal of an infinite s as it is)
 #pragma unroll
         for (int l = 0; l < P::LOADS; ++l) {
           const int c = c0 + COLS * j + LANES * P::VEC * l;
           const uint4 q = now.q[j][l];
           uint8_t *dst = p.codes + (size_t)r * p.ld + c;
           if constexpr (sizeof(T) == 4) {
-            const uint32_t w = e4m3x4(quotient(__uint_as_float(q.x), b, y), quotient(__uint_as_float(q.y), b, y),
-                                      quotient(__uint_as_float(q.z), b, y), quotient(__uint_as_float(q.w), b, y));
+            const uint32_t w = e4m3x4(by(__uint_as_float(q.x)), by(__uint_as_float(q.y)),
+                                      by(__uint_as_float(q.z)), by(__uint_as_float(q.w)));
             if (c < kp) *reinterpret_cast<uint32_t *>(dst) = w;
           } else {
             const float2 v0 = qr_pair(q.x, T()), v1 = qr_pair(q.y, T()), v2 = qr_pair(q.z, T()), v3 = qr_pair(q.w, T());
-            const uint2 w = make_uint2(e4m3x4(quotient(v0.x, b, y), quotient(v0.y, b, y), quotient(v1.x, b, y), quotient(v1.y, b, y)),
-                                       e4m3x4(quotient(v2.x, b, y), quotient(v2.y, b, y), quotient(v3.x, b, y), quotient(v3.y, b, y)));
+            const uint2 w = make_uint2(e4m3x4(by(v0.x), by(v0.y), by(v1.x), by(v1.y)),
+                                       e4m3x4(by(v2.x), by(v2.y), by(v3.x), by(v3.y)));
             if (c < kp) *reinterpret_cast<uint2 *>(dst) = w;
           }
         }
         const int block = (c0 + COLS * j) >> 7;
-        if (sub == 0 && block * 128 < p.K) p.scales[r * p.s_row + (long)block * p.s_blk] = s;
+        if (sub == 0 && block * 128 < p.K) p.scales[r * p.s_row + (long)block * p.s_blk] = by.scale;
       }
     }
     now = next;
@@ -357,9 +352,9 @@ __device__ __forceinline__ void f8_store_h(const Fp8MmParams &p, const float (&g
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
-  if (f < p.h_ld) *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)r * p.h_ld + f) = e4m3x4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-  if (lane == 0) p.h_scales[(size_t)nt * p.rows + r] = s;
+  const RowDivisor by(row_scale(a));
+  if (f < p.h_ld) *reinterpret_cast<uint32_t *>(p.h_codes + (size_t)r * p.h_ld + f) = e4m3x4(by(h[0] * by.up), by(h[1] * by.up), by(h[2] * by.up), by(h[3] * by.up));
+  if (lane == 0) p.h_scales[(size_t)nt * p.rows + r] = by.scale;
 }
 
 // One warp sums row i of the tile over the CTAs of the cluster and writes what becomes of it.
@@ -740,7 +735,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         asm volatile("bar.sync 1, %0;" ::"n"(F8_EPI_WARPS * 32) : "memory");
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) a = fmaxf(a, am[i * AR]);
-        const float s = row_scale(a), inv = __fdiv_rn(1.0f, s);
+        const RowDivisor by(row_scale(a));
+        if (__any_sync(0xffffffffu, by.up != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < HF; ++i) flat[i] *= by.up;
+        }
         const bool again = none && F8Row<GATED, BN, AR>(p, row_off, tile_off, t, row).asks(p);  // (every share of the row sees it)
         if (mine && alive && !again) {
           uint8_t *dst = p.h_codes + (size_t)(tile.row0 + row) * p.h_ld + f0;
@@ -749,10 +748,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = e4m3x4(flat[16 * c + 4 * i] * inv, flat[16 * c + 4 * i + 1] * inv, flat[16 * c + 4 * i + 2] * inv, flat[16 * c + 4 * i + 3] * inv);
+              w[i] = e4m3x4(by(flat[16 * c + 4 * i]), by(flat[16 * c + 4 * i + 1]), by(flat[16 * c + 4 * i + 2]), by(flat[16 * c + 4 * i + 3]));
             if (f0 + 16 * c < p.h_ld) reinterpret_cast<uint4 *>(dst)[c] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (part == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = s;
+          if (part == 0) p.h_scales[(size_t)tile.nt * p.rows + tile.row0 + row] = by.scale;
         }
         for (uint32_t left = part == 0 ? __ballot_sync(0xffffffffu, again) : 0u; left; left &= left - 1u) {
           const int r = r0 + __ffs(left) - 1;

@@ -21,6 +21,21 @@ __device__ __forceinline__ float row_scale(float a) {
     return a > 0.0f ? fmaxf(__fdiv_rn(a, 448.0f), TINY) : 1.0f;
   return s;
 }
+// Quotients by a block's scale.  The remainder of one of 2^-10 (below it the code is 0) or more is exact while the scale is 2^-93 or more:
+// smaller blocks are divided 2^64 times as large, `up`, by which the caller multiplies.  Values by an infinite scale are their products
+// with 0.
+struct RowDivisor {
+  static constexpr float UP = 18446744073709551616.0f;  // 2^64
+  float scale, up, b, y;
+  __device__ __forceinline__ explicit RowDivisor(float s) : scale(s) {
+    const bool tiny = s < 8.0779356694631609e-28f;  // 2^-90
+    up = tiny ? UP : 1.0f;
+    const float d = s * up;
+    y = __frcp_rn(d);
+    b = d <= 3.4028235e38f ? d : 0.0f;
+  }
+  __device__ __forceinline__ float operator()(float v) const { return quotient(v, b, y); }
+};
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t d;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
