@@ -31,20 +31,38 @@ struct QrPieces {
   static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 128 / LANES / VEC, COLS = 32 / LANES * 128, STEPS = QR_COLS / COLS;
   uint4 q[STEPS][LOADS];
 };
+// Rows and tokens (and in the products the rows' scales) are an earlier launch's results, which may be written while this one is already
+// resident: no constants.  The quantiser's loads may pass its own stores all the same, which the language's would not (4096 rows
+// gathered eight times 85.2 -> 91.4 us), but not the wait: their pointers are taken behind it.
+template <typename P>
+__device__ __forceinline__ const P *behind_wait(const P *p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+__device__ __forceinline__ uint4 qr_load16(const void *p) {
+  uint4 v;
+  asm("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int qr_load4(const int32_t *p) {
+  int v;
+  asm("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
 template <typename T, int LANES, bool WHOLE>
-__device__ __forceinline__ void qr_request(QrPieces<T, LANES> &d, const QuantRowsParams &p, int src, int c0) {
+__device__ __forceinline__ void qr_request(QrPieces<T, LANES> &d, const QuantRowsParams &p, const T *rows, int src, int c0) {
   using P = QrPieces<T, LANES>;
   constexpr int VEC = P::VEC, STEPS = P::STEPS, COLS = P::COLS;
-  const T *x = (const T *)p.x + (long)src * p.x_stride;
+  const T *x = rows + (long)src * p.x_stride;
 #pragma unroll
   for (int j = 0; j < STEPS; ++j)
 #pragma unroll
     for (int l = 0; l < P::LOADS; ++l) {
       const int c = c0 + COLS * j + LANES * VEC * l;
       if constexpr (WHOLE) {
-        d.q[j][l] = c < p.K ? __ldg(reinterpret_cast<const uint4 *>(x + c)) : make_uint4(0u, 0u, 0u, 0u);
+        d.q[j][l] = c < p.K ? qr_load16(x + c) : make_uint4(0u, 0u, 0u, 0u);
       } else if (p.x_vec && c + VEC <= p.K) {
-        d.q[j][l] = __ldg(reinterpret_cast<const uint4 *>(x + c));
+        d.q[j][l] = qr_load16(x + c);
       } else {
         alignas(16) T raw[VEC];
 #pragma unroll
@@ -94,21 +112,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
   using P = QrPieces<T, LANES>;
   constexpr int STEPS = P::STEPS, COLS = P::COLS;
   coli_grid_dependency_sync();
+  const T *x = behind_wait((const T *)p.x);
+  const int32_t *tokens = behind_wait(p.row_token);
   const int kp = (p.K + 15) & ~15;
   const int lane = threadIdx.x & 31, sub = lane % LANES;
   const int c0 = blockIdx.y * QR_COLS + lane / LANES * 128 + sub * P::VEC;
   const int step = gridDim.x * 8;
   const int rows = p.rows_used ? min(p.rows, *p.rows_used) : p.rows;
   // source of a row; outside [0, T): none
-  auto source = [&](long r) { return r < rows ? (p.row_token ? __ldg(p.row_token + r) : (int)r) : -1; };
+  auto source = [&](long r) { return r < rows ? (tokens ? qr_load4(tokens + r) : (int)r) : -1; };
   auto valid = [&](int src) { return (unsigned)src < (unsigned)p.T; };
   long r = blockIdx.x * 8 + (threadIdx.x >> 5);
   P now, next;
   int src = source(r), src_next = source(r + step);
-  if (valid(src)) qr_request<T, LANES, WHOLE>(now, p, src, c0);
+  if (valid(src)) qr_request<T, LANES, WHOLE>(now, p, x, src, c0);
   for (; r < rows; r += step) {
     const int src_after = source(r + 2 * (long)step);
-    if (valid(src_next)) qr_request<T, LANES, WHOLE>(next, p, src_next, c0);
+    if (valid(src_next)) qr_request<T, LANES, WHOLE>(next, p, x, src_next, c0);
     if (valid(src)) {  // (no token: the row is left as it was)
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
@@ -582,7 +602,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
 #pragma unroll
           for (int u = 0; u < F8_CHUNK; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[u][j] = alive && kb + u < kb1 ? __ldg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
+            for (int j = 0; j < 4; ++j) x[u][j] = alive && kb + u < kb1 ? __ldcg(sx[j] + (long)(kb + u) * p.s_blk) : 0.0f;
           // A row with a pair that is not f8_ordinary becomes NaN, and the summing warps look closer at those.  (The chunk's extremes first:
           // the pairs one by one would make this warp the slowest.)
           float most = fabsf(x[0][0]), least = most;

@@ -12,14 +12,15 @@ constexpr int RL_MAX_WARPS = 32;
 // per warp: keys of the candidates, their ids
 constexpr int RL_CAND_BYTES = 32 * (8 + 4);
 
+// Ordinary loads, of the biases too: an earlier launch may write them while this one is already resident, so that they are no constants.
 template <typename T>
 __device__ __forceinline__ double rl_load(const T *p);
 template <>
-__device__ __forceinline__ double rl_load<float>(const float *p) { return (double)__ldg(p); }
+__device__ __forceinline__ double rl_load<float>(const float *p) { return (double)*p; }
 template <>
-__device__ __forceinline__ double rl_load<__half>(const __half *p) { return (double)__half2float(__ldg(p)); }
+__device__ __forceinline__ double rl_load<__half>(const __half *p) { return (double)__half2float(*p); }
 template <>
-__device__ __forceinline__ double rl_load<__nv_bfloat16>(const __nv_bfloat16 *p) { return (double)__bfloat162float(__ldg(p)); }
+__device__ __forceinline__ double rl_load<__nv_bfloat16>(const __nv_bfloat16 *p) { return (double)__bfloat162float(*p); }
 
 // order-preserving key of a value above -inf (never 0); 0 for what cannot be chosen
 __device__ __forceinline__ uint64_t rl_key(double v) {
@@ -220,7 +221,7 @@ struct RlNorm {
 template <typename T>
 __device__ __forceinline__ double rl_z(const RouteLogitsParams &p, const T *z0, int e) {
   const double z = rl_load<T>(z0 + e);
-  return p.logit_bias ? z + (double)__ldg(p.logit_bias + e) : z;
+  return p.logit_bias ? z + (double)p.logit_bias[e] : z;
 }
 // (a largest logit of infinity shares the mass with its equals)
 __device__ __forceinline__ double rl_over(double z, double top) { return z == top ? 1.0 : rl_exp(z - top); }
@@ -264,7 +265,7 @@ __device__ __noinline__ RlNorm rl_choose64(const RouteLogitsParams &p, const T *
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int e = lane + 32 * s;
-    if (p.select_bias && e < p.E) score[s] += (double)__ldg(p.select_bias + e);
+    if (p.select_bias && e < p.E) score[s] += (double)p.select_bias[e];
     key[s] = key[s] && score[s] > NEG_INF ? rl_key(score[s]) : 0;
   }
   if (p.n_group > 1) rl_groups<SLOTS, uint64_t, double>(p, key, score, NEG_INF, row, reinterpret_cast<double *>(cand), lane);
@@ -293,7 +294,7 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s)
       if (lane + 32 * s < p.E) {
-        const float b = __ldg(p.logit_bias + lane + 32 * s), sum = z[s] + b;
+        const float b = p.logit_bias[lane + 32 * s], sum = z[s] + b;
         leaves |= isinf(sum) && isfinite(z[s]) && isfinite(b);
         z[s] = sum;
       }
@@ -327,7 +328,7 @@ __device__ __forceinline__ int rl_choose32(const RouteLogitsParams &p, const T *
     for (int s = 0; s < SLOTS; ++s) {
       const int e = lane + 32 * s;
       choice[s] = softmax ? (z[s] == m ? 1.0f : __expf(z[s] - m)) * inv : __fdividef(1.0f, 1.0f + __expf(fminf(-z[s], 80.0f)));
-      if (p.select_bias && e < p.E) choice[s] += __ldg(p.select_bias + e);
+      if (p.select_bias && e < p.E) choice[s] += p.select_bias[e];
       if (key[s]) key[s] = choice[s] > NEG_INF ? rl_key32(choice[s]) : 0u;
       if (key[s]) {
         size = fmaxf(size, fabsf(choice[s]));
