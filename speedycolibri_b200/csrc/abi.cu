@@ -1250,8 +1250,8 @@ extern "C" int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_
                                            int T, int rows, int K, void *codes_dev, int64_t ld, float *scales_dev, int64_t s_row,
                                            int64_t s_blk, void *stream) {
   const size_t es = type_size(x_type);
-  if (T < 0 || K < 1 || K > INT32_MAX - 256 || es == 0 || (rows > 0 && T > 0 && !x_dev) || (!row_token_dev && rows > T)) {
-    coli_set_error("quantize_rows_fp8: bad shape or type (T=%d rows=%d K=%d type=%d) or null pointer", T, rows, K, x_type);
+  if (T < 0 || K < 1 || K > colib::QR_MOST_COLS || es == 0 || (rows > 0 && T > 0 && !x_dev) || (!row_token_dev && rows > T)) {
+    coli_set_error("quantize_rows_fp8: bad shape or type (T=%d rows=%d K=%d of at most %d, type=%d) or null pointer", T, rows, K, colib::QR_MOST_COLS, x_type);
     return 0;
   }
   if (x_stride < 0 || !aligned_to(x_dev, es) || !aligned_to(row_token_dev, 4)) {

@@ -25,7 +25,6 @@ namespace colib {
 // stored half a sector at a time, keep eight (5000 rows of 1111 f16 11.0 us, with four 16.4).  WHOLE: gathered rows of whole pieces,
 // which the L2 has as a rule and the instructions bound, are read without a branch per piece (the gathered rows 92.0 -> 83.8 us);
 // rows as they are come faster from HBM with the branches, 108.7 against 131.
-constexpr int QR_COLS = 1024;
 template <typename T, int LANES>
 struct QrPieces {
   static constexpr int VEC = 16 / (int)sizeof(T), LOADS = 128 / LANES / VEC, COLS = 32 / LANES * 128, STEPS = QR_COLS / COLS;
@@ -178,10 +177,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) k_quant_rows(Quan
 int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
   if (p.rows == 0) return 1;
   const int chunks = (p.K + QR_COLS - 1) / QR_COLS;
-  if (chunks > 65535) {
-    coli_set_error("row quantiser: %d columns (at most %d)", p.K, 65535 * QR_COLS);
-    return 0;
-  }
   // CTAs that fit the SMs at once go through the rows
   const int fit = COLI_SMS * (p.type == COLI_TYPE_F32 ? 2 : 4), groups = (p.rows + 7) / 8;
   const int each = fit / chunks > 0 ? fit / chunks : 1;

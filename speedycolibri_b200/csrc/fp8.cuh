@@ -17,6 +17,8 @@ struct QuantRowsParams {
   float *scales;             // scale of (row, block) at row * s_row + block * s_blk
   long s_row, s_blk;
 };
+constexpr int QR_COLS = 1024;  // columns of a row that a warp takes; the rest of the row lies along the grid's second axis
+constexpr int QR_MOST_COLS = 65535 * QR_COLS;
 int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st);
 
 struct Fp8MmParams {

@@ -1,0 +1,15 @@
+"""Arguments of the 8-bit row and routing calls that were cut or written over one another, refused before anything is launched."""
+from tests.test_fp8_refusals_cpu import A, B, S, bind
+
+
+def quantise(fake, rows, K, sr, sb):
+    fake.fake_reset(0)
+    ld = (K + 15) // 16 * 16
+    return fake.coli_b200_quantize_rows_fp8(0, A, 2, K, None, rows, rows, K, B, ld, S, sr, sb, None), fake.fake_queued()
+
+
+def test_columns(fake_cuda):
+    fake, most = bind(fake_cuda), 65535 * 1024
+    assert quantise(fake, 1, most, 0, 1) == (1, 1)
+    for K in (most + 1, 2**31 - 1100, 2**31 - 300, 2**31 - 256, 2**31 - 1):  # (the grid's columns of these pass 32 bits)
+        assert quantise(fake, 1, K, 0, 1) == (0, 0), K
