@@ -315,7 +315,8 @@ int coli_b200_moe_finish_dev(ColiMoe *moe, const float *partial_dev, const void 
  *
  * Quantises rows x_dev of x_type (COLI_TYPE_*), x_stride elements apart: row r of the result is row r of
  * x (rows <= T), or with row_token_dev [rows] row row_token_dev[r] of it; an entry outside [0,T) is no
- * row, and its codes and scales are left as they were.  K is at most 65535 * 1024.  With a = the largest magnitude of the block's
+ * row, and its codes and scales are left as they were.  K is at most 65535 * 1024; strides that put two scales in one place
+ * are refused.  With a = the largest magnitude of the block's
  * non-NaN values: scale = 1 if a == 0, else max(a / 448, 2^-126); code = e4m3(x / scale), to nearest
  * even, saturating.  (The quotient is rounded once, where coli_b200_quantize_fp8_b128 multiplies by
  * a rounded reciprocal.)  A NaN keeps a NaN code and an infinity makes its block's scale infinite, so that

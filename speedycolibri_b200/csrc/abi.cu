@@ -7,6 +7,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <numeric>
 #include <vector>
 
 #include "fp8.cuh"
@@ -1228,6 +1229,12 @@ struct OnAnyDevice : OnDevice {
 };
 size_t type_size(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYPE_F16 || type == COLI_TYPE_BF16 ? 2 : 0; }
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// Whether two of m x n results at multiples of the strides a and b (not negative) fall on one place: the smallest shifts
+// that cancel are b / g along a's axis and a / g along b's.
+bool overlap(int64_t a, int64_t m, int64_t b, int64_t n) {
+  const int64_t g = std::gcd(a, b);
+  return g == 0 ? m * n > 1 : b / g < m && a / g < n;
+}
 // Codes are copied by TMA (16-byte rows), scales read one by one.
 bool check_fp8_rows(const char *who, const void *codes, int64_t ld, const float *scales, int64_t s_row, int64_t s_blk, int rows, int K) {
   if (rows < 0 || rows > 1 << 30 || (rows > 0 && (!codes || !scales))) {  // (tables add a tile's rows to them)
@@ -1259,6 +1266,10 @@ extern "C" int coli_b200_quantize_rows_fp8(int device, const void *x_dev, int x_
     return 0;
   }
   if (!check_fp8_rows("quantize_rows_fp8", codes_dev, ld, scales_dev, s_row, s_blk, rows, K)) return 0;
+  if (overlap(s_row, rows, s_blk, (K + 127) / 128)) {
+    coli_set_error("quantize_rows_fp8: two scales in one place (%d rows %lld apart, %d blocks %lld apart)", rows, (long long)s_row, (K + 127) / 128, (long long)s_blk);
+    return 0;
+  }
   OnAnyDevice on(device);
   if (!on.ok) return 0;
   colib::QuantRowsParams p = {};
