@@ -248,7 +248,8 @@ def quantize_rows_fp8_dev(x, row_token=None, out=None, stream=None):
     """coli_b200_quantize_rows_fp8: rows of x (f32, f16 or bf16 [T,K] on the GPU, any row stride) -> (codes u8 [R,K],
     scales f32 [R, ceil(K/128)]), on the current torch stream or on `stream` (a raw handle); `init` need not come first.  With `row_token` (int32 [R]) row r is x[row_token[r]]; an entry
     outside [0,T) leaves the row as it was (uninitialised without `out`).  Fresh results have rows of codes that start on 16
-    bytes and a block's scales next to each other; `out` = (codes, scales) are written in place whatever their strides."""
+    bytes and a block's scales next to each other; `out` = (codes, scales) are written in place whatever their strides, and
+    the bytes behind a row's K codes become zero up to a multiple of 16, whatever they hold."""
     if stream is not None and x.is_cuda:
         with _on(stream, x.device):
             return quantize_rows_fp8_dev(x, row_token, out)
@@ -325,7 +326,7 @@ class Routing(NamedTuple):
 
 def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=None, logit_bias=None, norm_topk: bool = False,
                      routed_scale: float = 1.0, n_group: int = 1, topk_group: int = 1, out=None, stream=None) -> Routing:
-    """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, any row stride) -> Routing, on the current torch
+    """coli_b200_route_logits: router logits (f32, f16 or bf16 [T,E] on the GPU, rows E or more apart) -> Routing, on the current torch
     stream or on `stream`; `init` need not come first.  Biases are f32 [E]; -inf and NaN logits close an expert to a token; `out` is a Routing whose tensors are
     written in place."""
     if stream is not None and logits.is_cuda:
@@ -338,6 +339,8 @@ def route_logits_dev(logits, k: int, score: int = SCORE_SOFTMAX, select_bias=Non
     T, E = shape
     if T > 1 << 20 or E > 512:
         raise ValueError(f"route_logits_dev: logits [{T}, {E}] (T <= 2^20, E <= 512)")
+    if not -(1 << 31) < min(k, score, n_group, topk_group) <= max(k, score, n_group, topk_group) < 1 << 31:  # (before ctypes cuts them)
+        raise ValueError(f"route_logits_dev: k={k}, score={score}, n_group={n_group} or topk_group={topk_group} is past 32 bits")
     for name, b in (("select_bias", select_bias), ("logit_bias", logit_bias)):
         if b is not None and (b.dtype != th.f32 or b.numel() != E or not b.is_contiguous()):
             raise ValueError(f"route_logits_dev: {name} must be contiguous f32 [{E}]")

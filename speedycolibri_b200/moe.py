@@ -234,7 +234,7 @@ class MoeBlock:
         if device != self.device:
             raise ValueError(f"experts_fp8_dev: the handle is on cuda:{self.device}, the rows on cuda:{device}")
         if not _lib_().coli_b200_moe_experts_fp8_dev(self.handle, codes.data_ptr(), ld, scales.data_ptr(), s_row, s_blk, seg_count.data_ptr(), R,
-                                                     rows_expected, y.data_ptr(), th.stream(device) if stream is None else stream):
+                                                     max(-1, min(rows_expected, R)), y.data_ptr(), th.stream(device) if stream is None else stream):
             _check(0, "coli_b200_moe_experts_fp8_dev")
 
     def shared_dev(self, x, y, stream):

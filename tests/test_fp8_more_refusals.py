@@ -1,4 +1,6 @@
 """Arguments of the 8-bit row and routing calls that were cut or written over one another, refused before anything is launched."""
+import pytest
+
 from tests.test_fp8_refusals_cpu import A, B, S, bind
 
 
@@ -23,3 +25,26 @@ def test_scales_in_one_place(fake_cuda):
         assert quantise(fake, rows, K, sr, sb) == ((1, 1) if fits else (0, 0)), (rows, K, sr, sb)
     for rows, K, sr, sb in ((5, 300, 0, 1), (5, 300, 1, 0), (5, 300, 0, 0), (5, 300, 1, 1), (5, 300, 1, 4), (2, 300, 1, 1), (5, 128, 0, 1)):
         assert quantise(fake, rows, K, sr, sb) == (0, 0), (rows, K, sr, sb)
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits_in_python(gpu_backend):
+    import torch
+
+    from tests.test_gpu_fp8_rows import expert_layer, rows
+
+    z = torch.zeros((4, 16), device="cuda")
+    for kw in (dict(k=2**32 + 1), dict(k=2, n_group=2**32 + 1), dict(k=2, topk_group=2**32 + 1), dict(k=2, score=2**32), dict(k=2, n_group=-(2**32) + 1)):
+        with pytest.raises(ValueError):
+            gpu_backend.route_logits_dev(z, **kw)
+    block, _ = expert_layer(gpu_backend, 2, 128, 64, 40)
+    q, s = gpu_backend.quantize_rows_fp8_dev(rows(40, 128, 1))
+    seg, y = torch.tensor([20, 20], dtype=torch.int32, device="cuda"), [torch.empty((40, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    block.experts_fp8_dev(q, s, seg, 40, y[0])
+    block.experts_fp8_dev(q, s, seg, 2**32, y[1])  # more than there are rows: the rows there are
+    assert torch.equal(*y)
+    with pytest.raises(gpu_backend.CudaError):
+        block.experts_fp8_dev(q, s, seg, -(2**32), y[0])
+    with pytest.raises(gpu_backend.CudaError):
+        gpu_backend.quantize_rows_fp8_dev(rows(4, 256, 1), out=(q[:4].new_empty((4, 256)), s.new_empty((4, 1)).expand(4, 2)))
+    block.close()
