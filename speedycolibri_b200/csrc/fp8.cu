@@ -348,12 +348,13 @@ struct F8Row {
     sw[1] = reinterpret_cast<const float *>(w1.s);
     f0 = tile.nt * (GATED ? 128 : BN);
   }
-  __device__ __forceinline__ bool asks(const Fp8MmParams &p) const {
+  __device__ __forceinline__ bool asks(const Fp8MmParams &p, int first = 0, int step = 1) const {
     const float *s0 = sw[0] + (size_t)(f0 >> 7) * p.KT;
-    return f8_again(sx, p.s_blk, s0, GATED ? sw[1] + (size_t)(f0 >> 7) * p.KT : BN == 256 && f0 + 128 < p.O ? s0 + p.KT : s0, 0, p.KT);
+    return f8_again(sx, p.s_blk, s0, GATED ? sw[1] + (size_t)(f0 >> 7) * p.KT : BN == 256 && f0 + 128 < p.O ? s0 + p.KT : s0, first, p.KT, step);
   }
+  __device__ __forceinline__ bool warp_asks(const Fp8MmParams &p, int lane) const { return __any_sync(0xffffffffu, asks(p, lane, 32)); }
   __device__ __forceinline__ float sum(const Fp8MmParams &p, int f, int up) const {
-    return f < p.O ? f8_sum_again(codes, sx, p.s_blk, p.K, q[up] + (size_t)f * 128, (size_t)p.Op * 128, f & 7, sw[up] + (size_t)(f >> 7) * p.KT, 0, p.KT) : 0.0f;
+    return f < p.O ? f8_sum_again<8>(codes, sx, p.s_blk, p.K, q[up] + (size_t)f * 128, (size_t)p.Op * 128, f & 7, sw[up] + (size_t)(f >> 7) * p.KT, 0, p.KT) : 0.0f;
   }
 };
 // Four neighbouring features of one row of h by each lane of a warp: its scale and codes.
@@ -398,7 +399,7 @@ __device__ __forceinline__ void f8_join_row(const Fp8MmParams &p, const F8Info &
   const float first = __shfl_sync(0xffffffffu, v[0].x, 0);  // (columns behind the last feature hold anything)
   if (first != first) {
     const F8Row<GATED, BN, AR> row(p, row_off, tile_off, t, i);
-    if (row.asks(p)) {
+    if (row.warp_asks(p, lane)) {
 #pragma unroll
       for (int j = 0; j < BN / 128; ++j) {
         const int f = row.f0 + (GATED ? 0 : 128 * j) + 4 * lane;
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
             }
           const uint32_t wbits = __float_as_uint(fabsf(w));
           const float wmost = __uint_as_float(__reduce_max_sync(0xffffffffu, wbits)), wleast = __uint_as_float(__reduce_min_sync(0xffffffffu, lane < 2 * F8_CHUNK ? wbits : 0x7fffffffu));
-          if (!__all_sync(0xffffffffu, f8_ordinary(most, wmost) && f8_ordinary(least, wleast) && least > 0.0f && wleast > 0.0f)) {
+          if (!__all_sync(0xffffffffu, f8_normal(most * wmost) && f8_normal(least * wleast))) {
             bool again[4] = {};
 #pragma unroll
             for (int u = 0; u < F8_CHUNK; ++u) {
@@ -788,7 +789,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         for (uint32_t left = __ballot_sync(0xffffffffu, none); left; left &= left - 1u) {
           const int r = r0 + __ffs(left) - 1;
           const F8Row<GATED, BN, AR> one(p, row_off, tile_off, t, r);
-          if (!one.asks(p)) continue;
+          if (!one.warp_asks(p, lane)) continue;
           for (int i = lane; i < NACC && f + i < p.O; i += 32) ((OutT *)p.y)[(long)(tile.row0 + r) * p.y_stride + f + i] = f8_out<OutT>(one.sum(p, f + i, 0));
         }
         __syncwarp();

@@ -47,25 +47,29 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 // (or one of them is 0): outside, scale x scale x sum may be one all the same (1e-38 and 1e-6 leave three bits of the product, 1e36
 // and 1e5 none, and a sum of 0 becomes NaN).  A row with such a pair is summed again, by f8_sum_again: a branch among the additions, or
 // one shared-memory read more a k-tile, costs every call 5 to 15 % (4096 x 7168 x 4096: 149.5 -> 157.7 and 170.7 us).
+__device__ __forceinline__ bool f8_normal(float product) { return fabsf(product) >= 1.17549435e-38f && fabsf(product) <= 3.4028235e38f; }
+// (an infinite scale or none gives the same either way)
 __device__ __forceinline__ bool f8_ordinary(float x, float w) {
-  const float product = fabsf(x * w);
-  return (product >= 1.17549435e-38f && product <= 3.4028235e38f) || x == 0.0f || w == 0.0f;
+  return f8_normal(x * w) || x == 0.0f || w == 0.0f || !(fabsf(x) <= 3.4028235e38f && fabsf(w) <= 3.4028235e38f);
 }
 // sum * x * w, however far apart: factors of 2^64 keep what is on the way in range
 __device__ __forceinline__ float f8_scaled(float sum, float x, float w) {
-  if (f8_ordinary(x, w) || !(fabsf(x) <= 3.4028235e38f && fabsf(w) <= 3.4028235e38f)) return sum * (x * w);
+  if (f8_ordinary(x, w)) return sum * (x * w);
   constexpr float UP = 18446744073709551616.0f, DOWN = 1.0f / UP;
   return fabsf(x * w) < 1.0f ? sum * ((x * UP) * (w * UP)) * DOWN * DOWN : sum * ((x * DOWN) * (w * DOWN)) * UP * UP;
 }
-// Whether a row has such a pair in k-tiles kb0 .. kb1 - 1, with either of two blocks of features
-__device__ __forceinline__ bool f8_again(const float *sx, long s_blk, const float *sw0, const float *sw1, int kb0, int kb1) {
+// Whether a row has such a pair in k-tiles kb0, kb0 + step .. kb1 - 1, with either of two blocks of features
+__device__ __forceinline__ bool f8_again(const float *sx, long s_blk, const float *sw0, const float *sw1, int kb0, int kb1, int step = 1) {
   bool again = false;
 #pragma unroll 1
-  for (int kb = kb0; kb < kb1; ++kb) again = again || !f8_ordinary(sx[kb * s_blk], sw0[kb]) || !f8_ordinary(sx[kb * s_blk], sw1[kb]);
+  for (int kb = kb0; kb < kb1; kb += step) again = again || !f8_ordinary(sx[kb * s_blk], sw0[kb]) || !f8_ordinary(sx[kb * s_blk], sw1[kb]);
   return again;
 }
 // One result over k-tiles kb0 .. kb1 - 1, code by code: the row's codes, and the feature's, whose k-tiles lie w_step bytes apart
-// (feature f, f & 7 = f7, with its chunks permuted).  Slow, and reached only by rows with scales as above.
+// (feature f, f & 7 = f7, with its chunks permuted).  Slow, and reached only by rows with scales as above; AHEAD chunks of 16 codes are
+// requested at once, as many as the caller's registers allow.  (All rows of 4096 x 7168 x 4096: 37.6 ms, 9 ms a tile of 128 x 256, in
+// which the tile's other warps wait; they would give up after 0.3 s, at a K of some 200000.)
+template <int AHEAD>
 static __device__ __noinline__ float f8_sum_again(const uint8_t *codes, const float *sx, long s_blk, int K, const uint8_t *w, size_t w_step, int f7,
                                                   const float *sw, int kb0, int kb1) {
   auto pair = [](uint32_t two) {
@@ -76,23 +80,33 @@ static __device__ __noinline__ float f8_sum_again(const uint8_t *codes, const fl
   float y = 0.0f;
   for (int kb = kb0; kb < kb1; ++kb) {
     float sum = 0.0f;
-#pragma unroll 2
-    for (int c = 0; c < 8; ++c) {
-      const int k = kb * 128 + c * 16;
-      uint32_t a[4] = {};
-      if (k + 16 <= K) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(codes + k);
-        a[0] = q.x, a[1] = q.y, a[2] = q.z, a[3] = q.w;
-      } else {  // (nothing behind a row's last code is read)
+#pragma unroll 1
+    for (int c0 = 0; c0 < 8; c0 += AHEAD) {
+      uint4 a[AHEAD], b[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) a[i >> 2] |= (k + i < K ? (uint32_t)codes[k + i] : 0u) << (8 * (i & 3));
+      for (int c = 0; c < AHEAD; ++c) {
+        const int k = kb * 128 + (c0 + c) * 16;
+        a[c] = k + 16 <= K ? *reinterpret_cast<const uint4 *>(codes + k) : make_uint4(0u, 0u, 0u, 0u);
+        b[c] = *reinterpret_cast<const uint4 *>(w + kb * w_step + (size_t)(((c0 + c) ^ f7) << 4));
       }
-      const uint4 q = *reinterpret_cast<const uint4 *>(w + kb * w_step + (size_t)((c ^ f7) << 4));
-      const uint32_t b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 u = pair(a[i >> 1] >> (16 * (i & 1))), v = pair(b[i >> 1] >> (16 * (i & 1)));
-        sum = fmaf(u.y, v.y, fmaf(u.x, v.x, sum));
+      for (int c = 0; c < AHEAD; ++c) {
+        const int k = kb * 128 + (c0 + c) * 16;
+        uint32_t row[4] = {a[c].x, a[c].y, a[c].z, a[c].w};
+        const uint32_t col[4] = {b[c].x, b[c].y, b[c].z, b[c].w};
+        if (k < K && k + 16 > K)  // (nothing behind a row's last code is read)
+          for (int i = 0; k + i < K; ++i) {
+            const uint32_t code = (uint32_t)codes[k + i] << (8 * (i & 3));
+            row[0] |= i < 4 ? code : 0u;
+            row[1] |= i >= 4 && i < 8 ? code : 0u;
+            row[2] |= i >= 8 && i < 12 ? code : 0u;
+            row[3] |= i >= 12 ? code : 0u;
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 u = pair(row[i >> 1] >> (16 * (i & 1))), v = pair(col[i >> 1] >> (16 * (i & 1)));
+          sum = fmaf(u.y, v.y, fmaf(u.x, v.x, sum));
+        }
       }
     }
     y += f8_scaled(sum, sx[kb * s_blk], sw[kb]);

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(FS_THREADS, 1) k_fp8_stream(const __grid_const
           const float *sr = p.sx + (long)(tile.row0 + r) * p.s_row;
           if (!f8_again(sr, p.s_blk, s0, s1, 0, p.KT)) continue;
           auto sum = [&](const uint8_t *w, const float *s, int f) {
-            return f8_sum_again(q, sr, p.s_blk, p.K, w + (size_t)f * 128, (size_t)p.Op * 128, f & 7, s, 0, p.KT);
+            return f8_sum_again<1>(q, sr, p.s_blk, p.K, w + (size_t)f * 128, (size_t)p.Op * 128, f & 7, s, 0, p.KT);
           };
 #pragma unroll 1
           for (int f = f0 + g; f < min(f0 + (GATED ? 16 : 16 * M), p.O); f += 8) {
