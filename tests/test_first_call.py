@@ -52,3 +52,28 @@ def test_before_initialisation_on_the_gpu(quantise):
     r = subprocess.run([sys.executable, "-c", PROGRAM.format(quantise=quantise)], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True,
                        text=True, timeout=240)
     assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
+
+
+CAPTURED = """
+import torch
+from speedycolibri_b200 import backend
+x, z = torch.randn((33, 300), device="cuda"), torch.randn((3000, 64), device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    first = [*backend.quantize_rows_fp8_dev(x), *backend.route_logits_dev(z, 4)]
+g.replay()
+then = [*backend.quantize_rows_fp8_dev(x), *backend.route_logits_dev(z, 4)]
+assert all(torch.equal(a, b) for a, b in zip(first, then))
+print("equal")
+"""
+
+
+@pytest.mark.gpu
+def test_captured_first_calls():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    r = subprocess.run([sys.executable, "-c", CAPTURED], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]
