@@ -1,6 +1,7 @@
 // Host side of libcoli_b200.so: the extern "C" entry points declared in include/coli_b200.h.
 // Lifecycle, resident-weight handles, the whole-block call and its stages, and the reference's
 // host-pointer expert calls expressed through the same kernels.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -1085,9 +1086,11 @@ extern "C" int coli_b200_moe_gather_local_dev(ColiMoe *m, const void *x_dev, con
   return colib::launch_permute(pp, st);
 }
 
-// scratch of a grouped-FFN run grows on demand (synchronises the device when it does)
+// scratch of a grouped-FFN run grows on demand (synchronises the device when it does), by half at least: the blocks that calls
+// of rising sizes leave behind are together no more than three times the last one
 static bool ensure_h(ColiMoe *m, SegScratch &sc, size_t rows) {
   if (rows <= sc.h_rows) return true;
+  rows = std::max(rows, sc.h_rows + sc.h_rows / 2);
   if (!coli_cuda_check(cudaDeviceSynchronize(), "scratch regrow sync")) return false;
   __half *nh = nullptr;
   if (!coli_cuda_check(cudaMalloc((void **)&nh, rows * m->L.I * sizeof(__half)), "scratch regrow")) return false;
