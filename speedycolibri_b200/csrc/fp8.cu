@@ -23,7 +23,8 @@ namespace colib {
 // halve what a block's scale costs (32768 gathered rows of 7168 bf16 99.7 -> 90.4 us before WHOLE, with eight lanes and two quotients an
 // instruction; rows as they are 112 -> 108.5, 6.5 TB/s); values read one by one, off the 16-byte grid, and f32, whose codes would be
 // stored half a sector at a time, keep eight (5000 rows of 1111 f16 11.0 us, with four 16.4).  WHOLE: gathered rows of whole pieces,
-// which the L2 has as a rule and the instructions bound, are read without a branch per piece (the gathered rows 92.0 -> 83.8 us);
+// which the L2 has as a rule and the instructions bound, are read without a branch per piece (the gathered rows 92.0 -> 83.8 us,
+// and 85.3 since tiny blocks are told apart);
 // rows as they are come faster from HBM with the branches, 108.7 against 131.
 template <typename T, int LANES>
 struct QrPieces {
@@ -201,12 +202,12 @@ int launch_quant_rows(const QuantRowsParams &p, cudaStream_t st) {
 // The scales are arbitrary f32, which the block-scaled MMA kinds do not take.  Four more warps copy, issue the products, look
 // up the next tiles and bring the scales: whatever waits for memory in the summing warps is added to every k-tile.
 // What bounds it: with short segments the weights' bytes; with long ones the hand-overs between products and sums, 1170 cycles
-// a k-tile of 128 x 256 whose products take 512 (4096 rows x 7168 x 4096: 154 us, 1560 TFLOP/s, tensor pipe 38 % active;
+// a k-tile of 128 x 256 whose products take 512 (4096 rows x 7168 x 4096: 154 us, 1560 TFLOP/s, tensor pipe 39 % active;
 // loads of the next k-tile always on their way across its end: 187 us), and in calls of many such tiles power (1.5 GHz at
-// 1000 W; 8192 rows on 64 experts, H 7168, I 2048: 805 us, 896 TFLOP/s of products without their padding).
+// 1000 W; 8192 rows on 64 experts, H 7168, I 2048: 806 us, 895 TFLOP/s of products without their padding).
 constexpr int F8_BM = 128;
 constexpr int F8_EPI_WARPS = 8;
-constexpr int F8_THREADS = (F8_EPI_WARPS + 4) * 32;  // (two warps stand by: registers are moved between whole warpgroups)
+constexpr int F8_THREADS = (F8_EPI_WARPS + 4) * 32;  // (registers are moved between whole warpgroups: four other warps, a role each)
 // 168 registers a thread at launch are 64512; the summing warps take 208 of them each, the others keep 88: all of them.
 constexpr int F8_REGS_SUM = 208, F8_REGS_OTHER = 88;
 constexpr int F8_MAPS = 5;  // boxes of 8, 16, 32, 64 and 128 rows
@@ -686,8 +687,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) k_fp8_mm(const __grid_constant_
         tc_fence_after();
         if (any && alive) {
           // FLY loads of 16 columns at a time, the next ones requested as each is added, so that the buffer goes back to the
-          // products after few round trips (with 64 columns on their way the sums no longer fit the registers); two sums an
-          // instruction.
+          // products after few round trips (48 columns on their way beside 128 sums leave 8 bytes of addresses a thread in memory, 64 would
+          // leave sums); two sums an instruction.
           constexpr int CH = NACC / 16, FLY = CH == 8 ? 3 : CH;
           uint32_t v[FLY][16];
           auto column = [&](int c) { return tbase + d * BN + (uint32_t)(GATED ? (c < CH / 2 ? HF * part + 16 * c : 128 + HF * part + 16 * (c - CH / 2)) : part * NACC + 16 * c); };
